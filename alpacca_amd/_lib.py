@@ -69,11 +69,32 @@ SIGNATURES = {
     "aq_greedy_advance": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _vp]),
     "aq_greedy_advance_penalized": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64,
                                            ctypes.c_double, _i32, _vp]),
+    "aq_logits_adjust": (_i32, [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64,
+                                _vp, _vp]),
+    "aq_kv8_sizes": (_i32, [_i32, _i32, _i64, _c.POINTER(_sz), _c.POINTER(_sz),
+                            _c.POINTER(_sz), _c.POINTER(_sz)]),
+    "aq_rope_kv8": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp,
+                           _vp]),
+    "aq_attention_kv8": (_i32, [_vp, _vp, _i64, _i32, _vp, _i64, _vp, _vp]),
+    "aq_attention_rope_kv8": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp,
+                                     _vp, _vp]),
+    "aq_kv8_read": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
     "aq_stream_read": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp]),
 }
 
 # sizeof(aq_decode_state): int64 token, uint64 key, int32 pos/fed/count/done
 DECODE_STATE_BYTES = 32
+
+
+
+class KV8(ctypes.Structure):
+    """aq_kv8: the arrays and the shape of one layer's 8-bit KV cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("k_tail", ctypes.c_void_p),
+                ("v_tail", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+                ("n_ctx", ctypes.c_int64), ("n_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
 
 _lib = None
 _lock = threading.Lock()

@@ -1226,3 +1226,149 @@ int aq_greedy_advance_penalized(const float *logits, int64_t n, aq_decode_state 
 }
 
 }  // extern "C"
+
+// ---- 8-bit KV cache -----------------------------------------------------------
+
+namespace {
+int kv8_check(const aq_kv8 *c) {
+  if (!c) return fail(AQ_ERR_VALUE, "cache is NULL");
+  if (c->n_kv <= 0 || c->n_ctx <= 0 || c->n_ctx > INT32_MAX)
+    return fail(AQ_ERR_VALUE, "bad cache shape (n_kv %d, n_ctx %lld)", c->n_kv,
+                (long long)c->n_ctx);
+  if (!aq::kv8_supported(c->head_dim))
+    return fail(AQ_ERR_VALUE, "the 8-bit cache takes head_dim 64, 128 or 256 (got %d)",
+                c->head_dim);
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_tail || !c->v_tail || !c->scratch)
+    return fail(AQ_ERR_VALUE, "NULL array in the cache");
+  if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_tail | (uintptr_t)c->v_tail |
+       (uintptr_t)c->scratch) % 16)
+    return fail(AQ_ERR_VALUE, "the cache's codes, tails and scratch must be 16-byte aligned");
+  return AQ_OK;
+}
+
+int kv8_heads_check(const aq_kv8 *c, int n_head) {
+  if (n_head <= 0 || n_head % c->n_kv || n_head / c->n_kv > 16)
+    return fail(AQ_ERR_VALUE, "bad attention shape (n_head %d, n_kv %d): groups of 1 to 16",
+                n_head, c->n_kv);
+  return AQ_OK;
+}
+
+int kv8_span_check(const aq_kv8 *c, const aq_decode_state *state, int64_t pos0, int64_t T) {
+  if (!state && (pos0 < 0 || pos0 > c->n_ctx || T > c->n_ctx - pos0))
+    return fail(AQ_ERR_VALUE, "positions %lld..%lld outside the cache of %lld",
+                (long long)pos0, (long long)(pos0 + T - 1), (long long)c->n_ctx);
+  return AQ_OK;
+}
+
+int kv8_rope_check(const aq_kv8 *c, int n_rot, const float *cos_tab, const float *sin_tab) {
+  if (n_rot < 0 || n_rot > c->head_dim || n_rot % 2)
+    return fail(AQ_ERR_VALUE, "n_rot %d must be even and <= head_dim %d", n_rot, c->head_dim);
+  if (n_rot && (!cos_tab || !sin_tab)) return fail(AQ_ERR_VALUE, "NULL rotation table");
+  return AQ_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *scales,
+                 size_t *tail, size_t *scratch) {
+  if (n_kv <= 0 || n_ctx <= 0 || n_ctx > INT32_MAX || !aq::kv8_supported(head_dim))
+    return fail(AQ_ERR_VALUE, "bad cache shape (n_kv %d, head_dim %d, n_ctx %lld)", n_kv,
+                head_dim, (long long)n_ctx);
+  const size_t blocks = (size_t)n_kv * ((n_ctx + aq::kKv8Block - 1) / aq::kKv8Block);
+  if (codes) *codes = blocks * aq::kKv8Block * head_dim;
+  if (scales) *scales = blocks * sizeof(float);
+  if (tail) *tail = (size_t)n_kv * aq::kKv8Block * head_dim * sizeof(float);
+  if (scratch) *scratch = aq::kv8_scratch_bytes(head_dim);
+  return AQ_OK;
+}
+
+int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, int64_t T,
+                int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
+                const aq_decode_state *state, int64_t pos0, const aq_kv8 *cache, void *stream) {
+  if (int rc = kv8_check(cache)) return rc;
+  if (T < 0) return fail(AQ_ERR_VALUE, "negative token count");
+  if (int rc = kv8_rope_check(cache, n_rot, cos_tab, sin_tab)) return rc;
+  if (q && n_head <= 0) return fail(AQ_ERR_VALUE, "bad n_head %d", n_head);
+  if (T && (!k || !v || (q && !q_out))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_span_check(cache, state, pos0, T)) return rc;
+  if (T == 0) return AQ_OK;
+  if (T > cache->n_ctx || T / aq::kKv8Block * cache->n_kv > ((int64_t)1 << 28))
+    return fail(AQ_ERR_VALUE, "%lld tokens are too many for one call", (long long)T);
+  hipError_t e = aq::launch_rope_kv8(q, k, v, q_out, T, n_head, n_rot, neox ? 1 : 0, cos_tab,
+                                     sin_tab, state, pos0, *cache,
+                                     static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "8-bit cache store launch");
+}
+
+int aq_attention_kv8(const float *q, const aq_kv8 *cache, int64_t T, int n_head,
+                     const aq_decode_state *state, int64_t pos0, float *out, void *stream) {
+  if (int rc = kv8_check(cache)) return rc;
+  if (T < 0) return fail(AQ_ERR_VALUE, "negative token count");
+  if (int rc = kv8_heads_check(cache, n_head)) return rc;
+  if (T > 65535) return fail(AQ_ERR_VALUE, "at most 65535 query tokens per call");
+  if (T && (!q || !out)) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_span_check(cache, state, pos0, T)) return rc;
+  if (T == 0) return AQ_OK;
+  hipError_t e = aq::launch_attention_kv8(q, *cache, T, n_head, state, pos0, out,
+                                          static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "8-bit cache attention launch");
+}
+
+int aq_attention_rope_kv8(const float *q, const float *k, const float *v, int n_head, int n_rot,
+                          int neox, const float *cos_tab, const float *sin_tab,
+                          const aq_decode_state *state, int64_t pos0, const aq_kv8 *cache,
+                          float *out, void *stream) {
+  if (int rc = kv8_check(cache)) return rc;
+  if (int rc = kv8_heads_check(cache, n_head)) return rc;
+  if (int rc = kv8_rope_check(cache, n_rot, cos_tab, sin_tab)) return rc;
+  if (neox && n_rot % 8)
+    return fail(AQ_ERR_VALUE, "fused rope needs n_rot a multiple of 8 for neox, got %d", n_rot);
+  if (!q || !k || !v || !out) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_span_check(cache, state, pos0, 1)) return rc;
+  hipError_t e = aq::launch_attention_rope_kv8(q, k, v, n_head, n_rot, neox ? 1 : 0, cos_tab,
+                                               sin_tab, state, pos0, *cache, out,
+                                               static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "8-bit cache attention launch");
+}
+
+int aq_kv8_read(const aq_kv8 *cache, int64_t start, int64_t n, float *k, float *v, void *stream) {
+  if (int rc = kv8_check(cache)) return rc;
+  if (n < 0 || start < 0 || start > cache->n_ctx || n > cache->n_ctx - start)
+    return fail(AQ_ERR_VALUE, "positions %lld..%lld outside the cache of %lld", (long long)start,
+                (long long)(start + n - 1), (long long)cache->n_ctx);
+  if (n && (!k || !v)) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (n == 0) return AQ_OK;
+  hipError_t e = aq::launch_kv8_read(*cache, start, n, k, v, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "8-bit cache read launch");
+}
+
+// ---- adjustment of logits --------------------------------------------------------
+
+int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t *window,
+                     int64_t last_n, const double *penalties, const int64_t *bias_ids,
+                     const float *bias, const int64_t *bias_off, int64_t n_bias,
+                     const uint32_t *mask, int64_t mask_ld, float *out, void *stream) {
+  if (rows < 0 || n < 0 || n_bias < 0) return fail(AQ_ERR_VALUE, "negative shape");
+  if (rows > 65535) return fail(AQ_ERR_VALUE, "at most 65535 rows per call");
+  if (n > 0xFFFFFFFFll || n_bias > 0xFFFFFFFEll) return fail(AQ_ERR_VALUE, "too many logits or biases");
+  if (!window != !penalties)
+    return fail(AQ_ERR_VALUE, "window and penalties come together or not at all");
+  if (window && last_n < 1) return fail(AQ_ERR_VALUE, "last_n must be >= 1");
+  if (n_bias && (!bias_ids || !bias)) return fail(AQ_ERR_VALUE, "NULL bias list");
+  const int64_t words = (n + 31) / 32;
+  if (mask && mask_ld != 0 && mask_ld < words)
+    return fail(AQ_ERR_VALUE, "mask rows of %lld words hold fewer than %lld tokens",
+                (long long)mask_ld, (long long)n);
+  if (rows == 0 || n == 0) return AQ_OK;
+  if (!logits || !out) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  const uintptr_t a = (uintptr_t)logits, b = (uintptr_t)out, bytes = (uintptr_t)rows * n * 4;
+  if (a != b && a < b + bytes && b < a + bytes)
+    return fail(AQ_ERR_VALUE, "out overlaps logits without being it");
+  hipError_t e = aq::launch_logits_adjust(logits, rows, n, window, last_n, penalties, bias_ids,
+                                          bias, bias_off, n_bias, mask, mask_ld, out,
+                                          static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "logits adjustment launch");
+}
+
+}  // extern "C"

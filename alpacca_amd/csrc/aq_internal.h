@@ -212,4 +212,29 @@ hipError_t launch_greedy_advance(const float *logits, int64_t n,
                                  int take_argmax, int64_t *window, int64_t last_n,
                                  int penalize, double penalty, hipStream_t s);
 
+// 8-bit KV cache (aq_kv8.hip) and adjustment of logits (aq_logits.hip).
+// Device pointers; enqueue only.
+constexpr int kKv8Block = 32;  // positions that share a scale
+bool kv8_supported(int head_dim);
+size_t kv8_scratch_bytes(int head_dim);
+// q may be NULL (keys and values alone), and q_out may be q
+hipError_t launch_rope_kv8(const float *q, const float *k, const float *v, float *q_out, int64_t T,
+                           int n_head, int n_rot, int neox, const float *cos_t,
+                           const float *sin_t, const aq_decode_state *st, int64_t pos0,
+                           const aq_kv8 &c, hipStream_t s);
+hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, float *v,
+                           hipStream_t s);
+hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int n_head,
+                                const aq_decode_state *st, int64_t pos0, float *out,
+                                hipStream_t s);
+hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float *v, int n_head,
+                                     int n_rot, int neox, const float *cos_t, const float *sin_t,
+                                     const aq_decode_state *st, int64_t pos0, const aq_kv8 &c,
+                                     float *out, hipStream_t s);
+hipError_t launch_logits_adjust(const float *logits, int64_t rows, int64_t n,
+                                const int64_t *window, int64_t last_n, const double *pen,
+                                const int64_t *bias_ids, const float *bias,
+                                const int64_t *bias_off, int64_t n_bias, const uint32_t *mask,
+                                int64_t mask_ld, float *out, hipStream_t s);
+
 }  // namespace aq

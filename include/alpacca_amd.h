@@ -410,6 +410,101 @@ int aq_greedy_advance_penalized(const float *logits, int64_t n, aq_decode_state 
                                 int64_t capacity, int64_t *window, int64_t last_n,
                                 double penalty, int take_argmax, void *stream);
 
+/* Penalties, biases and a mask on the logits of each of `rows` sequences (n
+ * logits a row, row-major), before a token is chosen.  For a logit x of token t
+ * in row r, in double and rounded to fp32 once at the end:
+ *   t seen c > 0 times in the row's window: x = x > 0 ? x / repeat : x * repeat
+ *     (repeat 0 or 1: as it is), then x -= presence + frequency * c;
+ *   t in the row's bias list: x += its bias (of several entries of one token
+ *     the last counts);
+ *   t's bit in the mask clear: -inf, whatever the rest says.
+ * window [rows][1 + last_n] int64, each row as in aq_greedy_advance_penalized
+ * (count, ring), and penalties [rows][3] double (repeat, presence, frequency):
+ * both or neither NULL.  bias_ids / bias: n_bias entries (0: none); row r owns
+ * entries bias_off[r] .. bias_off[r + 1] - 1 (clipped to 0 .. n_bias), or,
+ * bias_off NULL, every row all of them.  mask: bit t % 32 of word t / 32 allows
+ * token t, row r's words at mask + r * mask_ld (mask_ld 0: one mask for all),
+ * NULL: all allowed; a row may be left with no token (all -inf).  Tokens outside
+ * [0, n) in windows and lists are skipped.  out may be logits; any other
+ * overlap is AQ_ERR_VALUE.  Device pointers; enqueue only.  rows up to 65535.
+ * Penalties and the ring extend Sampler.sample's repeat penalty
+ * (alpacca/sample.py:36-45); the reference has no counterpart for the rest. */
+int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t *window,
+                     int64_t last_n, const double *penalties, const int64_t *bias_ids,
+                     const float *bias, const int64_t *bias_off, int64_t n_bias,
+                     const uint32_t *mask, int64_t mask_ld, float *out, void *stream);
+
+/* ==== 8-bit KV cache =====================================================
+ *
+ * The cache of one layer with keys and values in int8, a quarter of the fp32
+ * cache's bytes (no counterpart in the reference, whose cache is fp32,
+ * model.py:368-371).  Blocks of 32 positions of one kv head, K and V apart:
+ * with amax the largest magnitude among the tokens the block holds so far, the
+ * scale is s = fl32(amax / 127), a value x is coded as the whole number c
+ * nearest to x / s (ties to even, at most 127 in magnitude; 0 where s is 0),
+ * and stands for s c.  A block that holds an infinity or a NaN has a NaN scale
+ * and reads as NaN.  The last block stored is also kept in fp32 (the tail), so a
+ * token that joins it has it coded anew from the values themselves: the codes
+ * do not depend on how many calls brought the tokens.
+ *
+ * The caller allocates the arrays (device memory, 16-byte aligned but for the
+ * scales; sizes from aq_kv8_sizes; no initial content needed).  Calls on one
+ * cache, and on caches that share a scratch, are the caller's to order: on one
+ * stream, or by events; so are replays of graphs that hold them.  Layouts: K
+ * codes [n_kv][n_blocks][32][head_dim], V codes [n_kv][n_blocks][head_dim / 2]
+ * [4][2][8] (aq_kv8.hip), scales [n_kv][n_blocks], tails [n_kv][32][head_dim],
+ * n_blocks = ceil(n_ctx / 32).  head_dim 64, 128 or 256.
+ */
+typedef struct aq_kv8 {
+  int8_t *k, *v;            /* codes                                         */
+  float *k_scale, *v_scale; /* a scale per block                             */
+  float *k_tail, *v_tail;   /* the last block stored, in fp32                */
+  float *scratch;           /* of attention calls; nothing in it outlives one */
+  int64_t n_ctx;            /* positions                                     */
+  int32_t n_kv, head_dim;
+} aq_kv8;
+
+/* Bytes of each codes array, each scales array, each tail and the scratch.
+ * Host only.  AQ_ERR_VALUE for an unsupported shape. */
+int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *scales,
+                 size_t *tail, size_t *scratch);
+
+/* aq_rope_kv into an 8-bit cache: q [T][n_head * head_dim] rotated into q_out
+ * (which may be q; q NULL: no queries), k rotated and coded, v coded, at
+ * positions p0 .. p0+T-1 (p0 = state->pos, or pos0 when state is NULL).  The
+ * rotation is aq_rope_kv's bit for bit (n_rot 0: none; any even n_rot).  A call
+ * that starts inside a block continues it: the block must be the last one
+ * stored, and its positions before p0 stored (going back inside the last block
+ * is fine, what followed is dropped; to go back further, start at a block's
+ * first position).  Slots of the last block past p0+T-1 are cleared, blocks
+ * after it left as they are.  AQ_ERR_VALUE when p0 + T > n_ctx (checked only for
+ * a host position; the kernels skip positions past the cache).  Enqueues only. */
+int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, int64_t T,
+                int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
+                const aq_decode_state *state, int64_t pos0, const aq_kv8 *cache, void *stream);
+
+/* Causal attention of T query tokens (q [T][n_head * head_dim], rotated) at
+ * positions p0 .. p0+T-1, all stored, over the cache's values: token t attends
+ * to positions 0 .. p0+t.  out [T][n_head * head_dim].  float32 accuracy over the
+ * values the codes stand for.  Groups n_head / n_kv of 1 to 16; T up to 65535.
+ * A query with an infinity or a NaN gives NaN.  Enqueues only, and allocates
+ * nothing. */
+int aq_attention_kv8(const float *q, const aq_kv8 *cache, int64_t T, int n_head,
+                     const aq_decode_state *state, int64_t pos0, float *out, void *stream);
+
+/* aq_rope_kv8 of one token and aq_attention_kv8 of its query in one call (the
+ * decode step's form): q, k, v are left as they are, out [n_head * head_dim].
+ * The same codes and scales as the two calls, bit for bit.  n_rot must be a
+ * multiple of 8 for neox.  Enqueues only, and allocates nothing. */
+int aq_attention_rope_kv8(const float *q, const float *k, const float *v, int n_head, int n_rot,
+                          int neox, const float *cos_tab, const float *sin_tab,
+                          const aq_decode_state *state, int64_t pos0, const aq_kv8 *cache,
+                          float *out, void *stream);
+
+/* k, v [n_kv][n][head_dim] fp32: the values of positions start .. start+n-1
+ * (s c, rounded to fp32).  Enqueues only. */
+int aq_kv8_read(const aq_kv8 *cache, int64_t start, int64_t n, float *k, float *v, void *stream);
+
 /* ==== calibration ========================================================
  *
  * Reads rows * row_bytes bytes of device memory at p (row_bytes <= 4096):
