@@ -1260,6 +1260,12 @@ int kv8_span_check(const aq_kv8 *c, const aq_decode_state *state, int64_t pos0, 
   return AQ_OK;
 }
 
+int kv8_aligned(const void *a, const void *b, const void *c, const void *d) {
+  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16)
+    return fail(AQ_ERR_VALUE, "q, k, v and outputs must be 16-byte aligned");
+  return AQ_OK;
+}
+
 int kv8_rope_check(const aq_kv8 *c, int n_rot, const float *cos_tab, const float *sin_tab) {
   if (n_rot < 0 || n_rot > c->head_dim || n_rot % 2)
     return fail(AQ_ERR_VALUE, "n_rot %d must be even and <= head_dim %d", n_rot, c->head_dim);
@@ -1291,6 +1297,7 @@ int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, in
   if (int rc = kv8_rope_check(cache, n_rot, cos_tab, sin_tab)) return rc;
   if (q && n_head <= 0) return fail(AQ_ERR_VALUE, "bad n_head %d", n_head);
   if (T && (!k || !v || (q && !q_out))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(q, k, v, q_out)) return rc;
   if (int rc = kv8_span_check(cache, state, pos0, T)) return rc;
   if (T == 0) return AQ_OK;
   if (T > cache->n_ctx || T / aq::kKv8Block * cache->n_kv > ((int64_t)1 << 28))
@@ -1308,6 +1315,7 @@ int aq_attention_kv8(const float *q, const aq_kv8 *cache, int64_t T, int n_head,
   if (int rc = kv8_heads_check(cache, n_head)) return rc;
   if (T > 65535) return fail(AQ_ERR_VALUE, "at most 65535 query tokens per call");
   if (T && (!q || !out)) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(q, nullptr, nullptr, out)) return rc;
   if (int rc = kv8_span_check(cache, state, pos0, T)) return rc;
   if (T == 0) return AQ_OK;
   hipError_t e = aq::launch_attention_kv8(q, *cache, T, n_head, state, pos0, out,
@@ -1324,7 +1332,10 @@ int aq_attention_rope_kv8(const float *q, const float *k, const float *v, int n_
   if (int rc = kv8_rope_check(cache, n_rot, cos_tab, sin_tab)) return rc;
   if (neox && n_rot % 8)
     return fail(AQ_ERR_VALUE, "fused rope needs n_rot a multiple of 8 for neox, got %d", n_rot);
+  if (n_head > aq::kKv8StepHeads)
+    return fail(AQ_ERR_VALUE, "at most %d query heads per step (got %d)", aq::kKv8StepHeads, n_head);
   if (!q || !k || !v || !out) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(q, k, v, out)) return rc;
   if (int rc = kv8_span_check(cache, state, pos0, 1)) return rc;
   hipError_t e = aq::launch_attention_rope_kv8(q, k, v, n_head, n_rot, neox ? 1 : 0, cos_tab,
                                                sin_tab, state, pos0, *cache, out,

@@ -43,137 +43,275 @@ __device__ __forceinline__ Span span_of(const aq_decode_state *st, int64_t pos0,
   return {p0, T < n_ctx - p0 ? T : n_ctx - p0};
 }
 
-// element d of a head vector, rotated for position pos: pairs (2i, 2i + 1) or,
-// neox, (i, i + n_rot / 2); products and differences rounded separately
-__device__ __forceinline__ float rotated(const float *x, int d, int64_t pos, int n_rot,
-                                         int neox, const float *__restrict__ cos_t,
-                                         const float *__restrict__ sin_t) {
+// The rotation: pairs (2i, 2i + 1) or, neox, (i, i + n_rot / 2) of a head's first
+// n_rot dimensions, products and differences rounded separately.
+struct Rope {
+  const float *cos_t, *sin_t;
+  int n_rot, neox;
+};
+// element d of the head vector x at position pos
+__device__ __forceinline__ float rotated(const float *x, int d, int64_t pos, const Rope &r) {
 #pragma clang fp contract(off)
-  if (d >= n_rot) return x[d];
-  const int half = n_rot / 2;
-  const int i = neox ? (d < half ? d : d - half) : d >> 1;
-  const bool lo = neox ? d < half : !(d & 1);
-  const int other = neox ? (lo ? d + half : d - half) : d ^ 1;
-  const float c = cos_t[pos * half + i], s = sin_t[pos * half + i];
+  if (d >= r.n_rot) return x[d];
+  const int half = r.n_rot / 2;
+  const int i = r.neox ? (d < half ? d : d - half) : d >> 1;
+  const bool lo = r.neox ? d < half : !(d & 1);
+  const int other = r.neox ? (lo ? d + half : d - half) : d ^ 1;
+  const float c = r.cos_t[pos * half + i], s = r.sin_t[pos * half + i];
   const float a = x[d], b = x[other];
   return lo ? a * c - b * s : b * s + a * c;
 }
-
-// the whole number nearest to x / s, ties to even, exactly: rem is x - r s
-// without rounding (a multiple of the smaller of their units, below 2^24 of
-// it), so it tells which side of a half the quotient lies on
-__device__ __forceinline__ int code_of(float x, float s) {
+// elements d .. d + 3 (d a multiple of 4).  neox: n_rot a multiple of 8, so that
+// a group of four has its partners side by side.  Table values are loaded at
+// clamped places before they are needed, without branches between the loads.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f4v rotated4(const float *x, int d, int64_t pos, const Rope &r) {
 #pragma clang fp contract(off)
-  if (!(s > 0.f)) return 0;  // an empty block's scale, or a NaN
-  float r = rintf(x / s);
-  const float rem = fmaf(-r, s, x), two = 2.f * fabsf(rem);
-  if (two > s || (two == s && ((int)r & 1))) r += copysignf(1.f, rem);
-  return (int)fminf(fmaxf(r, -127.f), 127.f);
+  const int half = r.n_rot / 2;
+  const f4v v = *reinterpret_cast<const f4v *>(x + d);
+  if (half == 0) return v;
+  const float *cr = r.cos_t + pos * half, *sr = r.sin_t + pos * half;
+  f4v o = v;
+  if (r.neox) {
+    const bool lo = d < half, in = d < r.n_rot;
+    const int i = in ? (lo ? d : d - half) : 0;
+    const f4v y = *reinterpret_cast<const f4v *>(x + (in ? (lo ? d + half : d - half) : d));
+    const f4v c = *reinterpret_cast<const f4u *>(cr + i), s = *reinterpret_cast<const f4u *>(sr + i);
+    if (in) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = lo ? v[e] * c[e] - y[e] * s[e] : y[e] * s[e] + v[e] * c[e];
+    }
+  } else {
+    float c[2], s[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int i = d / 2 + p < half ? d / 2 + p : half - 1;
+      c[p] = cr[i];
+      s[p] = sr[i];
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (d / 2 + p >= half) continue;
+      o[2 * p] = v[2 * p] * c[p] - v[2 * p + 1] * s[p];
+      o[2 * p + 1] = v[2 * p] * s[p] + v[2 * p + 1] * c[p];
+    }
+  }
+  return o;
+}
+// whether rotated4 takes this rotation
+__device__ __forceinline__ bool rope_by4(const Rope &r) { return !r.neox || r.n_rot % 8 == 0; }
+
+// A block's coding: c = round-half-even(x / s) over the reals.  x * (1 / s) is
+// off by less than 127 2^-22, so its nearest whole number r is the code or, next
+// to a half, one beside it; rem = x - r s is exact (a multiple of the smaller of
+// their units, below 2^24 of it) and tells which.  Scales below 2^-100 are
+// lifted by 2^100, exactly, with the values.
+struct Coder {
+  float s, inv, lift;
+  __device__ __forceinline__ explicit Coder(float scale) {
+    lift = scale < 0x1p-100f ? 0x1p100f : 1.f;
+    s = scale * lift;
+    inv = s > 0.f ? 1.f / s : 0.f;  // an empty block's scale, or a NaN: every code 0
+  }
+  __device__ __forceinline__ int operator()(float x) const {
+#pragma clang fp contract(off)
+    if (!(s > 0.f)) return 0;
+    x *= lift;
+    float r = rintf(x * inv);
+    const float rem = fmaf(-r, s, x), two = 2.f * fabsf(rem);
+    if (two > s || (two == s && ((int)r & 1))) r += copysignf(1.f, rem);
+    return (int)fminf(fmaxf(r, -127.f), 127.f);
+  }
+};
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
+  return amax_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u)
+                                  : __uint_as_float(amax_bits) / 127.f;
+}
+
+// The tokens of one block of one kv head's K or V, in the units of 16 codes that
+// are 16 bytes of the layout: of K 16 dimensions of a position, of V two
+// dimensions of the eight positions 16 pt + 4 g + r.
+template <int HD>
+struct BlockTokens {
+  static constexpr int UNITS = kBlk * HD / 16;
+  bool is_v, by4;
+  const float *src;   // the head's vector of the call's first token
+  int64_t stride;     // from a token to the next
+  float *tail;
+  Span sp;
+  int64_t b;
+  Rope rope;
+  // value pointers: the token's position p (first of its block's row 0)
+  __device__ __forceinline__ void load(int u, float (&x)[16]) const {
+    const int64_t base = b * kBlk;
+    if (!is_v) {
+      const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
+      const int64_t p = base + row;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = 0.f;
+      if (p < sp.p0) {
+        const float *t = tail + row * HD + d0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put4(x, i, *reinterpret_cast<const f4v *>(t + 4 * i));
+      } else if (p < sp.p0 + sp.n) {
+        const float *t = src + (p - sp.p0) * stride;
+        if (by4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) put4(x, i, rotated4(t, d0 + 4 * i, p, rope));
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < 16; ++e) x[e] = rotated(t, d0 + e, p, rope);
+        }
+      }
+      return;
+    }
+    const int d0 = 2 * (u >> 2);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int row = 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
+      const int64_t p = base + row;
+      float2 v = make_float2(0.f, 0.f);
+      const float *t = p < sp.p0 ? tail + row * HD : src + (p - sp.p0) * stride;
+      if (p < sp.p0 + sp.n) v = *reinterpret_cast<const float2 *>(t + d0);
+      x[k] = v.x;
+      x[8 + k] = v.y;
+    }
+  }
+  __device__ __forceinline__ static void put4(float (&x)[16], int i, f4v v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * i + e] = v[e];
+  }
+  // the call's tokens of the block into the tail
+  __device__ __forceinline__ void keep(int u, const float (&x)[16]) const {
+    const int64_t base = b * kBlk;
+    if (!is_v) {
+      const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
+      const int64_t p = base + row;
+      if (p < sp.p0 || p >= sp.p0 + sp.n) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f4v *>(tail + row * HD + d0 + 4 * i) =
+            f4v{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+      return;
+    }
+    const int d0 = 2 * (u >> 2);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int row = 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
+      const int64_t p = base + row;
+      if (p >= sp.p0 && p < sp.p0 + sp.n)
+        *reinterpret_cast<float2 *>(tail + row * HD + d0) = make_float2(x[k], x[8 + k]);
+    }
+  }
+};
+__device__ __forceinline__ uint32_t amax16(const float (&x)[16], uint32_t am) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) am = max(am, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+  return am;  // (as bits: a NaN's lie above infinity's)
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off));
+  return v;
+}
+__device__ __forceinline__ uint4 code16(const Coder &cd, const float (&x)[16]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[i] |= ((uint32_t)cd(x[4 * i + e]) & 0xFFu) << (8 * e);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- rotation and store ------------------------------------------------------
-// Workgroups 0 .. n_store - 1 code one block of one kv head each, K or V: the
-// block's tokens go to LDS (those before the call's from the tail, the call's
-// own rotated), their largest magnitude gives the scale, and every thread codes
-// 16-byte units.  Slots past the last token are cleared.  The workgroup of the
-// call's first block also keeps the tail: it alone reads it (before), and
-// writes the tokens of the last block (after), so no two workgroups meet there.
-// The rest rotate q.
+// Workgroups 0 .. n_store - 1 code one block of one kv head each, K or V: every
+// thread holds one or two units' values (those before the call's from the tail,
+// the call's own rotated), their largest magnitude gives the scale.  Slots past
+// the last token are cleared.  The workgroup of the call's first block also keeps
+// the tail: it alone reads it (before), and writes the tokens of the last block
+// (after), so no two workgroups meet there.  The rest rotate q, four dimensions
+// (neox: and their partners) a thread.
 template <int HD>
-__global__ void __launch_bounds__(kWG)
+constexpr int kStoreWG = HD == 64 ? 128 : 256;
+template <int HD>
+__global__ void __launch_bounds__(kStoreWG<HD>)
     k_kv8_store(const float *q, const float *__restrict__ k, const float *__restrict__ v,
-                float *q_out, int64_t T, int n_head,
-                int n_rot, int neox, const float *__restrict__ cos_t,
-                const float *__restrict__ sin_t, const aq_decode_state *st, int64_t pos0, aq_kv8 c,
-                int64_t n_store) {
-  __shared__ __attribute__((aligned(16))) float xs[kBlk * HD];
-  __shared__ uint32_t red[kWG / 64];
+                float *q_out, int64_t T, int n_head, Rope rope, const aq_decode_state *st,
+                int64_t pos0, aq_kv8 c, int64_t n_store) {
+  constexpr int NT = kStoreWG<HD>, UPT = BlockTokens<HD>::UNITS / NT;
+  __shared__ uint32_t red[NT / 64];
   const Span sp = span_of(st, pos0, T, c.n_ctx);
   if (sp.n == 0) return;
   const int tid = threadIdx.x;
-  if ((int64_t)blockIdx.x >= n_store) {  // q: one element a thread, in place allowed by pairs
-    const int64_t n = sp.n * n_head * (HD / 2);
-    for (int64_t i = ((int64_t)blockIdx.x - n_store) * kWG + tid; i < n;
-         i += (int64_t)(gridDim.x - n_store) * kWG) {
-      const int64_t t = i / (n_head * (HD / 2));
-      const int r = (int)(i - t * (n_head * (HD / 2)));
-      const int h = r / (HD / 2), j = r - h * (HD / 2), half = n_rot / 2;
-      int a, b;
-      if (j < half) {
-        a = neox ? j : 2 * j;
-        b = neox ? j + half : 2 * j + 1;
-      } else {
-        a = n_rot + 2 * (j - half);
-        b = a + 1;
+  if ((int64_t)blockIdx.x >= n_store) {
+    const bool by4 = rope_by4(rope);
+    const int half = rope.n_rot / 2;
+    // a thread's share of a head: four dimensions; neox: the first half's groups
+    // with their partners, and the dimensions past n_rot
+    const int per = by4 ? HD / 4 : HD / 2;
+    const int64_t n = sp.n * n_head * per;
+    for (int64_t i = ((int64_t)blockIdx.x - n_store) * NT + tid; i < n;
+         i += (int64_t)(gridDim.x - n_store) * NT) {
+      const int64_t th = i / per;
+      const int j = (int)(i - th * per);
+      const int64_t p = sp.p0 + th / n_head;
+      const float *x = q + th * HD;
+      float *y = q_out + th * HD;
+      if (by4) {
+        const int d = 4 * j;
+        if (rope.neox && d >= half && d < rope.n_rot) continue;  // its partner's thread's
+        const f4v a = rotated4(x, d, p, rope);
+        if (rope.neox && d < half) {
+          const f4v b = rotated4(x, d + half, p, rope);
+          *reinterpret_cast<f4v *>(y + d + half) = b;
+        }
+        *reinterpret_cast<f4v *>(y + d) = a;
+      } else {  // pairs (j, j + half), then the dimensions past n_rot
+        const int a = j < half ? j : rope.n_rot + 2 * (j - half);
+        const int b = j < half ? j + half : a + 1;
+        const float ra = rotated(x, a, p, rope), rb = rotated(x, b, p, rope);
+        y[a] = ra;
+        y[b] = rb;
       }
-      const float *x = q + (t * n_head + h) * HD;
-      const float ra = rotated(x, a, sp.p0 + t, n_rot, neox, cos_t, sin_t);
-      const float rb = rotated(x, b, sp.p0 + t, n_rot, neox, cos_t, sin_t);
-      float *y = q_out + (t * n_head + h) * HD;
-      y[a] = ra;
-      y[b] = rb;
     }
     return;
   }
-  const int which = (int)(blockIdx.x & 1);
+  const bool is_v = blockIdx.x & 1;
   const int kvh = (int)((blockIdx.x >> 1) % c.n_kv);
   const int64_t b0 = sp.p0 / kBlk, bl = (sp.p0 + sp.n - 1) / kBlk;
   const int64_t b = b0 + (int64_t)(blockIdx.x >> 1) / c.n_kv;
   if (b > bl) return;
-  const float *src = which ? v : k;
-  float *tail = (which ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD;
-  // the call's value at position p (p0 <= p < p0 + n)
-  auto fresh = [&](int64_t p, int d) {
-    const float *x = src + ((p - sp.p0) * c.n_kv + kvh) * HD;
-    return which ? x[d] : rotated(x, d, p, n_rot, neox, cos_t, sin_t);
-  };
-  uint32_t am = 0;  // the largest magnitude, as bits (a NaN's lie above infinity's)
-  for (int i = tid; i < kBlk * HD; i += kWG) {
-    const int row = i / HD, d = i - row * HD;
-    const int64_t p = b * kBlk + row;
-    float x = 0.f;
-    if (p < sp.p0) x = tail[i];
-    else if (p < sp.p0 + sp.n) x = fresh(p, d);
-    xs[i] = x;
-    am = max(am, __float_as_uint(x) & 0x7FFFFFFFu);
-  }
+  BlockTokens<HD> blk{is_v, rope_by4(rope), (is_v ? v : k) + kvh * HD, (int64_t)c.n_kv * HD,
+                      (is_v ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, b, rope};
+  float x[UPT][16];
+  uint32_t am = 0;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) am = max(am, (uint32_t)__shfl_xor((int)am, off));
+  for (int i = 0; i < UPT; ++i) {
+    blk.load(tid + NT * i, x[i]);
+    am = amax16(x[i], am);
+  }
+  am = wave_umax(am);
   if ((tid & 63) == 0) red[tid >> 6] = am;
   __syncthreads();  // (and the tail has been read)
 #pragma unroll
-  for (int w = 0; w < kWG / 64; ++w) am = max(am, red[w]);
-  const float s = am >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(am) / 127.f;
+  for (int w = 0; w < NT / 64; ++w) am = max(am, red[w]);
+  const float s = scale_of(am);
+  const Coder code(s);
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  if (tid == 0) (which ? c.v_scale : c.k_scale)[kvh * n_blocks + b] = s;
-  int8_t *dst = (which ? c.v : c.k) + (kvh * n_blocks + b) * (kBlk * HD);
-  for (int u = tid; u < kBlk * HD / 16; u += kWG) {
-    union {
-      int8_t c8[16];
-      uint4 w;
-    } o;
+  if (tid == 0) (is_v ? c.v_scale : c.k_scale)[kvh * n_blocks + b] = s;
+  uint4 *dst = reinterpret_cast<uint4 *>((is_v ? c.v : c.k) + (kvh * n_blocks + b) * (kBlk * HD));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      int row, d;
-      if (which) {  // unit (dimension pair, g): 2 dimensions x 8 positions
-        row = 16 * ((e >> 2) & 1) + 4 * (u & 3) + (e & 3);
-        d = 2 * (u >> 2) + (e >> 3);
-      } else {
-        row = u / (HD / 16);
-        d = 16 * (u % (HD / 16)) + e;
-      }
-      o.c8[e] = (int8_t)code_of(xs[row * HD + d], s);
-    }
-    reinterpret_cast<uint4 *>(dst)[u] = o.w;
+  for (int i = 0; i < UPT; ++i) dst[tid + NT * i] = code16(code, x[i]);
+  if (b != b0) return;
+  if (bl != b0) {
+    blk.b = bl;
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) blk.load(tid + NT * i, x[i]);
   }
-  if (b == b0) {  // the tail: the last block's tokens of this call
-    const int64_t first = bl == b0 ? sp.p0 : bl * kBlk;
-    const int n = (int)(sp.p0 + sp.n - first), r0 = (int)(first - bl * kBlk);
-    for (int i = tid; i < n * HD; i += kWG) {
-      const int row = i / HD, d = i - row * HD;
-      tail[(r0 + row) * HD + d] = fresh(first + row, d);
-    }
-  }
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) blk.keep(tid + NT * i, x[i]);
 }
 
 // ---- read-back ---------------------------------------------------------------
@@ -281,8 +419,10 @@ template <int HD>
 struct QRow {
   h8 hi[HD / 32], lo[HD / 32];
   float f;
-  __device__ __forceinline__ void load(const float *__restrict__ q, bool live, int cg,
-                                       float scale) {
+  // ROPE: q is rotated for position pos on the way
+  template <bool ROPE>
+  __device__ __forceinline__ void load(const float *__restrict__ q, bool live, int cg, float scale,
+                                       int64_t pos, const Rope &rope) {
     f4v v[HD / 16];
     float am = 0.f;
     bool fin = true;
@@ -291,8 +431,13 @@ struct QRow {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         f4v x = {0.f, 0.f, 0.f, 0.f};
-        if (live)
-          x = *reinterpret_cast<const f4v *>(q + 64 * (ks >> 1) + 16 * cg + 8 * (ks & 1) + 4 * i);
+        const int d = 64 * (ks >> 1) + 16 * cg + 8 * (ks & 1) + 4 * i;
+        if constexpr (ROPE) {  // (rows that do not exist: row 0's, then zeros)
+          x = rotated4(q, d, pos, rope);
+          if (!live) x = f4v{0.f, 0.f, 0.f, 0.f};
+        } else if (live) {
+          x = *reinterpret_cast<const f4v *>(q + d);
+        }
         v[2 * ks + i] = x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -415,16 +560,24 @@ struct OutScale {
 // ..., straight from memory into operand order (no LDS), the next block's loads
 // under way while one is computed; the waves' states meet in LDS, the splits'
 // in k_kv8_combine.  One split writes the output itself.
+//
+// ROPE: one token, whose q, k and v are not rotated yet.  Every workgroup
+// rotates its q rows in registers; one more workgroup per kv head (the last)
+// takes the token's block, which it alone reads: it codes the block anew from
+// the tail and the token (k_kv8_store's codes, bit for bit), stores it and
+// attends to it from LDS, while the others go through the blocks before.
 constexpr int kWaves = 4;
-template <int HD>
+template <int HD, bool ROPE>
 __global__ void __launch_bounds__(64 * kWaves)
     k_kv8_split(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
-                int64_t T, int G, float scale, float *__restrict__ part,
-                float *__restrict__ out) {
+                int64_t T, int G, float scale, float *__restrict__ part, float *__restrict__ out,
+                const float *__restrict__ kn, const float *__restrict__ vn, Rope rope) {
   constexpr int KJ = HD / 64, VJ = HD / 32, PS = HD + 4;
   constexpr int PARTS = HD == 256 ? 2 : 1, VP = VJ / PARTS;  // the merge's LDS: at most 32 KB
   __shared__ f4v os[kWaves][2 * VP][64];
   __shared__ float stat[kWaves][3][16];
+  __shared__ uint4 own[ROPE ? 2 : 1][ROPE ? BlockTokens<HD>::UNITS : 1];  // the token's block
+  __shared__ uint32_t red[2][kWaves];
   const Span sp = span_of(st, pos0, T, c.n_ctx);
   const int j = blockIdx.x, S = gridDim.x, kvh = blockIdx.y, n_head = gridDim.y * G;
   const int id0 = blockIdx.z * 16, rows = (int)sp.n * G;  // at most 65535 x 16
@@ -436,7 +589,8 @@ __global__ void __launch_bounds__(64 * kWaves)
   const int g = live ? id - tok * G : 0;
   const int64_t lim = sp.p0 + tok;              // the row's last position
   const int64_t lim0 = sp.p0 + id0 / G;         // the tile's first row's
-  const int nb = (int)((sp.p0 + id_last / G) / kBlk) + 1;  // blocks the tile sees
+  const int nb_all = (int)((sp.p0 + id_last / G) / kBlk) + 1;  // blocks the tile sees
+  const int nb = ROPE ? nb_all - 1 : nb_all;                   // of them from memory
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
   const int8_t *kb = c.k + kvh * n_blocks * (kBlk * HD), *vb = c.v + kvh * n_blocks * (kBlk * HD);
   const float *ksc = c.k_scale + kvh * n_blocks, *vsc = c.v_scale + kvh * n_blocks;
@@ -445,7 +599,7 @@ __global__ void __launch_bounds__(64 * kWaves)
     float ks, vs;
   };
   auto load = [&](int b, Buf &x) {
-    b = b < nb ? b : nb - 1;  // (past the last one: not used)
+    b = b < nb ? b : nb_all - 1;  // (past the last one: not used)
     const int8_t *kp = kb + (int64_t)b * (kBlk * HD), *vp = vb + (int64_t)b * (kBlk * HD);
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt)
@@ -459,10 +613,12 @@ __global__ void __launch_bounds__(64 * kWaves)
     x.vs = vsc[b];
   };
   Buf b0, b1;
-  int b = j * kWaves + wave;
-  load(b, b0);
+  const bool owner = ROPE && j == S - 1;
+  int b = owner ? nb : j * kWaves + wave;
+  if (!owner) load(b, b0);
   QRow<HD> qr;
-  qr.load(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale);
+  qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, sp.p0,
+                         rope);
   RowState<HD> s;
   s.clear();
   auto compute = [&](int blk, Buf &x) {
@@ -504,7 +660,64 @@ __global__ void __launch_bounds__(64 * kWaves)
       }
     }
   };
-  const int stride = S * kWaves;
+  if constexpr (ROPE) {
+    if (owner) {
+      constexpr int UNITS = BlockTokens<HD>::UNITS, NT = 64 * kWaves;
+      constexpr int UPT = (UNITS + NT - 1) / NT;
+      const int tid = threadIdx.x;
+      float x[2][UPT][16];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const BlockTokens<HD> blk{w == 1, true, (w ? vn : kn) + kvh * HD, (int64_t)c.n_kv * HD,
+                                  (w ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp,
+                                  (int64_t)nb, rope};
+        uint32_t am = 0;
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+          const int u = tid + NT * i;
+          if (u >= UNITS) continue;
+          blk.load(u, x[w][i]);
+          blk.keep(u, x[w][i]);  // (its own row; no other thread reads it)
+          am = amax16(x[w][i], am);
+        }
+        am = wave_umax(am);
+        if (lane == 0) red[w][wave] = am;
+      }
+      __syncthreads();
+      float sc[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        sc[w] = scale_of(max(max(red[w][0], red[w][1]), max(red[w][2], red[w][3])));
+        const Coder code(sc[w]);
+        if (tid == 0) (w ? c.v_scale : c.k_scale)[kvh * n_blocks + nb] = sc[w];
+        uint4 *dst =
+            reinterpret_cast<uint4 *>((w ? c.v : c.k) + (kvh * n_blocks + nb) * (kBlk * HD));
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+          const int u = tid + NT * i;
+          if (u >= UNITS) continue;
+          own[w][u] = code16(code, x[w][i]);
+          dst[u] = own[w][u];
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int jj = 0; jj < KJ; ++jj)
+            b0.k[pt][jj] = *reinterpret_cast<const u4v *>(
+                &own[0][((16 * pt + r16) * HD + 64 * jj + 16 * cg) / 16]);
+#pragma unroll
+        for (int i = 0; i < VJ; ++i)
+          b0.v[i] = *reinterpret_cast<const u4v *>(&own[1][(16 * i + r16) * 4 + cg]);
+        b0.ks = sc[0];
+        b0.vs = sc[1];
+        compute(nb, b0);
+      }
+    }
+  }
+  const int stride = (ROPE ? S - 1 : S) * kWaves;
   while (b < nb) {
     load(b + stride, b1);
     compute(b, b0);
@@ -563,29 +776,86 @@ __global__ void __launch_bounds__(64 * kWaves)
     *reinterpret_cast<f4v *>(dst + HD) = f4v{M, R, den, 0.f};
 }
 
-// One workgroup of HD threads per query row merges the splits' states.
+// One workgroup per query row merges the splits' states: HD / 4 threads of 16
+// bytes a split, all of a chunk's loads (and the m, R, l of every split) in
+// flight at once.
+constexpr int kMaxSplits = 512;
 template <int HD>
-__global__ void __launch_bounds__(HD)
+__global__ void __launch_bounds__(kWG)
     k_kv8_combine(const float *__restrict__ part, const aq_decode_state *st, int64_t pos0,
                   int64_t n_ctx, int64_t T, int G, int S, float *__restrict__ out) {
-  constexpr int PS = HD + 4;
-  const Span sp = span_of(st, pos0, T, n_ctx);
-  const int id = blockIdx.x, t = id / G;
-  if (t >= sp.n) return;
-  const int kvh = blockIdx.y, d = threadIdx.x, n_head = gridDim.y * G;
+  constexpr int PS = HD + 4, LP = HD / 4, NG = kWG / LP, U = 8;
+  __shared__ float fo[kMaxSplits + 8];
+  __shared__ float red[3][kWG / 64];
+  __shared__ f4v acc[NG][LP];
+  const int id = blockIdx.x, t = id / G, kvh = blockIdx.y, n_head = gridDim.y * G;
+  const int tid = threadIdx.x, d4 = tid % LP, grp = tid / LP;
   const float *p = part + ((int64_t)kvh * T * G + id) * S * PS;
-  float M = -INFINITY, R = kLow;
-  for (int s = 0; s < S; ++s) {
-    M = fmaxf(M, p[s * PS + HD]);
-    R = fmaxf(R, p[s * PS + HD + 1]);
+  f4v x[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int s = grp + NG * u;
+    x[u] = *reinterpret_cast<const f4v *>(p + (s < S ? s : 0) * PS + 4 * d4);
+  }
+  f4v e[2];  // m, R, l of splits tid and tid + 256
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = tid + kWG * i;
+    e[i] = f4v{-INFINITY, kLow, 0.f, 0.f};
+    if (s < S) e[i] = *reinterpret_cast<const f4v *>(p + s * PS + HD);
+  }
+  const Span sp = span_of(st, pos0, T, n_ctx);
+  if (t >= sp.n) return;
+  float M = fmaxf(e[0][0], e[1][0]), R = fmaxf(e[0][1], e[1][1]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    M = fmaxf(M, __shfl_xor(M, off));
+    R = fmaxf(R, __shfl_xor(R, off));
+  }
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = M;
+    red[1][tid >> 6] = R;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWG / 64; ++w) {
+    M = fmaxf(M, red[0][w]);
+    R = fmaxf(R, red[1][w]);
   }
   const float mref = M == -INFINITY ? 0.f : M;
-  float num = 0.f, den = 0.f;
-  for (int s = 0; s < S; ++s) {
-    num = fmaf(p[s * PS + d], exp2_(p[s * PS + HD + 1] - R), num);
-    den = fmaf(p[s * PS + HD + 2], exp2_(p[s * PS + HD] - mref), den);
+  float den = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (tid + kWG * i < S) fo[tid + kWG * i] = exp2_(e[i][1] - R);
+    den = fmaf(e[i][2], exp2_(e[i][0] - mref), den);
   }
-  out[((int64_t)t * n_head + kvh * G + (id - t * G)) * HD + d] = OutScale(R, M, den)(num);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+  if ((tid & 63) == 0) red[2][tid >> 6] = den;
+  __syncthreads();
+  den = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  f4v o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + grp + NG * u;
+      if (s < S) o += x[u] * fo[s];
+    }
+    s0 += NG * U;
+    if (s0 >= S) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + grp + NG * u;
+      x[u] = *reinterpret_cast<const f4v *>(p + (s < S ? s : 0) * PS + 4 * d4);
+    }
+  }
+  acc[grp][d4] = o;
+  __syncthreads();
+  if (tid >= LP) return;
+#pragma unroll
+  for (int w = 1; w < NG; ++w) o += acc[w][d4];
+  const OutScale fin(R, M, den);
+  reinterpret_cast<f4v *>(out + ((int64_t)t * n_head + kvh * G + (id - t * G)) * HD)[d4] = fin(o);
 }
 
 // ---- many rows: tiles of rows over all positions they see -------------------------
@@ -624,7 +894,8 @@ __global__ void __launch_bounds__(64 * kWaves)
     const int tok = live ? id / G : 0;
     const int g = live ? id - tok * G : 0;
     lim[n] = sp.p0 + tok;
-    qr[n].load(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale);
+    qr[n].template load<false>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, 0,
+                               Rope{});
     s[n].clear();
   }
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
@@ -746,7 +1017,7 @@ bool kv8_supported(int head_dim) { return head_dim == 64 || head_dim == 128 || h
 // partials of at most this many (query row, split)s
 constexpr int64_t kScratchRows = 16384;
 size_t kv8_scratch_bytes(int head_dim) {
-  return (size_t)2 * kScratchRows * (head_dim + 4) * sizeof(float);
+  return (size_t)kScratchRows * (head_dim + 4) * sizeof(float);
 }
 
 #define AQ_HD(hd, CALL)                                   \
@@ -763,10 +1034,13 @@ hipError_t launch_rope_kv8(const float *q, const float *k, const float *v, float
                            const aq_kv8 &c, hipStream_t s) {
   const int64_t blocks = (T + kBlk - 2) / kBlk + 1;  // blocks T positions can touch
   const int64_t n_store = blocks * c.n_kv * 2;
-  int64_t n_q = q ? (T * n_head * (c.head_dim / 2) + kWG - 1) / kWG : 0;
-  if (n_q > 8192) n_q = 8192;
-  AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_store<HD>, dim3((unsigned)(n_store + n_q)), dim3(kWG),
-                                       0, s, q, k, v, q_out, T, n_head, n_rot, neox, cos_t, sin_t,
+  const Rope rope{cos_t, sin_t, n_rot, neox};
+  const int64_t per = !neox || n_rot % 8 == 0 ? c.head_dim / 4 : c.head_dim / 2;
+  const int wg = c.head_dim == 64 ? 128 : 256;
+  int64_t n_q = q ? (T * n_head * per + wg - 1) / wg : 0;
+  if (n_q > 16384) n_q = 16384;
+  AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_store<HD>, dim3((unsigned)(n_store + n_q)),
+                                       dim3(kStoreWG<HD>), 0, s, q, k, v, q_out, T, n_head, rope,
                                        st, pos0, c, n_store))
   return hipGetLastError();
 }
@@ -788,8 +1062,8 @@ int kv8_splits(const aq_kv8 &c, int64_t T, int n_head) {
   const int64_t G = n_head / c.n_kv, tiles = (T * G + 15) / 16;
   const int64_t blocks = (c.n_ctx + kBlk - 1) / kBlk;
   int64_t S = (blocks + kWaves - 1) / kWaves;
-  const int64_t fill = (512 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
-  const int64_t room = kScratchRows / (T * n_head);
+  const int64_t fill = (kMaxSplits - 1 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
+  const int64_t room = kScratchRows / (T * n_head) - 1;  // (the step's last one)
   S = S < fill ? S : fill;
   S = S < room ? S : room;
   return (int)(S < 1 ? 1 : S);
@@ -804,11 +1078,13 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
   if (rows <= 64) {
     const int S = kv8_splits(c, T, n_head);
     AQ_HD(c.head_dim,
-          hipLaunchKernelGGL(k_kv8_split<HD>, dim3((unsigned)S, (unsigned)c.n_kv,
-                                                   (unsigned)((rows + 15) / 16)),
-                             dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale, c.scratch, out);
+          hipLaunchKernelGGL((k_kv8_split<HD, false>),
+                             dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)((rows + 15) / 16)),
+                             dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale, c.scratch, out,
+                             nullptr, nullptr, Rope{});
           if (S > 1) hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)rows, (unsigned)c.n_kv),
-                                        dim3(HD), 0, s, c.scratch, st, pos0, c.n_ctx, T, G, S, out))
+                                        dim3(kWG), 0, s, c.scratch, st, pos0, c.n_ctx, T, G, S,
+                                        out))
     return hipGetLastError();
   }
   const int64_t tiles = (rows + 63) / 64;
@@ -822,11 +1098,16 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      int n_rot, int neox, const float *cos_t, const float *sin_t,
                                      const aq_decode_state *st, int64_t pos0, const aq_kv8 &c,
                                      float *out, hipStream_t s) {
-  if (n_head > kScratchRows) return hipErrorInvalidValue;
-  float *qr = c.scratch + kScratchRows * (c.head_dim + 4);
-  hipError_t e = launch_rope_kv8(q, k, v, qr, 1, n_head, n_rot, neox, cos_t, sin_t, st,
-                                 pos0, c, s);
-  return e != hipSuccess ? e : launch_attention_kv8(qr, c, 1, n_head, st, pos0, out, s);
+  const float scale = (float)(1.0 / sqrt((double)c.head_dim));
+  const int G = n_head / c.n_kv;
+  const int S = kv8_splits(c, 1, n_head) + 1;
+  AQ_HD(c.head_dim,
+        hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
+                           dim3(64 * kWaves), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
+                           c.scratch, out, k, v, Rope{cos_t, sin_t, n_rot, neox});
+        hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)G, (unsigned)c.n_kv), dim3(kWG), 0, s,
+                           c.scratch, st, pos0, c.n_ctx, (int64_t)1, G, S, out))
+  return hipGetLastError();
 }
 
 }  // namespace aq

@@ -103,7 +103,8 @@ class QuantKVCache:
         if heads is not None and width != heads * self.head_dim:
             raise ValueError(f"{name} has {width} values per token, expected "
                              f"{heads} x {self.head_dim}")
-        return x if x.is_contiguous() else x.contiguous()
+        x = x if x.is_contiguous() else x.contiguous()
+        return x if x.data_ptr() % 16 == 0 else x.clone()  # (the kernels load 16 bytes)
 
     def _query_heads(self, q) -> int:
         n, rem = divmod(q.shape[1], self.head_dim)

@@ -450,7 +450,8 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  * The caller allocates the arrays (device memory, 16-byte aligned but for the
  * scales; sizes from aq_kv8_sizes; no initial content needed).  Calls on one
  * cache, and on caches that share a scratch, are the caller's to order: on one
- * stream, or by events; so are replays of graphs that hold them.  Layouts: K
+ * stream, or by events; so are replays of graphs that hold them.  q, k, v
+ * and outputs are 16-byte aligned too (AQ_ERR_VALUE).  Layouts: K
  * codes [n_kv][n_blocks][32][head_dim], V codes [n_kv][n_blocks][head_dim / 2]
  * [4][2][8] (aq_kv8.hip), scales [n_kv][n_blocks], tails [n_kv][32][head_dim],
  * n_blocks = ceil(n_ctx / 32).  head_dim 64, 128 or 256.
