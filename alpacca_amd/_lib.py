@@ -147,6 +147,15 @@ def check(rc: int) -> None:
     raise RuntimeError(msg or f"alpacca_amd error {rc}")
 
 
+def current_stream(index: int) -> int:
+    """The hipStream_t of torch's current stream on device `index`."""
+    import torch
+    try:  # without a Stream object per call (1 us of a call's few)
+        return torch._C._cuda_getCurrentRawStream(index)
+    except AttributeError:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def device_count() -> int:
     n = ctypes.c_int(0)
     check(load().aq_device_count(ctypes.byref(n)))

@@ -17,6 +17,8 @@
 //   scales [n_kv][n_blocks] fp32; tails [n_kv][32][head_dim] fp32.
 #include <math.h>
 
+#include <type_traits>
+
 #include "aq_internal.h"
 
 namespace aq {
@@ -98,30 +100,127 @@ __device__ __forceinline__ f4v rotated4(const float *x, int d, int64_t pos, cons
   }
   return o;
 }
+// a where mask is all ones, b where it is 0 (bits; a conditional here becomes
+// branches, which part the loads and the waits)
+__device__ __forceinline__ float pick(uint32_t mask, float a, float b) {
+  return __uint_as_float((__float_as_uint(a) & mask) | (__float_as_uint(b) & ~mask));
+}
+__device__ __forceinline__ uint32_t ones_if(bool c) { return c ? 0xFFFFFFFFu : 0u; }
+// elements d0 .. d0 + 15 (d0 a multiple of 16) of x: every load goes out before
+// the first use
+__device__ __forceinline__ void rotated16(const float *x, int d0, int64_t pos, const Rope &r,
+                                          float (&o)[16]) {
+#pragma clang fp contract(off)
+  const int half = r.n_rot / 2;
+  f4v v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f4v *>(x + d0 + 4 * i);
+  if (half == 0) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = v[e >> 2][e & 3];
+    return;
+  }
+  const float *cr = r.cos_t + pos * half, *sr = r.sin_t + pos * half;
+  if (r.neox) {
+    f4v y[4], c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + 4 * i;
+      const bool lo = d < half, in = d < r.n_rot;
+      const int t = in ? (lo ? d : d - half) : 0;
+      y[i] = *reinterpret_cast<const f4v *>(x + (in ? (lo ? d + half : d - half) : d));
+      c[i] = *reinterpret_cast<const f4u *>(cr + t);
+      s[i] = *reinterpret_cast<const f4u *>(sr + t);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + 4 * i;
+      const uint32_t in = ones_if(d < r.n_rot), minus = d < half ? 0x80000000u : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = v[i][e] * c[i][e], b = y[i][e] * s[i][e];
+        o[4 * i + e] = pick(in, a + __uint_as_float(__float_as_uint(b) ^ minus), v[i][e]);
+      }
+    }
+    return;
+  }
+  float c[8], s[8];
+  if (r.n_rot % 16 == 0) {  // the pairs are all rotated or none
+    const int t = d0 / 2 < half ? d0 / 2 : 0;
+    const f4u c0 = *reinterpret_cast<const f4u *>(cr + t),
+              c1 = *reinterpret_cast<const f4u *>(cr + t + 4),
+              s0 = *reinterpret_cast<const f4u *>(sr + t),
+              s1 = *reinterpret_cast<const f4u *>(sr + t + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = c0[e], c[4 + e] = c1[e];
+      s[e] = s0[e], s[4 + e] = s1[e];
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int t = d0 / 2 + p < half ? d0 / 2 + p : half - 1;
+      c[p] = cr[t];
+      s[p] = sr[t];
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const float a = v[p >> 1][2 * (p & 1)], b = v[p >> 1][2 * (p & 1) + 1];
+    const uint32_t in = ones_if(d0 / 2 + p < half);
+    const float ra = a * c[p] - b * s[p], rb = a * s[p] + b * c[p];
+    o[2 * p] = pick(in, ra, a);
+    o[2 * p + 1] = pick(in, rb, b);
+  }
+}
 // whether rotated4 takes this rotation
 __device__ __forceinline__ bool rope_by4(const Rope &r) { return !r.neox || r.n_rot % 8 == 0; }
 
-// A block's coding: c = round-half-even(x / s) over the reals.  x * (1 / s) is
-// off by less than 127 2^-22, so its nearest whole number r is the code or, next
-// to a half, one beside it; rem = x - r s is exact (a multiple of the smaller of
-// their units, below 2^24 of it) and tells which.  Scales below 2^-100 are
-// lifted by 2^100, exactly, with the values.
+// A block's coding: c = round-half-even(x / s) over the reals.  y = x (1 / s) is
+// off by less than 127 2^-23, so its nearest whole number r is the code unless it
+// lies that near a half (one value in thirty thousand); then the remainder
+// x - r s, which is exact (a multiple of the smaller of their units, below 2^24 of
+// it), tells.  Scales below 2^-100 are lifted by 2^100, exactly, with the
+// values; among the subnormals a scale can be too small, and codes end at 127.
 struct Coder {
   float s, inv, lift;
   __device__ __forceinline__ explicit Coder(float scale) {
     lift = scale < 0x1p-100f ? 0x1p100f : 1.f;
     s = scale * lift;
-    inv = s > 0.f ? 1.f / s : 0.f;  // an empty block's scale, or a NaN: every code 0
+    inv = s > 0.f ? 1.f / s : 0.f;
   }
-  __device__ __forceinline__ int operator()(float x) const {
-#pragma clang fp contract(off)
-    if (!(s > 0.f)) return 0;
-    x *= lift;
-    float r = rintf(x * inv);
-    const float rem = fmaf(-r, s, x), two = 2.f * fabsf(rem);
-    if (two > s || (two == s && ((int)r & 1))) r += copysignf(1.f, rem);
-    return (int)fminf(fmaxf(r, -127.f), 127.f);
+  // 16 values as bytes: 1.5 2^23 added to y leaves its nearest whole number in
+  // the sum's low bits
+  __device__ __forceinline__ uint4 operator()(const float (&x)[16]) const {
+    uint32_t t[16], w[4];
+    if (!(s >= 0.f)) return make_uint4(0, 0, 0, 0);
+    float far = lift - 1.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float m = fmaf(x[e], inv, kMagic), r = m - kMagic;
+      far = fmaxf(far, fabsf(fmaf(x[e], inv, -r)));
+      t[e] = __float_as_uint(m);
+    }
+    if (far > 0.49998f) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float v = x[e] * lift, r = rintf(v * inv), rem = fmaf(-r, s, v);
+        int c = (int)r;
+        const float two = 2.f * fabsf(rem);
+        const bool fix = (two > s) | ((two == s) & ((c & 1) != 0));
+        c += fix ? (rem < 0.f ? -1 : 1) : 0;
+        t[e] = (uint32_t)min(max(c, -127), 127);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0C0C0400u);
+      const uint32_t b = __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x0C0C0400u);
+      w[i] = a | b << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  static constexpr float kMagic = 12582912.f;
 };
 __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
   return amax_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u)
@@ -135,59 +234,69 @@ template <int HD>
 struct BlockTokens {
   static constexpr int UNITS = kBlk * HD / 16;
   bool is_v, by4;
-  const float *src;   // the head's vector of the call's first token
-  int64_t stride;     // from a token to the next
-  float *tail;
-  Span sp;
-  int64_t b;
+  float *tail;         // rows before the call's tokens
+  const float *first;  // where the call's token of row 0 would be
+  int64_t stride;      // from a token to the next
+  int before, end;     // rows 0 .. before - 1 from the tail, before .. end - 1 the call's
+  int64_t pos;         // the position of row 0
   Rope rope;
-  // value pointers: the token's position p (first of its block's row 0)
+  // block b of a call's tokens sp at x (the head's vector of the first of them)
+  __device__ __forceinline__ BlockTokens(bool is_v, bool by4, const float *x, int64_t stride,
+                                         float *tail, const Span &sp, int64_t b, const Rope &rope)
+      : is_v(is_v), by4(by4), tail(tail), stride(stride), rope(rope) {
+    pos = b * kBlk;
+    const int64_t lead = sp.p0 - pos, e = lead + sp.n;
+    first = x - lead * stride;
+    before = lead > 0 ? (int)lead : 0;
+    end = e < kBlk ? (int)e : kBlk;
+  }
+  // the vector of a row (past the last token: of the last, not used)
+  __device__ __forceinline__ const float *row_of(int row) const {
+    const float *t = tail + row * HD, *f = first + (int64_t)min(max(row, before), end - 1) * stride;
+    return row < before ? t : f;
+  }
+  // the unit's values (0 past the last token); the loads do not wait for any
   __device__ __forceinline__ void load(int u, float (&x)[16]) const {
-    const int64_t base = b * kBlk;
     if (!is_v) {
       const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
-      const int64_t p = base + row;
+      const float *t = row_of(row);
+      if (by4) {
+        float y[16];
+        rotated16(t, d0, pos + min(max(row, before), end - 1), rope, y);
+        const uint32_t old = ones_if(row < before), live = ones_if(row < end);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = 0.f;
-      if (p < sp.p0) {
-        const float *t = tail + row * HD + d0;
+        for (int i = 0; i < 4; ++i) {
+          const f4v v = *reinterpret_cast<const f4v *>(t + d0 + 4 * i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put4(x, i, *reinterpret_cast<const f4v *>(t + 4 * i));
-      } else if (p < sp.p0 + sp.n) {
-        const float *t = src + (p - sp.p0) * stride;
-        if (by4) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) put4(x, i, rotated4(t, d0 + 4 * i, p, rope));
-        } else {
-#pragma unroll 1
-          for (int e = 0; e < 16; ++e) x[e] = rotated(t, d0 + e, p, rope);
+          for (int e = 0; e < 4; ++e) x[4 * i + e] = pick(old, v[e], pick(live, y[4 * i + e], 0.f));
         }
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e)
+          x[e] = row < before ? t[d0 + e] : row < end ? rotated(t, d0 + e, pos + row, rope) : 0.f;
       }
       return;
     }
     const int d0 = 2 * (u >> 2);
+    float2 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      v[k] = *reinterpret_cast<const float2 *>(row_of(v_row(u, k)) + d0);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int row = 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
-      const int64_t p = base + row;
-      float2 v = make_float2(0.f, 0.f);
-      const float *t = p < sp.p0 ? tail + row * HD : src + (p - sp.p0) * stride;
-      if (p < sp.p0 + sp.n) v = *reinterpret_cast<const float2 *>(t + d0);
-      x[k] = v.x;
-      x[8 + k] = v.y;
+      const uint32_t live = ones_if(v_row(u, k) < end);
+      x[k] = pick(live, v[k].x, 0.f);
+      x[8 + k] = pick(live, v[k].y, 0.f);
     }
   }
-  __device__ __forceinline__ static void put4(float (&x)[16], int i, f4v v) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[4 * i + e] = v[e];
+  __device__ __forceinline__ static int v_row(int u, int k) {
+    return 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
   }
   // the call's tokens of the block into the tail
   __device__ __forceinline__ void keep(int u, const float (&x)[16]) const {
-    const int64_t base = b * kBlk;
     if (!is_v) {
       const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
-      const int64_t p = base + row;
-      if (p < sp.p0 || p >= sp.p0 + sp.n) return;
+      if (row < before || row >= end) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f4v *>(tail + row * HD + d0 + 4 * i) =
@@ -197,9 +306,8 @@ struct BlockTokens {
     const int d0 = 2 * (u >> 2);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int row = 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
-      const int64_t p = base + row;
-      if (p >= sp.p0 && p < sp.p0 + sp.n)
+      const int row = v_row(u, k);
+      if (row >= before && row < end)
         *reinterpret_cast<float2 *>(tail + row * HD + d0) = make_float2(x[k], x[8 + k]);
     }
   }
@@ -209,20 +317,19 @@ __device__ __forceinline__ uint32_t amax16(const float (&x)[16], uint32_t am) {
   for (int e = 0; e < 16; ++e) am = max(am, __float_as_uint(x[e]) & 0x7FFFFFFFu);
   return am;  // (as bits: a NaN's lie above infinity's)
 }
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off));
-  return v;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dppu(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
 }
-__device__ __forceinline__ uint4 code16(const Coder &cd, const float (&x)[16]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[i] |= ((uint32_t)cd(x[4 * i + e]) & 0xFFu) << (8 * e);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = max(v, dppu<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = max(v, dppu<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = max(v, dppu<0x141>(v));  // row_half_mirror
+  v = max(v, dppu<0x140>(v));  // row_mirror
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
 }
 
 // ---- rotation and store ------------------------------------------------------
@@ -231,12 +338,11 @@ __device__ __forceinline__ uint4 code16(const Coder &cd, const float (&x)[16]) {
 // the call's own rotated), their largest magnitude gives the scale.  Slots past
 // the last token are cleared.  The workgroup of the call's first block also keeps
 // the tail: it alone reads it (before), and writes the tokens of the last block
-// (after), so no two workgroups meet there.  The rest rotate q, four dimensions
-// (neox: and their partners) a thread.
+// (after), so no two workgroups meet there.  The rest rotate q, a token each.
 template <int HD>
 constexpr int kStoreWG = HD == 64 ? 128 : 256;
 template <int HD>
-__global__ void __launch_bounds__(kStoreWG<HD>)
+__global__ void __launch_bounds__(kStoreWG<HD>, HD == 256 ? 2 : 4)
     k_kv8_store(const float *q, const float *__restrict__ k, const float *__restrict__ v,
                 float *q_out, int64_t T, int n_head, Rope rope, const aq_decode_state *st,
                 int64_t pos0, aq_kv8 c, int64_t n_store) {
@@ -248,32 +354,32 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
   if ((int64_t)blockIdx.x >= n_store) {
     const bool by4 = rope_by4(rope);
     const int half = rope.n_rot / 2;
-    // a thread's share of a head: four dimensions; neox: the first half's groups
-    // with their partners, and the dimensions past n_rot
-    const int per = by4 ? HD / 4 : HD / 2;
-    const int64_t n = sp.n * n_head * per;
-    for (int64_t i = ((int64_t)blockIdx.x - n_store) * NT + tid; i < n;
-         i += (int64_t)(gridDim.x - n_store) * NT) {
-      const int64_t th = i / per;
-      const int j = (int)(i - th * per);
-      const int64_t p = sp.p0 + th / n_head;
-      const float *x = q + th * HD;
-      float *y = q_out + th * HD;
-      if (by4) {
-        const int d = 4 * j;
-        if (rope.neox && d >= half && d < rope.n_rot) continue;  // its partner's thread's
-        const f4v a = rotated4(x, d, p, rope);
-        if (rope.neox && d < half) {
-          const f4v b = rotated4(x, d + half, p, rope);
-          *reinterpret_cast<f4v *>(y + d + half) = b;
+    for (int64_t t = (int64_t)blockIdx.x - n_store; t < sp.n; t += gridDim.x - n_store) {
+      const int64_t p = sp.p0 + t;
+      if (by4) {  // a thread's share: four dimensions; neox: and their partners
+        for (int i = tid; i < n_head * (HD / 4); i += NT) {
+          const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+          const float *x = q + (t * n_head + h) * HD;
+          float *y = q_out + (t * n_head + h) * HD;
+          if (rope.neox && d >= half && d < rope.n_rot) continue;  // its partner's thread's
+          const f4v a = rotated4(x, d, p, rope);
+          if (rope.neox && d < half) {
+            const f4v b = rotated4(x, d + half, p, rope);
+            *reinterpret_cast<f4v *>(y + d + half) = b;
+          }
+          *reinterpret_cast<f4v *>(y + d) = a;
         }
-        *reinterpret_cast<f4v *>(y + d) = a;
       } else {  // pairs (j, j + half), then the dimensions past n_rot
-        const int a = j < half ? j : rope.n_rot + 2 * (j - half);
-        const int b = j < half ? j + half : a + 1;
-        const float ra = rotated(x, a, p, rope), rb = rotated(x, b, p, rope);
-        y[a] = ra;
-        y[b] = rb;
+        for (int i = tid; i < n_head * (HD / 2); i += NT) {
+          const int h = i / (HD / 2), j = i % (HD / 2);
+          const float *x = q + (t * n_head + h) * HD;
+          float *y = q_out + (t * n_head + h) * HD;
+          const int a = j < half ? j : rope.n_rot + 2 * (j - half);
+          const int b = j < half ? j + half : a + 1;
+          const float ra = rotated(x, a, p, rope), rb = rotated(x, b, p, rope);
+          y[a] = ra;
+          y[b] = rb;
+        }
       }
     }
     return;
@@ -283,8 +389,11 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
   const int64_t b0 = sp.p0 / kBlk, bl = (sp.p0 + sp.n - 1) / kBlk;
   const int64_t b = b0 + (int64_t)(blockIdx.x >> 1) / c.n_kv;
   if (b > bl) return;
-  BlockTokens<HD> blk{is_v, rope_by4(rope), (is_v ? v : k) + kvh * HD, (int64_t)c.n_kv * HD,
-                      (is_v ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, b, rope};
+  auto tokens = [&](int64_t bi) {
+    return BlockTokens<HD>(is_v, rope_by4(rope), (is_v ? v : k) + kvh * HD, (int64_t)c.n_kv * HD,
+                           (is_v ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, bi, rope);
+  };
+  BlockTokens<HD> blk = tokens(b);
   float x[UPT][16];
   uint32_t am = 0;
 #pragma unroll
@@ -303,10 +412,10 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
   if (tid == 0) (is_v ? c.v_scale : c.k_scale)[kvh * n_blocks + b] = s;
   uint4 *dst = reinterpret_cast<uint4 *>((is_v ? c.v : c.k) + (kvh * n_blocks + b) * (kBlk * HD));
 #pragma unroll
-  for (int i = 0; i < UPT; ++i) dst[tid + NT * i] = code16(code, x[i]);
+  for (int i = 0; i < UPT; ++i) dst[tid + NT * i] = code(x[i]);
   if (b != b0) return;
   if (bl != b0) {
-    blk.b = bl;
+    blk = tokens(bl);
 #pragma unroll
     for (int i = 0; i < UPT; ++i) blk.load(tid + NT * i, x[i]);
   }
@@ -423,40 +532,43 @@ struct QRow {
   template <bool ROPE>
   __device__ __forceinline__ void load(const float *__restrict__ q, bool live, int cg, float scale,
                                        int64_t pos, const Rope &rope) {
-    f4v v[HD / 16];
-    float am = 0.f;
-    bool fin = true;
+    float v[HD / 64][16];
+    const uint32_t exists = ones_if(live);
+    uint32_t am = 0;  // the largest magnitude, as bits (infinity's and NaNs' above all)
 #pragma unroll
-    for (int ks = 0; ks < HD / 32; ++ks)
+    for (int jj = 0; jj < HD / 64; ++jj) {
+      const int d0 = 64 * jj + 16 * cg;
+      if constexpr (ROPE) {
+        rotated16(q, d0, pos, rope, v[jj]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f4v x = {0.f, 0.f, 0.f, 0.f};
-        const int d = 64 * (ks >> 1) + 16 * cg + 8 * (ks & 1) + 4 * i;
-        if constexpr (ROPE) {  // (rows that do not exist: row 0's, then zeros)
-          x = rotated4(q, d, pos, rope);
-          if (!live) x = f4v{0.f, 0.f, 0.f, 0.f};
-        } else if (live) {
-          x = *reinterpret_cast<const f4v *>(q + d);
-        }
-        v[2 * ks + i] = x;
+        for (int i = 0; i < 4; ++i) {
+          const f4v x = *reinterpret_cast<const f4v *>(q + d0 + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          fin = fin && fabsf(x[e]) < INFINITY;
-          am = fmaxf(am, fabsf(x[e]));
+          for (int e = 0; e < 4; ++e) v[jj][4 * i + e] = x[e];
         }
       }
-    am = row_max(am);
-    const bool bad = row_max(fin ? 0.f : 1.f) != 0.f;
-    const int up = am > 0.f && !bad ? 15 - __builtin_amdgcn_frexp_expf(am) : 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        v[jj][e] = pick(exists, v[jj][e], 0.f);  // (rows that do not exist read row 0)
+        am = max(am, __float_as_uint(v[jj][e]) & 0x7FFFFFFFu);
+      }
+    }
+    const auto r = __builtin_amdgcn_permlane16_swap(am, am, false, false);
+    am = max(r[0], r[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(am, am, false, false);
+    am = max(t[0], t[1]);
+    const bool bad = am >= 0x7F800000u;
+    const int up = am > 0 && !bad ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(am)) : 0;
     f = bad ? __uint_as_float(0x7FC00000u) : ldexpf(scale * kLog2e, -up);
+    const uint32_t good = ones_if(!bad);
 #pragma unroll
     for (int ks = 0; ks < HD / 32; ++ks) {
       u4v h, l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f4v x = v[2 * ks + (i >> 1)];
-        const float a = bad ? 0.f : ldexpf(x[2 * (i & 1)], up);
-        const float b = bad ? 0.f : ldexpf(x[2 * (i & 1) + 1], up);
+        const float a = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i], up), 0.f);
+        const float b = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i + 1], up), 0.f);
         uint32_t hh, ll;
         pieces2(a, b, hh, ll);
         h[i] = hh, l[i] = ll;
@@ -562,7 +674,7 @@ struct OutScale {
 // in k_kv8_combine.  One split writes the output itself.
 //
 // ROPE: one token, whose q, k and v are not rotated yet.  Every workgroup
-// rotates its q rows in registers; one more workgroup per kv head (the last)
+// rotates its q rows in registers; one more workgroup per kv head (the first)
 // takes the token's block, which it alone reads: it codes the block anew from
 // the tail and the token (k_kv8_store's codes, bit for bit), stores it and
 // attends to it from LDS, while the others go through the blocks before.
@@ -613,15 +725,43 @@ __global__ void __launch_bounds__(64 * kWaves)
     x.vs = vsc[b];
   };
   Buf b0, b1;
-  const bool owner = ROPE && j == S - 1;
-  int b = owner ? nb : j * kWaves + wave;
+  const bool owner = ROPE && j == 0;
+  int b = owner ? nb : (ROPE ? j - 1 : j) * kWaves + wave;
   if (!owner) load(b, b0);
+  // the owner's tokens: on their way before q's are waited for
+  constexpr int UNITS = BlockTokens<HD>::UNITS, NT = 64 * kWaves;
+  constexpr int UPT = 2 * UNITS / NT;  // units of K, then V, per thread
+  float x[ROPE ? UPT : 1][16];
+  auto tokens = [&](int i, int &u) {  // (the same w for the wave)
+    int w;
+    if constexpr (UNITS < NT) {
+      w = __builtin_amdgcn_readfirstlane(threadIdx.x / UNITS);
+      u = threadIdx.x % UNITS;
+    } else {
+      w = i / (UNITS / NT);
+      u = threadIdx.x + NT * (i % (UNITS / NT));
+    }
+    return BlockTokens<HD>(w == 1, true, (w ? vn : kn) + kvh * HD, (int64_t)c.n_kv * HD,
+                           (w ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, (int64_t)nb,
+                           rope);
+  };
+  if constexpr (ROPE) {
+    if (owner) {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        int u;
+        const BlockTokens<HD> blk = tokens(i, u);
+        blk.load(u, x[i]);
+      }
+    }
+  }
   QRow<HD> qr;
   qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, sp.p0,
                          rope);
   RowState<HD> s;
   s.clear();
-  auto compute = [&](int blk, Buf &x) {
+  auto compute = [&](int blk, Buf &x, auto mask) {
+    constexpr bool MASK = decltype(mask)::value;
     f4v sc[2];
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt) {
@@ -639,7 +779,7 @@ __global__ void __launch_bounds__(64 * kWaves)
     h8 ph[1], pl[1];
     const float ks[1] = {x.ks}, vs[1] = {x.vs};
     const int64_t first = (int64_t)blk * kBlk;
-    if (first + kBlk - 1 > lim0) {  // (uniform) some row ends inside the block or before it
+    if (MASK && first + kBlk - 1 > lim0) {  // (uniform) some row ends inside it or before
       const int64_t d = lim - first - 4 * cg;
       const int last[1] = {(int)(d > 64 ? 64 : d < -1 ? -1 : d)};
       softmax_step<HD, 1, true>(s, sc, qr.f, ks, vs, last, ph, pl);
@@ -662,43 +802,38 @@ __global__ void __launch_bounds__(64 * kWaves)
   };
   if constexpr (ROPE) {
     if (owner) {
-      constexpr int UNITS = BlockTokens<HD>::UNITS, NT = 64 * kWaves;
-      constexpr int UPT = (UNITS + NT - 1) / NT;
-      const int tid = threadIdx.x;
-      float x[2][UPT][16];
+      uint32_t am[2] = {0, 0};  // of K's and V's units (a wave's units are of one each)
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        int u;
+        const BlockTokens<HD> blk = tokens(i, u);
+        if (!blk.is_v) blk.keep(u, x[i]);  // (its own row; no other thread reads it)
+        const uint32_t a = amax16(x[i], 0);
+        am[0] = max(am[0], blk.is_v ? 0u : a);
+        am[1] = max(am[1], blk.is_v ? a : 0u);
+      }
+      for (int d = threadIdx.x; d < HD; d += NT)  // V's tail row: the token's values
+        c.v_tail[((int64_t)kvh * kBlk + sp.p0 % kBlk) * HD + d] = vn[kvh * HD + d];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const BlockTokens<HD> blk{w == 1, true, (w ? vn : kn) + kvh * HD, (int64_t)c.n_kv * HD,
-                                  (w ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp,
-                                  (int64_t)nb, rope};
-        uint32_t am = 0;
-#pragma unroll
-        for (int i = 0; i < UPT; ++i) {
-          const int u = tid + NT * i;
-          if (u >= UNITS) continue;
-          blk.load(u, x[w][i]);
-          blk.keep(u, x[w][i]);  // (its own row; no other thread reads it)
-          am = amax16(x[w][i], am);
-        }
-        am = wave_umax(am);
-        if (lane == 0) red[w][wave] = am;
+        am[w] = wave_umax(am[w]);
+        if (lane == 0) red[w][wave] = am[w];
       }
       __syncthreads();
       float sc[2];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         sc[w] = scale_of(max(max(red[w][0], red[w][1]), max(red[w][2], red[w][3])));
-        const Coder code(sc[w]);
-        if (tid == 0) (w ? c.v_scale : c.k_scale)[kvh * n_blocks + nb] = sc[w];
-        uint4 *dst =
-            reinterpret_cast<uint4 *>((w ? c.v : c.k) + (kvh * n_blocks + nb) * (kBlk * HD));
+        if (threadIdx.x == 0) (w ? c.v_scale : c.k_scale)[kvh * n_blocks + nb] = sc[w];
+      }
 #pragma unroll
-        for (int i = 0; i < UPT; ++i) {
-          const int u = tid + NT * i;
-          if (u >= UNITS) continue;
-          own[w][u] = code16(code, x[w][i]);
-          dst[u] = own[w][u];
-        }
+      for (int i = 0; i < UPT; ++i) {
+        int u;
+        const BlockTokens<HD> blk = tokens(i, u);
+        const int w = blk.is_v ? 1 : 0;
+        const uint4 cd = Coder(w ? sc[1] : sc[0])(x[i]);
+        own[w][u] = cd;
+        reinterpret_cast<uint4 *>((w ? c.v : c.k) + (kvh * n_blocks + nb) * (kBlk * HD))[u] = cd;
       }
       __syncthreads();
       if (wave == 0) {
@@ -713,17 +848,18 @@ __global__ void __launch_bounds__(64 * kWaves)
           b0.v[i] = *reinterpret_cast<const u4v *>(&own[1][(16 * i + r16) * 4 + cg]);
         b0.ks = sc[0];
         b0.vs = sc[1];
-        compute(nb, b0);
+        compute(nb, b0, std::true_type());
       }
     }
   }
   const int stride = (ROPE ? S - 1 : S) * kWaves;
+  constexpr auto mask = std::integral_constant<bool, !ROPE>();  // (full blocks before the token's)
   while (b < nb) {
     load(b + stride, b1);
-    compute(b, b0);
+    compute(b, b0, mask);
     if ((b += stride) >= nb) break;
     load(b + stride, b0);
-    compute(b, b1);
+    compute(b, b1, mask);
     b += stride;
   }
   // the waves' states, then one state per row
@@ -1035,10 +1171,7 @@ hipError_t launch_rope_kv8(const float *q, const float *k, const float *v, float
   const int64_t blocks = (T + kBlk - 2) / kBlk + 1;  // blocks T positions can touch
   const int64_t n_store = blocks * c.n_kv * 2;
   const Rope rope{cos_t, sin_t, n_rot, neox};
-  const int64_t per = !neox || n_rot % 8 == 0 ? c.head_dim / 4 : c.head_dim / 2;
-  const int wg = c.head_dim == 64 ? 128 : 256;
-  int64_t n_q = q ? (T * n_head * per + wg - 1) / wg : 0;
-  if (n_q > 16384) n_q = 16384;
+  const int64_t n_q = !q ? 0 : T < 65536 ? T : 65536;
   AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_store<HD>, dim3((unsigned)(n_store + n_q)),
                                        dim3(kStoreWG<HD>), 0, s, q, k, v, q_out, T, n_head, rope,
                                        st, pos0, c, n_store))

@@ -39,7 +39,7 @@ class QuantKVCache:
         _lib.check(_lib.load().aq_kv8_sizes(n_kv, head_dim, n_ctx,
                                             *[ctypes.byref(s) for s in sizes]))
         codes, scales, tail, scr = (s.value for s in sizes)
-        _lib.ensure_device()
+        self._lib = _lib.ensure_device()
         self._torch = torch
         self.device = torch.device("cuda" if device is None else device)
         if self.device.type != "cuda":
@@ -87,23 +87,23 @@ class QuantKVCache:
     def _rows(self, x, name: str, heads=None):
         """x as a contiguous float32 [T, heads * head_dim] on the device."""
         torch = self._torch
-        if not isinstance(x, torch.Tensor) or x.dtype != torch.float32:
+        if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32:
             raise ValueError(f"{name} must be a float32 tensor")
         if x.device != self.device:
             raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
-        width = x.shape[-1] if x.dim() == 2 else x.numel() // max(1, x.shape[0] if x.dim() else 1)
-        if x.dim() == 1:
-            x, width = x.view(1, -1) if x.is_contiguous() else x.reshape(1, -1), x.numel()
-        elif x.dim() == 3:
+        dim = x.dim()
+        if dim == 1:
+            x = x.unsqueeze(0)
+        elif dim == 3:
             if x.shape[2] != self.head_dim:
                 raise ValueError(f"{name} has shape {tuple(x.shape)}, head_dim is {self.head_dim}")
-            x, width = x.reshape(x.shape[0], -1), x.shape[1] * x.shape[2]
-        elif x.dim() != 2:
+            x = x.reshape(x.shape[0], x.shape[1] * x.shape[2])
+        elif dim != 2:
             raise ValueError(f"{name} must be (T, heads * head_dim), got {tuple(x.shape)}")
-        if heads is not None and width != heads * self.head_dim:
-            raise ValueError(f"{name} has {width} values per token, expected "
+        if heads is not None and x.shape[1] != heads * self.head_dim:
+            raise ValueError(f"{name} has {x.shape[1]} values per token, expected "
                              f"{heads} x {self.head_dim}")
-        x = x if x.is_contiguous() else x.contiguous()
+        x = x.contiguous()
         return x if x.data_ptr() % 16 == 0 else x.clone()  # (the kernels load 16 bytes)
 
     def _query_heads(self, q) -> int:
@@ -143,8 +143,14 @@ class QuantKVCache:
             raise ValueError(f"position {pos} lies inside a block before the last one: go back "
                              f"to {pos - pos % BLOCK}")
 
-    def _stream(self):
-        return self._torch.cuda.current_stream(self.device).cuda_stream
+    def _call(self, fn, *args):
+        """fn(*args, stream) with the cache's device current."""
+        cuda = self._torch.cuda
+        if cuda.current_device() == self.device.index:
+            _lib.check(fn(*args, _lib.current_stream(self.device.index)))
+        else:
+            with cuda.device(self.device):
+                _lib.check(fn(*args, _lib.current_stream(self.device.index)))
 
     # ---- operators -----------------------------------------------------------
 
@@ -169,7 +175,9 @@ class QuantKVCache:
             if q.shape[0] != T:
                 raise ValueError(f"k has {T} tokens, q {q.shape[0]}")
             if q_out is None:
-                q_out = torch.empty_like(q).view(shape)
+                q_out = torch.empty_like(q)
+                if len(shape) != 2:
+                    q_out = q_out.view(shape)
             elif (q_out.dtype != torch.float32 or q_out.numel() != q.numel()
                   or q_out.device != self.device or not q_out.is_contiguous()):
                 raise ValueError("q_out must be a contiguous float32 tensor of q's size")
@@ -179,32 +187,26 @@ class QuantKVCache:
         self._span(pos, T, True)
         n_rot, cp, sp = self._tables(cos, sin, pos + T)
         if T:
-            with torch.cuda.device(self.device):
-                _lib.check(_lib.load().aq_rope_kv8(
-                    qp, k.data_ptr(), v.data_ptr(), op, T, n_head, n_rot, 1 if neox else 0, cp, sp,
-                    None, pos, self._ref, self._stream()))
+            self._call(self._lib.aq_rope_kv8, qp, k.data_ptr(), v.data_ptr(), op, T, n_head, n_rot,
+                       1 if neox else 0, cp, sp, None, pos, self._ref)
             self.length = pos + T
         return q_out
 
     def attend(self, q, pos: int, out=None):
         """Attention of the queries q (T, n_head * head_dim, rotated) at
         positions pos .., each over the positions up to its own; as q."""
-        torch = self._torch
         qc = self._rows(q, "q")
         n_head, T = self._query_heads(qc), qc.shape[0]
         self._span(pos, T, False)
         out = self._out(out, q, qc)
         if T:
-            with torch.cuda.device(self.device):
-                _lib.check(_lib.load().aq_attention_kv8(
-                    qc.data_ptr(), self._ref, T, n_head, None, pos, out.data_ptr(),
-                    self._stream()))
+            self._call(self._lib.aq_attention_kv8, qc.data_ptr(), self._ref, T, n_head, None, pos,
+                       out.data_ptr())
         return out
 
     def step(self, q, k, v, pos: int, cos=None, sin=None, neox: bool = False, out=None):
         """store and attend for one token, q, k and v as they are before the
         rotation: the attention output, as q."""
-        torch = self._torch
         qc = self._rows(q, "q")
         k, v = self._rows(k, "k", self.n_kv), self._rows(v, "v", self.n_kv)
         n_head = self._query_heads(qc)
@@ -213,16 +215,15 @@ class QuantKVCache:
         self._span(pos, 1, True)
         n_rot, cp, sp = self._tables(cos, sin, pos + 1)
         out = self._out(out, q, qc)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().aq_attention_rope_kv8(
-                qc.data_ptr(), k.data_ptr(), v.data_ptr(), n_head, n_rot, 1 if neox else 0, cp, sp,
-                None, pos, self._ref, out.data_ptr(), self._stream()))
+        self._call(self._lib.aq_attention_rope_kv8, qc.data_ptr(), k.data_ptr(), v.data_ptr(),
+                   n_head, n_rot, 1 if neox else 0, cp, sp, None, pos, self._ref, out.data_ptr())
         self.length = pos + 1
         return out
 
     def _out(self, out, q, qc):
         if out is None:
-            return self._torch.empty_like(qc).view(q.shape)
+            out = self._torch.empty_like(qc)
+            return out if q.dim() == 2 else out.view(q.shape)
         if (out.dtype != self._torch.float32 or out.numel() != qc.numel()
                 or out.device != self.device or not out.is_contiguous()):
             raise ValueError("out must be a contiguous float32 tensor of q's size")
@@ -235,12 +236,12 @@ class QuantKVCache:
         stop = self.length if stop is None else stop
         if not 0 <= start <= stop <= self.length:
             raise ValueError(f"positions {start}..{stop - 1} of {self.length} stored")
-        k, v = (torch.empty((self.n_kv, stop - start, self.head_dim), dtype=torch.float32,
-                            device=self.device) for _ in range(2))
+        kv = torch.empty((2, self.n_kv, stop - start, self.head_dim), dtype=torch.float32,
+                         device=self.device)
+        k, v = kv[0], kv[1]
         if stop > start:
-            with torch.cuda.device(self.device):
-                _lib.check(_lib.load().aq_kv8_read(self._ref, start, stop - start, k.data_ptr(),
-                                                   v.data_ptr(), self._stream()))
+            self._call(self._lib.aq_kv8_read, self._ref, start, stop - start, k.data_ptr(),
+                       v.data_ptr())
         return k, v
 
 

@@ -27,13 +27,13 @@ def pack_mask(allowed):
 
 def _tensor(x, name, dtype, shape, device):
     import torch
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype or tuple(x.shape) != tuple(shape):
+    if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.shape != shape:
         have = (f"{x.dtype} {tuple(x.shape)}" if isinstance(x, torch.Tensor)
                 else type(x).__name__)
         raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {have}")
     if x.device != device:
         raise ValueError(f"{name} is on {x.device}, the logits on {device}")
-    return x if x.is_contiguous() else x.contiguous()
+    return x.contiguous()
 
 
 def adjust_logits(logits, *, window=None, penalties=None, bias=None, mask=None, out=None):
@@ -61,7 +61,7 @@ def adjust_logits(logits, *, window=None, penalties=None, bias=None, mask=None, 
                                 and out.shape == logits.shape and out.device == dev
                                 and out.is_contiguous()):
         raise ValueError("out must be a contiguous float32 tensor of the logits' shape and device")
-    x = logits if logits.is_contiguous() else logits.contiguous()
+    x = logits.contiguous()
     rows, n = (1, x.shape[0]) if one else x.shape
     if (window is None) != (penalties is None):
         raise ValueError("window and penalties come together or not at all")
@@ -95,11 +95,14 @@ def adjust_logits(logits, *, window=None, penalties=None, bias=None, mask=None, 
 
     def p(t):
         return None if t is None else t.data_ptr()
-    _lib.ensure_device()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().aq_logits_adjust(
-            x.data_ptr(), rows, n, p(window), last_n, p(penalties), p(ids), p(val), p(off), n_bias,
-            p(mask), mask_ld, out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+    args = (x.data_ptr(), rows, n, p(window), last_n, p(penalties), p(ids), p(val), p(off), n_bias,
+            p(mask), mask_ld, out.data_ptr())
+    fn, index = _lib.ensure_device().aq_logits_adjust, dev.index
+    if torch.cuda.current_device() == index:
+        _lib.check(fn(*args, _lib.current_stream(index)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, _lib.current_stream(index)))
     return out
 
 
