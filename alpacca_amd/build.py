@@ -35,7 +35,11 @@ HIPCC_FLAGS = [
 # matvec take their leading scalar arguments preloaded into scalar registers
 # at wave launch (gfx950 kernel argument preloading): the kernels whose first
 # memory operations depend on them skip the argument load's round trip.
+# The 8-bit cache's kernels keep their matrix instructions' accumulators in
+# vector registers, which their softmax rescales and reads: in accumulation
+# registers (the compiler's choice) every pass moved them across.
 FILE_FLAGS = {
+    "aq_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "aq_decode.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "aq_matvec_i8.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }

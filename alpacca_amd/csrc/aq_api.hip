@@ -1318,6 +1318,8 @@ int aq_attention_kv8(const float *q, const aq_kv8 *cache, int64_t T, int n_head,
   if (int rc = kv8_aligned(q, nullptr, nullptr, out)) return rc;
   if (int rc = kv8_span_check(cache, state, pos0, T)) return rc;
   if (T == 0) return AQ_OK;
+  int dev = 0;
+  if (int rc = current_device(dev)) return rc;
   hipError_t e = aq::launch_attention_kv8(q, *cache, T, n_head, state, pos0, out,
                                           static_cast<hipStream_t>(stream));
   return e == hipSuccess ? AQ_OK : hip_fail(e, "8-bit cache attention launch");

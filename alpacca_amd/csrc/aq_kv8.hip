@@ -485,6 +485,11 @@ __device__ __forceinline__ float row_sum(float v) {
   p = lane_pair<32>(p.x + p.y);
   return p.x + p.y;
 }
+// a float that no store of this kernel reaches, at a wave's common place: a
+// scalar load
+__device__ __forceinline__ float load_const(const float *p) {
+  return *(const __attribute__((address_space(4))) float *)p;
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // four signed codes as exact fp16: 1024 + (c + 128) by its bits, less 1152
@@ -514,8 +519,12 @@ __device__ __forceinline__ void codes16(u4v w, h8 &lo, h8 &hi) {
 // (a, b) as pieces: fp16 of the value, and fp16 of what that leaves
 __device__ __forceinline__ void pieces2(float a, float b, uint32_t &hi, uint32_t &lo) {
   const h2 h = __builtin_convertvector(f2v{a, b}, h2);
+  // (a factor that the compiler does not know keeps this one mixed-precision
+  // fused multiply-add a value, exact, instead of a conversion and a difference)
+  float minus = -1.f;
+  asm("" : "+v"(minus));
   const h2 l = __builtin_convertvector(
-      f2v{fmaf((float)h[0], -1.f, a), fmaf((float)h[1], -1.f, b)}, h2);
+      f2v{fmaf((float)h[0], minus, a), fmaf((float)h[1], minus, b)}, h2);
   hi = __builtin_bit_cast(uint32_t, h);
   lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -618,12 +627,13 @@ __device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB]
     if (vs[b] > 0.f) R = fmaxf(R, t[b] + ve[b]);
   }
   const float mref = mn == -INFINITY ? 0.f : mn;
-  const float corr = exp2_(st.m - mref), corr_o = exp2_(st.R - R);
+  // (whole exponents: an integer conversion and a ldexp, a quarter of exp2's time)
+  const float corr = ldexpf(1.f, (int)(st.m - mref)), corr_o = ldexpf(1.f, (int)(st.R - R));
   float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const float g =
-        __builtin_amdgcn_frexp_mantf(vs[b]) * exp2_(fminf(ve[b] + mref - R + kTop, 120.f));
+    const float g = ldexpf(__builtin_amdgcn_frexp_mantf(vs[b]),
+                           (int)fminf(ve[b] + mref - R + kTop, 120.f));
     u4v h, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -645,9 +655,12 @@ __device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB]
   }
   st.l = fmaf(st.l, corr, sum);
   st.m = mn;
-  st.R = R;
+  // (R moves in whole powers of two, so seldom)
+  if (__any(R != st.R)) {
 #pragma unroll
-  for (int i = 0; i < HD / 16; ++i) st.o[i] *= corr_o;
+    for (int i = 0; i < HD / 16; ++i) st.o[i] *= corr_o;
+  }
+  st.R = R;
 }
 
 // v 2^(R - m - kTop) / den, the power in two whole parts so that neither leaves
@@ -1002,18 +1015,25 @@ __global__ void __launch_bounds__(kWG)
 template <int HD, int NR>
 __global__ void __launch_bounds__(64 * kWaves)
     k_kv8_tiles(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
-                int64_t T, int G, float scale, int tiles, float *__restrict__ out) {
+                int64_t T, int G, float scale, int tiles, int layer,
+                float *__restrict__ out) {
   constexpr int KJ = HD / 64, VJ = HD / 32, KS = HD / 32, NU = HD / 64;
   __shared__ __attribute__((aligned(16))) h8 kl[4 * KS][64];   // [position tile, k step][lane]
   __shared__ __attribute__((aligned(16))) h8 vl[4 * VJ][64];   // [block, dimension tile][lane]
   const Span sp = span_of(st, pos0, T, c.n_ctx);
-  // the tiles that see most first; a kv head's tiles side by side in the grid
-  // are n_kv apart (workgroup id modulo 8 is the XCD: one L2 per kv head)
+  // The tiles that see most first; every other layer of `layer` tiles (what the
+  // GPU's CUs take of a kv head at once) the other way round, so that CUs that
+  // hold several workgroups get alike sums.  A kv head's tiles are n_kv apart in
+  // the grid (workgroup id modulo 8 is the XCD: one L2 per kv head).
   const int n_kv = c.n_kv, kvh = blockIdx.x % n_kv, n_head = n_kv * G;
-  const int tile = tiles - 1 - (int)(blockIdx.x / n_kv);
+  int rank = (int)(blockIdx.x / n_kv);
+  const int ly = rank / layer, in = rank - ly * layer;
+  if ((ly & 1) && (ly + 1) * layer <= tiles) rank = ly * layer + layer - 1 - in;
+  const int tile = tiles - 1 - rank;
   const int rows = (int)sp.n * G, id0 = tile * (16 * NR * kWaves);
   if (id0 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, cg = lane >> 4;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, cg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wid0 = id0 + wave * (16 * NR);  // the wave's first row
   int id_last = id0 + 16 * NR * kWaves - 1;
   id_last = id_last < rows ? id_last : rows - 1;
@@ -1037,33 +1057,22 @@ __global__ void __launch_bounds__(64 * kWaves)
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
   const int8_t *kb = c.k + kvh * n_blocks * (kBlk * HD), *vb = c.v + kvh * n_blocks * (kBlk * HD);
   const float *ksc = c.k_scale + kvh * n_blocks, *vsc = c.v_scale + kvh * n_blocks;
+  const int8_t *kl0 = kb + r16 * HD + 16 * cg, *vl0 = vb + r16 * 64 + 16 * cg;
   u4v rk[NU], rv[NU];
   float ks[2], vs[2], nks[2], nvs[2];
-  auto fetch = [&](int ch) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      int b = 2 * ch + u;
-      b = b < nb ? b : nb - 1;  // (an odd last block's partner: masked)
-      nks[u] = ksc[b];
-      nvs[u] = vsc[b];
-    }
+  auto fetch = [&](int ch) {  // (block numbers are the wave's: scalar)
+    const int64_t b0 = 2 * ch, b1 = 2 * ch + 1 < nb ? 2 * ch + 1 : nb - 1;  // (b1 past: masked)
+    nks[0] = load_const(ksc + b0);
+    nks[1] = load_const(ksc + b1);
+    nvs[0] = load_const(vsc + b0);
+    nvs[1] = load_const(vsc + b1);
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int x = wave + kWaves * i;
-      {
-        const int pt = x / KJ, jj = x % KJ;
-        int b = 2 * ch + (pt >> 1);
-        b = b < nb ? b : nb - 1;
-        rk[i] = *reinterpret_cast<const u4v *>(kb + (int64_t)b * (kBlk * HD) +
-                                               (16 * (pt & 1) + r16) * HD + 64 * jj + 16 * cg);
-      }
-      {
-        const int u = x / VJ, jv = x % VJ;
-        int b = 2 * ch + u;
-        b = b < nb ? b : nb - 1;
-        rv[i] = *reinterpret_cast<const u4v *>(vb + (int64_t)b * (kBlk * HD) +
-                                               ((16 * jv + r16) * 4 + cg) * 16);
-      }
+      const int pt = x / KJ, jj = x % KJ, u = x / VJ, jv = x % VJ;
+      rk[i] = *reinterpret_cast<const u4v *>(
+          kl0 + ((pt >> 1 ? b1 : b0) * kBlk + 16 * (pt & 1)) * HD + 64 * jj);
+      rv[i] = *reinterpret_cast<const u4v *>(vl0 + (u ? b1 : b0) * (kBlk * HD) + 1024 * jv);
     }
   };
   fetch(0);
@@ -1220,10 +1229,17 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
                                         out))
     return hipGetLastError();
   }
-  const int64_t tiles = (rows + 63) / 64;
-  AQ_HD(c.head_dim, hipLaunchKernelGGL((k_kv8_tiles<HD, 1>), dim3((unsigned)(tiles * c.n_kv)),
-                                       dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale,
-                                       (int)tiles, out))
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev)) return e;
+  const int cus = device_info(dev).cus;
+  const int layer = cus / c.n_kv > 1 ? cus / c.n_kv : 1;
+#define AQ_TILES(NR)                                                                          \
+  hipLaunchKernelGGL((k_kv8_tiles<HD, NR>),                                                   \
+                     dim3((unsigned)((rows + 64 * NR - 1) / (64 * NR) * c.n_kv)),             \
+                     dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale,                    \
+                     (int)((rows + 64 * NR - 1) / (64 * NR)), layer, out)
+  AQ_HD(c.head_dim, AQ_TILES(1))
+#undef AQ_TILES
   return hipGetLastError();
 }
 
