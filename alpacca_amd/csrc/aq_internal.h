@@ -215,7 +215,7 @@ hipError_t launch_greedy_advance(const float *logits, int64_t n,
 // 8-bit KV cache (aq_kv8.hip) and adjustment of logits (aq_logits.hip).
 // Device pointers; enqueue only.
 constexpr int kKv8Block = 32;  // positions that share a scale
-constexpr int kKv8StepHeads = 8192;  // most query heads whose step the scratch holds
+constexpr int kKv8StepHeads = 32768;  // most query heads whose step the scratch holds
 bool kv8_supported(int head_dim);
 size_t kv8_scratch_bytes(int head_dim);
 // q may be NULL (keys and values alone), and q_out may be q

@@ -1008,18 +1008,27 @@ __global__ void __launch_bounds__(kWG)
 }
 
 // ---- many rows: tiles of rows over all positions they see -------------------------
-// One workgroup of four waves per 64 NR rows (16 NR per wave) of a kv head.
-// The chunks of two blocks are converted to fp16 in operand order in LDS once
-// for all waves (each lane's 16 bytes at its place: no conflicts), the next
-// chunk's codes in flight meanwhile.
-template <int HD, int NR>
+// One workgroup of four waves per 64 rows (16 per wave) of a kv head and split of
+// the positions (gridDim.y of them; one writes the output, several their states
+// for k_kv8_combine).  The chunks of two blocks are converted to fp16 in operand order in LDS once for all waves
+// (each lane's 16 bytes at its place: no conflicts).  A wave's pass over chunk ch
+// forms the scores of chunk ch + 1 while the softmax of chunk ch runs (the matrix
+// and the vector instructions of one pass do not wait for each other), then adds
+// the values of chunk ch; K of chunk ch + 2 and V of chunk ch + 1 go to LDS
+// meanwhile, the codes after them are on their way, and one barrier ends it.
+template <int HD>
 __global__ void __launch_bounds__(64 * kWaves)
     k_kv8_tiles(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
-                int64_t T, int G, float scale, int tiles, int layer,
+                int64_t T, int G, float scale, int tiles, int layer, float *__restrict__ part,
                 float *__restrict__ out) {
-  constexpr int KJ = HD / 64, VJ = HD / 32, KS = HD / 32, NU = HD / 64;
-  __shared__ __attribute__((aligned(16))) h8 kl[4 * KS][64];   // [position tile, k step][lane]
-  __shared__ __attribute__((aligned(16))) h8 vl[4 * VJ][64];   // [block, dimension tile][lane]
+  constexpr int KJ = HD / 64, VJ = HD / 32, KS = HD / 32;
+  constexpr int NU = HD / 64;  // 1 KB units of a chunk's K (and of its V) per wave
+  // 128 dimensions and more have the registers to read four operands ahead (146
+  // against 134 us below; at 64 it costs: 56 against 59)
+  constexpr int AHEAD = HD >= 128 ? 4 : 1;
+  extern __shared__ __attribute__((aligned(16))) h8 lds[];
+  auto kl = reinterpret_cast<h8(*)[4 * KS][64]>(lds);                // [2][position tile, k step][lane]
+  auto vl = reinterpret_cast<h8(*)[4 * VJ][64]>(lds + 2 * 4 * KS * 64);  // [2][block, dim. tile][lane]
   const Span sp = span_of(st, pos0, T, c.n_ctx);
   // The tiles that see most first; every other layer of `layer` tiles (what the
   // GPU's CUs take of a kv head at once) the other way round, so that CUs that
@@ -1030,128 +1039,160 @@ __global__ void __launch_bounds__(64 * kWaves)
   const int ly = rank / layer, in = rank - ly * layer;
   if ((ly & 1) && (ly + 1) * layer <= tiles) rank = ly * layer + layer - 1 - in;
   const int tile = tiles - 1 - rank;
-  const int rows = (int)sp.n * G, id0 = tile * (16 * NR * kWaves);
+  const int rows = (int)sp.n * G, id0 = tile * (16 * kWaves);
   if (id0 >= rows) return;
   const int lane = threadIdx.x & 63, r16 = lane & 15, cg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wid0 = id0 + wave * (16 * NR);  // the wave's first row
-  int id_last = id0 + 16 * NR * kWaves - 1;
+  int id_last = id0 + 16 * kWaves - 1;
   id_last = id_last < rows ? id_last : rows - 1;
   const int64_t p_last = sp.p0 + id_last / G;  // the last position any row sees
   const int nb = (int)(p_last / kBlk) + 1, nc = (nb + 1) / 2;
-  const int64_t lim0 = sp.p0 + wid0 / G;       // the wave's first row's last position
-  QRow<HD> qr[NR];
-  RowState<HD> s[NR];
-  int64_t lim[NR];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int id = wid0 + 16 * n + r16;
-    const bool live = id < rows;
-    const int tok = live ? id / G : 0;
-    const int g = live ? id - tok * G : 0;
-    lim[n] = sp.p0 + tok;
-    qr[n].template load<false>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, 0,
-                               Rope{});
-    s[n].clear();
-  }
+  // the split's chunks c0 .. c1 - 1, of which every row sees those below n_full whole
+  const int S = gridDim.y, split = blockIdx.y;
+  const int c0 = (int)((int64_t)nc * split / S), c1 = (int)((int64_t)nc * (split + 1) / S);
+  int n_full = (int)((sp.p0 + id0 / G + 1) / (2 * kBlk));
+  n_full = n_full < c1 ? n_full : c1;
+  const int id = id0 + wave * 16 + r16;
+  const bool live = id < rows;
+  const int tok = live ? id / G : 0, g = live ? id - tok * G : 0;
+  const int64_t lim = sp.p0 + tok, qo = ((int64_t)tok * n_head + kvh * G + g) * HD;
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  const int8_t *kb = c.k + kvh * n_blocks * (kBlk * HD), *vb = c.v + kvh * n_blocks * (kBlk * HD);
+  const int8_t *kb = c.k + kvh * n_blocks * (kBlk * HD) + r16 * HD + 16 * cg;
+  const int8_t *vb = c.v + kvh * n_blocks * (kBlk * HD) + r16 * 64 + 16 * cg;
   const float *ksc = c.k_scale + kvh * n_blocks, *vsc = c.v_scale + kvh * n_blocks;
-  const int8_t *kl0 = kb + r16 * HD + 16 * cg, *vl0 = vb + r16 * 64 + 16 * cg;
   u4v rk[NU], rv[NU];
-  float ks[2], vs[2], nks[2], nvs[2];
-  auto fetch = [&](int ch) {  // (block numbers are the wave's: scalar)
-    const int64_t b0 = 2 * ch, b1 = 2 * ch + 1 < nb ? 2 * ch + 1 : nb - 1;  // (b1 past: masked)
-    nks[0] = load_const(ksc + b0);
-    nks[1] = load_const(ksc + b1);
-    nvs[0] = load_const(vsc + b0);
-    nvs[1] = load_const(vsc + b1);
+  // block 2 ch + u, the last one past the end (a partner that is masked, or a
+  // chunk that is not used); block numbers are the wave's: scalar
+  auto block = [&](int ch, int u) { return (int64_t)(2 * ch + u < nb ? 2 * ch + u : nb - 1); };
+  auto fetch_k = [&](int ch) {
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int x = wave + kWaves * i;
-      const int pt = x / KJ, jj = x % KJ, u = x / VJ, jv = x % VJ;
+      const int x = wave + kWaves * i, pt = x / KJ, jj = x % KJ;
       rk[i] = *reinterpret_cast<const u4v *>(
-          kl0 + ((pt >> 1 ? b1 : b0) * kBlk + 16 * (pt & 1)) * HD + 64 * jj);
-      rv[i] = *reinterpret_cast<const u4v *>(vl0 + (u ? b1 : b0) * (kBlk * HD) + 1024 * jv);
+          kb + (block(ch, pt >> 1) * kBlk + 16 * (pt & 1)) * HD + 64 * jj);
     }
   };
-  fetch(0);
-  for (int ch = 0; ch < nc; ++ch) {
-    __syncthreads();  // the previous chunk is consumed
+  auto fetch_v = [&](int ch) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int x = wave + kWaves * i, u = x / VJ, jv = x % VJ;
+      rv[i] = *reinterpret_cast<const u4v *>(vb + block(ch, u) * (kBlk * HD) + 1024 * jv);
+    }
+  };
+  auto stage = [&](const u4v (&r)[NU], h8 (*dst)[64]) {
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int x = wave + kWaves * i;
-      codes16(rk[i], kl[2 * x][lane], kl[2 * x + 1][lane]);
-      codes16(rv[i], vl[2 * x][lane], vl[2 * x + 1][lane]);
+      codes16(r[i], dst[2 * x][lane], dst[2 * x + 1][lane]);
     }
+  };
+  auto scales = [&](int ch, float (&ks)[2], float (&vs)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      ks[u] = load_const(ksc + block(ch, u));
+      vs[u] = load_const(vsc + block(ch, u));
+    }
+  };
+  QRow<HD> qr;
+  RowState<HD> s;
+  s.clear();
+  auto scores = [&](const h8 (*k)[64], f4v (&sc)[4]) {
+#pragma unroll
+    for (int pt = 0; pt < 4; ++pt) sc[pt] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int p0 = 0; p0 < 4; p0 += AHEAD) {
+        h8 kf[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kf[i] = k[(p0 + i) * KS + ks][lane];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          sc[p0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qr.lo[ks], sc[p0 + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          sc[p0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qr.hi[ks], sc[p0 + i], 0, 0, 0);
+      }
+  };
+  float ks[2], vs[2];
+  auto pass = [&](int ch, f4v (&sc)[4], f4v (&next)[4], auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const int odd = (ch - c0) & 1;
+    stage(rk, kl[odd]);
+    stage(rv, vl[odd ^ 1]);
+    fetch_k(ch + 3);
+    fetch_v(ch + 2);
+    float nks[2], nvs[2];
+    scales(ch + 1, nks, nvs);
+    scores(kl[odd ^ 1], next);
+    h8 ph[2], pl[2];
+    int last[2] = {0, 0};
+    if constexpr (MASK) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int64_t d = lim - ((int64_t)(2 * ch + u) * kBlk + 4 * cg);
+        last[u] = (int)(d > 64 ? 64 : d < -1 ? -1 : d);
+      }
+    }
+    softmax_step<HD, 2, MASK>(s, sc, qr.f, ks, vs, last, ph, pl);
+    const h8 (*v)[64] = vl[odd];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h0 = 0; h0 < 2 * VJ; h0 += AHEAD) {
+        h8 vf[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) vf[i] = v[2 * u * VJ + h0 + i][lane];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          s.o[h0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pl[u], s.o[h0 + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          s.o[h0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], ph[u], s.o[h0 + i], 0, 0, 0);
+      }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       ks[u] = nks[u];
       vs[u] = nvs[u];
     }
     __syncthreads();
-    if (ch + 1 < nc) fetch(ch + 1);
-    f4v sc[NR][4];
-#pragma unroll
-    for (int pt = 0; pt < 4; ++pt) {
-#pragma unroll
-      for (int n = 0; n < NR; ++n) sc[n][pt] = f4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const h8 kf = kl[pt * KS + k][lane];
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          sc[n][pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qr[n].lo[k], sc[n][pt], 0, 0, 0);
-          sc[n][pt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qr[n].hi[k], sc[n][pt], 0, 0, 0);
-        }
-      }
-    }
-    h8 ph[NR][2], pl[NR][2];
-    const int64_t first = (int64_t)ch * (2 * kBlk);
-    if (first + 2 * kBlk - 1 > lim0) {  // (uniform)
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        int last[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int64_t d = lim[n] - first - 32 * u - 4 * cg;
-          last[u] = (int)(d > 64 ? 64 : d < -1 ? -1 : d);
-        }
-        softmax_step<HD, 2, true>(s[n], sc[n], qr[n].f, ks, vs, last, ph[n], pl[n]);
-      }
-    } else {
-      const int last[2] = {0, 0};
-#pragma unroll
-      for (int n = 0; n < NR; ++n)
-        softmax_step<HD, 2, false>(s[n], sc[n], qr[n].f, ks, vs, last, ph[n], pl[n]);
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int ht = 0; ht < 2 * VJ; ++ht) {
-        const h8 vf = vl[2 * u * VJ + ht][lane];
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          s[n].o[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[n][u], s[n].o[ht], 0, 0, 0);
-          s[n].o[ht] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[n][u], s[n].o[ht], 0, 0, 0);
-        }
-      }
+  };
+  fetch_k(c0);
+  fetch_v(c0);
+  scales(c0, ks, vs);
+  qr.template load<false>(q + qo, live, cg, scale, 0, Rope{});
+  stage(rk, kl[0]);
+  stage(rv, vl[0]);
+  fetch_k(c0 + 1);
+  fetch_v(c0 + 1);
+  stage(rk, kl[1]);
+  fetch_k(c0 + 2);
+  __syncthreads();
+  f4v sa[4], sb[4];
+  scores(kl[0], sa);
+  __syncthreads();  // (the first chunk's keys have been read)
+  int ch = c0;
+  for (; ch + 1 < n_full; ch += 2) {
+    pass(ch, sa, sb, std::false_type());
+    pass(ch + 1, sb, sa, std::false_type());
   }
+  for (; ch < c1; ++ch) {
+    pass(ch, sa, sb, std::true_type());
 #pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int id = wid0 + 16 * n + r16;
-    const float den = row_sum(s[n].l);
-    if (id >= rows) continue;
-    const int tok = id / G;
-    const OutScale fin(s[n].R, s[n].m, den);
-    float *dst = out + ((int64_t)tok * n_head + kvh * G + (id - tok * G)) * HD + 8 * cg;
+    for (int i = 0; i < 4; ++i) sa[i] = sb[i];
+  }
+  const float den = row_sum(s.l);
+  if (!live) return;
+  const OutScale fin(s.R, s.m, den);
+  float *dst = S == 1 ? out + qo : part + (((int64_t)kvh * T * G + id) * S + split) * (HD + 4);
+  if (S > 1 && cg == 0) *reinterpret_cast<f4v *>(dst + HD) = f4v{s.m, s.R, den, 0.f};
 #pragma unroll
-    for (int i = 0; i < VJ; ++i) {
-      const f4v a = fin(s[n].o[2 * i]), b = fin(s[n].o[2 * i + 1]);
-      f4v *o4 = reinterpret_cast<f4v *>(dst + 32 * i);
-      o4[0] = f4v{a[0], b[0], a[1], b[1]};
-      o4[1] = f4v{a[2], b[2], a[3], b[3]};
-    }
+  for (int i = 0; i < VJ; ++i) {
+    f4v a = s.o[2 * i], b = s.o[2 * i + 1];
+    if (S == 1) a = fin(a), b = fin(b);
+    f4v *o4 = reinterpret_cast<f4v *>(dst + 8 * cg + 32 * i);
+    o4[0] = f4v{a[0], b[0], a[1], b[1]};
+    o4[1] = f4v{a[2], b[2], a[3], b[3]};
   }
 }
 
@@ -1160,7 +1201,13 @@ __global__ void __launch_bounds__(64 * kWaves)
 bool kv8_supported(int head_dim) { return head_dim == 64 || head_dim == 128 || head_dim == 256; }
 
 // partials of at most this many (query row, split)s
-constexpr int64_t kScratchRows = 16384;
+constexpr int64_t kScratchRows = 65536;
+// most rows per kv head for the split kernel: it converts every block once per
+// tile of 16 rows, the tiles kernel once per 64, but by way of LDS and barriers.
+// 32/8 heads of 128 after 8000 positions, split against tiles: 32 rows 14.8 / 20.5
+// us, 64 18.2 / 20.6, 128 24.1 / 26.3, 256 36.0 / 38.9; heads of 256 (groups of 2):
+// 64 rows 24.9 / 26.1, 128 30.7 / 30.2.
+constexpr int64_t kSplitRows = 256;
 size_t kv8_scratch_bytes(int head_dim) {
   return (size_t)kScratchRows * (head_dim + 4) * sizeof(float);
 }
@@ -1196,16 +1243,16 @@ hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, 
   return hipGetLastError();
 }
 
-// The splits of the positions for T tokens: about two workgroups per CU, no
-// more than the cache's blocks give every wave one of, nor than the scratch
-// holds.  By the cache's length, not by the position, which the host may not
-// know: a call gives the same bits however it is told where it is.
-int kv8_splits(const aq_kv8 &c, int64_t T, int n_head) {
-  const int64_t G = n_head / c.n_kv, tiles = (T * G + 15) / 16;
-  const int64_t blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  int64_t S = (blocks + kWaves - 1) / kWaves;
+// The splits of the positions for `tiles` row tiles per kv head and `rows` query
+// rows in all: about two workgroups per CU, no more than give each `blocks` of the
+// cache's blocks, nor than the scratch holds (and one left for the step's last).
+// By the cache's length, not by the position, which the host may not know: a
+// call gives the same bits however it is told where it is.
+int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int blocks) {
+  const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
+  int64_t S = (n_blocks + blocks - 1) / blocks;
   const int64_t fill = (kMaxSplits - 1 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
-  const int64_t room = kScratchRows / (T * n_head) - 1;  // (the step's last one)
+  const int64_t room = kScratchRows / rows - 1;
   S = S < fill ? S : fill;
   S = S < room ? S : room;
   return (int)(S < 1 ? 1 : S);
@@ -1217,29 +1264,38 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
   const float scale = (float)(1.0 / sqrt((double)c.head_dim));
   const int G = n_head / c.n_kv;
   const int64_t rows = T * G;
-  if (rows <= 64) {
-    const int S = kv8_splits(c, T, n_head);
+  int S;
+  if (rows <= kSplitRows) {
+    const int64_t tiles = (rows + 15) / 16;
+    S = kv8_splits(c, tiles, T * n_head, kWaves);
     AQ_HD(c.head_dim,
           hipLaunchKernelGGL((k_kv8_split<HD, false>),
-                             dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)((rows + 15) / 16)),
+                             dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
                              dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale, c.scratch, out,
-                             nullptr, nullptr, Rope{});
-          if (S > 1) hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)rows, (unsigned)c.n_kv),
-                                        dim3(kWG), 0, s, c.scratch, st, pos0, c.n_ctx, T, G, S,
-                                        out))
-    return hipGetLastError();
+                             nullptr, nullptr, Rope{}))
+  } else {
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) return e;
+    const int cus = device_info(dev).cus;
+    const int layer = cus / c.n_kv > 1 ? cus / c.n_kv : 1;
+    const int64_t tiles = (rows + 16 * kWaves - 1) / (16 * kWaves);
+    // Splits of 64 blocks at least: their states go through memory, 2 KB and
+    // more a row (256 tokens of 32/8 heads of 128: 172 -> 95 us by four splits of
+    // 8600 positions, 33 -> 42 us by four of 1600).
+    S = kv8_splits(c, tiles, T * n_head, 64);
+    const int lds = 512 * c.head_dim;  // two chunks of K and of V in fp16
+    AQ_HD(c.head_dim,
+          if (hipError_t e = set_dynamic_lds(reinterpret_cast<const void *>(k_kv8_tiles<HD>), lds))
+            return e;
+          hipLaunchKernelGGL(k_kv8_tiles<HD>, dim3((unsigned)(tiles * c.n_kv), (unsigned)S),
+                             dim3(64 * kWaves), lds, s, q, c, st, pos0, T, G, scale, (int)tiles,
+                             layer, c.scratch, out))
   }
-  int dev = 0;
-  if (hipError_t e = hipGetDevice(&dev)) return e;
-  const int cus = device_info(dev).cus;
-  const int layer = cus / c.n_kv > 1 ? cus / c.n_kv : 1;
-#define AQ_TILES(NR)                                                                          \
-  hipLaunchKernelGGL((k_kv8_tiles<HD, NR>),                                                   \
-                     dim3((unsigned)((rows + 64 * NR - 1) / (64 * NR) * c.n_kv)),             \
-                     dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale,                    \
-                     (int)((rows + 64 * NR - 1) / (64 * NR)), layer, out)
-  AQ_HD(c.head_dim, AQ_TILES(1))
-#undef AQ_TILES
+  if (S > 1) {
+    AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)rows, (unsigned)c.n_kv),
+                                         dim3(kWG), 0, s, c.scratch, st, pos0, c.n_ctx, T, G, S,
+                                         out))
+  }
   return hipGetLastError();
 }
 
@@ -1249,7 +1305,7 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      float *out, hipStream_t s) {
   const float scale = (float)(1.0 / sqrt((double)c.head_dim));
   const int G = n_head / c.n_kv;
-  const int S = kv8_splits(c, 1, n_head) + 1;
+  const int S = kv8_splits(c, 1, n_head, kWaves) + 1;
   AQ_HD(c.head_dim,
         hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
                            dim3(64 * kWaves), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
