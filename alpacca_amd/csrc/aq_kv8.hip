@@ -1007,6 +1007,45 @@ __global__ void __launch_bounds__(kWG)
   reinterpret_cast<f4v *>(out + ((int64_t)t * n_head + kvh * G + (id - t * G)) * HD)[d4] = fin(o);
 }
 
+// The merge of up to kFewSplits splits of many rows: HD / 4 threads per row, all
+// its loads in flight at once, no LDS.
+constexpr int kFewSplits = 8;
+template <int HD>
+__global__ void __launch_bounds__(kWG)
+    k_kv8_combine_few(const float *__restrict__ part, const aq_decode_state *st, int64_t pos0,
+                      int64_t n_ctx, int64_t T, int G, int S, float *__restrict__ out) {
+  constexpr int PS = HD + 4, LP = HD / 4;
+  const int id = blockIdx.x * (kWG / LP) + threadIdx.x / LP, d4 = threadIdx.x % LP;
+  const int kvh = blockIdx.y, n_head = gridDim.y * G, t = id / G;
+  const Span sp = span_of(st, pos0, T, n_ctx);
+  if (t >= sp.n) return;
+  const float *p = part + ((int64_t)kvh * T * G + id) * S * PS;
+  f4v x[kFewSplits], e[kFewSplits];  // numerators; m, R, l
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float *ps = p + (s < S ? s : 0) * PS;
+    x[s] = *reinterpret_cast<const f4v *>(ps + 4 * d4);
+    e[s] = *reinterpret_cast<const f4v *>(ps + HD);
+  }
+  float M = -INFINITY, R = kLow;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {  // (repeats of the first split change no maximum)
+    M = fmaxf(M, e[s][0]);
+    R = fmaxf(R, e[s][1]);
+  }
+  const float mref = M == -INFINITY ? 0.f : M;
+  f4v o = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    if (s >= S) break;
+    o += x[s] * exp2_(e[s][1] - R);
+    den = fmaf(e[s][2], exp2_(e[s][0] - mref), den);
+  }
+  const OutScale fin(R, M, den);
+  reinterpret_cast<f4v *>(out + ((int64_t)t * n_head + kvh * G + (id - t * G)) * HD)[d4] = fin(o);
+}
+
 // ---- many rows: tiles of rows over all positions they see -------------------------
 // One workgroup of four waves per 64 rows (16 per wave) of a kv head and split of
 // the positions (gridDim.y of them; one writes the output, several their states
@@ -1243,19 +1282,39 @@ hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, 
   return hipGetLastError();
 }
 
-// The splits of the positions for `tiles` row tiles per kv head and `rows` query
-// rows in all: about two workgroups per CU, no more than give each `blocks` of the
-// cache's blocks, nor than the scratch holds (and one left for the step's last).
-// By the cache's length, not by the position, which the host may not know: a
-// call gives the same bits however it is told where it is.
-int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int blocks) {
+// The splits of the positions.  Both rules go by the cache's length, not by the
+// position, which the host may not know: a call gives the same bits however it
+// is told where it is.
+//
+// The split kernel: about two workgroups per CU, no more than give every wave a
+// block of a full cache, nor than the scratch holds (the step has one more).
+int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows) {
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  int64_t S = (n_blocks + blocks - 1) / blocks;
+  int64_t S = (n_blocks + kWaves - 1) / kWaves;
   const int64_t fill = (kMaxSplits - 1 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
   const int64_t room = kScratchRows / rows - 1;
   S = S < fill ? S : fill;
   S = S < room ? S : room;
   return (int)(S < 1 ? 1 : S);
+}
+// The tiles kernel: the smallest estimate.  A workgroup takes about head_dim / 96
+// us per chunk, two on a CU 1.3 times that, more in turn; the splits' states go
+// through memory once each way, in a launch of its own.  32/8 heads of 128: 256
+// tokens at 8000 172 us whole, 85 split; 64 of heads of 256 (groups of 2) at 1000 56, 27.
+int kv8_tile_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int cus) {
+  const double chunks = (double)((c.n_ctx + 2 * kBlk - 1) / (2 * kBlk));
+  double best = 0.0;
+  int pick = 1;
+  for (int S = 1; S <= kFewSplits && S <= chunks && (S == 1 || rows * S <= kScratchRows); ++S) {
+    const double turns = ceil((double)(tiles * c.n_kv * S) / cus);
+    const double t = ceil(chunks / S) * (c.head_dim / 96.0) * (turns > 1 ? 0.65 * turns : 1.0) +
+                     (S > 1 ? 4.0 + (double)rows * S * (c.head_dim + 4) * 8 / 4e6 : 0.0);
+    if (S == 1 || t < best) {
+      best = t;
+      pick = S;
+    }
+  }
+  return pick;
 }
 
 hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int n_head,
@@ -1267,7 +1326,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
   int S;
   if (rows <= kSplitRows) {
     const int64_t tiles = (rows + 15) / 16;
-    S = kv8_splits(c, tiles, T * n_head, kWaves);
+    S = kv8_splits(c, tiles, T * n_head);
     AQ_HD(c.head_dim,
           hipLaunchKernelGGL((k_kv8_split<HD, false>),
                              dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
@@ -1279,10 +1338,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
     const int cus = device_info(dev).cus;
     const int layer = cus / c.n_kv > 1 ? cus / c.n_kv : 1;
     const int64_t tiles = (rows + 16 * kWaves - 1) / (16 * kWaves);
-    // Splits of 64 blocks at least: their states go through memory, 2 KB and
-    // more a row (256 tokens of 32/8 heads of 128: 172 -> 95 us by four splits of
-    // 8600 positions, 33 -> 42 us by four of 1600).
-    S = kv8_splits(c, tiles, T * n_head, 64);
+    S = kv8_tile_splits(c, tiles, T * n_head, cus);
     const int lds = 512 * c.head_dim;  // two chunks of K and of V in fp16
     AQ_HD(c.head_dim,
           if (hipError_t e = set_dynamic_lds(reinterpret_cast<const void *>(k_kv8_tiles<HD>), lds))
@@ -1291,7 +1347,13 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
                              dim3(64 * kWaves), lds, s, q, c, st, pos0, T, G, scale, (int)tiles,
                              layer, c.scratch, out))
   }
-  if (S > 1) {
+  if (S > 1 && S <= kFewSplits) {
+    AQ_HD(c.head_dim,
+          constexpr int R = kWG / (HD / 4);
+          hipLaunchKernelGGL(k_kv8_combine_few<HD>,
+                             dim3((unsigned)((rows + R - 1) / R), (unsigned)c.n_kv), dim3(kWG), 0,
+                             s, c.scratch, st, pos0, c.n_ctx, T, G, S, out))
+  } else if (S > 1) {
     AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)rows, (unsigned)c.n_kv),
                                          dim3(kWG), 0, s, c.scratch, st, pos0, c.n_ctx, T, G, S,
                                          out))
@@ -1305,7 +1367,7 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      float *out, hipStream_t s) {
   const float scale = (float)(1.0 / sqrt((double)c.head_dim));
   const int G = n_head / c.n_kv;
-  const int S = kv8_splits(c, 1, n_head, kWaves) + 1;
+  const int S = kv8_splits(c, 1, n_head) + 1;
   AQ_HD(c.head_dim,
         hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
                            dim3(64 * kWaves), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
