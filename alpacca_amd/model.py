@@ -11,7 +11,12 @@ Mirrors the reference's ``Model`` where it touches the hot path:
   (model.py:610-641; prompt tokens run through the decode step one by one,
   which computes the same function as the reference's chunked forward_batch);
 * ``generate_greedy(prompt, n)`` - ``n`` greedy tokens after the prompt
-  (argmax of the logits, tensor.py:187-194, fed back as the next token).
+  (argmax of the logits, tensor.py:187-194, fed back as the next token),
+  with the reference sampler's repetition penalty, or presence and frequency
+  penalties, per-token biases and a mask of allowed tokens (logits.py).
+
+``Model(..., kv_dtype="q8")`` keeps the KV cache in 8 bits (kvcache.py): a
+quarter of the fp32 cache's bytes, which the reference keeps.
 
 Layer weights, KV cache, activations, position and token all stay in HBM.
 One decode step is a fixed sequence of kernel launches that reads the token
@@ -32,6 +37,9 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
+from .kvcache import BLOCK as KV_BLOCK
+from .kvcache import QuantKVCache
+from .logits import adjust_logits, pack_mask
 from .qmatrix import (DENSE_DTYPES, MIXABLE_DTYPES, DenseMatrix, QuantMatrix,
                       interleave_rows, matvec_fused_device, matvec_multi_device,
                       pair_rows_supported)
@@ -84,8 +92,10 @@ class Model:
     """Greedy decode of a model given as a dict of Tensors (GGUF names)."""
 
     def __init__(self, hp: Hyperparams, tensors: dict, n_ctx: int = 0, layout=None,
-                 fused: bool = True):
+                 fused: bool = True, kv_dtype: str = "f32"):
         import torch
+        if kv_dtype not in ("f32", "q8"):
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r} (f32, q8)")
         if not torch.cuda.is_available():
             raise RuntimeError("alpacca_amd.model.Model needs a HIP device (gfx950)")
         _lib.ensure_device()
@@ -175,7 +185,15 @@ class Model:
         cos, sin = rope_tables(hp, self.n_ctx)
         self.rope_cos = torch.from_numpy(np.ascontiguousarray(cos)).to(self.dev)
         self.rope_sin = torch.from_numpy(np.ascontiguousarray(sin)).to(self.dev)
-        self.kv = torch.zeros((hp.n_layer, 2, hp.n_kv, self.n_ctx, hp.head_dim), **f32)
+        # one fp32 tensor, or an 8-bit cache per layer (their calls are ordered
+        # on self.stream, so they share one scratch)
+        self.kv_dtype = kv_dtype
+        self.kv, self.kv8 = None, []
+        if kv_dtype == "f32":
+            self.kv = torch.zeros((hp.n_layer, 2, hp.n_kv, self.n_ctx, hp.head_dim), **f32)
+        for _ in range(hp.n_layer if kv_dtype == "q8" else 0):
+            self.kv8.append(QuantKVCache(hp.n_kv, self.n_ctx, hp.head_dim, self.dev,
+                                         scratch=self.kv8[0] if self.kv8 else None))
         self.x = torch.zeros(hp.n_embd, **f32)
         self.h = torch.zeros(hp.n_embd, **f32)
         self.o = torch.zeros(hp.n_embd, **f32)
@@ -233,7 +251,6 @@ class Model:
         p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
         sv = ctypes.c_void_p(s)
         for li, ly in enumerate(self.layers):
-            kc, vc = self.kv[li, 0], self.kv[li, 1]
             if self.fused:
                 self._matvecs([ly["attn_q"], ly["attn_k"], ly["attn_v"]],
                               [self.q, self.k, self.v], self.x, s, norm=ly["attn_norm"])
@@ -246,12 +263,25 @@ class Model:
                 if ly[b + ".bias"] is not None:
                     chk(lib.aq_add(p(out), p(ly[b + ".bias"]), out.numel(), sv))
             neox = 1 if hp.rope_style == "neox" else 0
-            if self.fused and not (neox and hp.n_rot % 8):
+            one_call = self.fused and not (neox and hp.n_rot % 8)
+            if self.kv8 and one_call:
+                chk(lib.aq_attention_rope_kv8(
+                    p(self.q), p(self.k), p(self.v), hp.n_head, hp.n_rot, neox, p(self.rope_cos),
+                    p(self.rope_sin), ctypes.c_void_p(st), 0, self.kv8[li].handle, p(self.att), sv))
+            elif self.kv8:
+                chk(lib.aq_rope_kv8(p(self.q), p(self.k), p(self.v), p(self.q), 1, hp.n_head,
+                                    hp.n_rot, neox, p(self.rope_cos), p(self.rope_sin),
+                                    ctypes.c_void_p(st), 0, self.kv8[li].handle, sv))
+                chk(lib.aq_attention_kv8(p(self.q), self.kv8[li].handle, 1, hp.n_head,
+                                         ctypes.c_void_p(st), 0, p(self.att), sv))
+            elif one_call:
+                kc, vc = self.kv[li, 0], self.kv[li, 1]
                 chk(lib.aq_attention_rope(p(self.q), p(self.k), p(self.v), hp.n_head, hp.n_kv,
                                           hp.head_dim, hp.n_rot, neox, p(self.rope_cos),
                                           p(self.rope_sin), ctypes.c_void_p(st), 0,
                                           self.n_ctx, p(kc), p(vc), p(self.att), sv))
             else:
+                kc, vc = self.kv[li, 0], self.kv[li, 1]
                 chk(lib.aq_rope_kv(p(self.q), p(self.k), p(self.v), 1, hp.n_head, hp.n_kv,
                                    hp.head_dim, hp.n_rot, neox, p(self.rope_cos),
                                    p(self.rope_sin), ctypes.c_void_p(st), 0, self.n_ctx,
@@ -380,6 +410,9 @@ class Model:
             n = max(0, len(tokens) - 1)
         if n != self.n_past:
             n = min(n, self.n_past)
+            # an 8-bit cache goes back inside its last block, or to a block's start
+            if self.kv8 and n // KV_BLOCK != (self.n_past - 1) // KV_BLOCK:
+                n -= n % KV_BLOCK
             self.n_past = n
             del self.cached_ids[n:]
         suffix = list(tokens[n:])
@@ -445,17 +478,24 @@ class Model:
                 chk(lib.aq_rmsnorm(p(X), p(self.layers[0]["attn_norm"]), T, hp.n_embd, eps,
                                    p(H), sv))
                 for li, ly in enumerate(self.layers):
-                    kc, vc = self.kv[li, 0], self.kv[li, 1]
                     for role, out in (("attn_q", Q), ("attn_k", K), ("attn_v", V)):
                         ly[role].matmul_t_device(H.data_ptr(), T, out.data_ptr(), s, prec)
                         if ly[role + ".bias"] is not None:  # q + bq over the batch
                             chk(lib.aq_add_rows(p(out), p(ly[role + ".bias"]), T,
                                                 out.shape[1], sv))
-                    chk(lib.aq_rope_kv(p(Q), p(K), p(V), T, hp.n_head, hp.n_kv, hp.head_dim,
-                                       hp.n_rot, neox, p(self.rope_cos), p(self.rope_sin),
-                                       None, pos0, self.n_ctx, p(kc), p(vc), sv))
-                    chk(lib.aq_attention_batch(p(Q), p(kc), p(vc), T, hp.n_head, hp.n_kv,
-                                               hp.head_dim, self.n_ctx, None, pos0, p(A), sv))
+                    if self.kv8:
+                        cache = self.kv8[li].handle
+                        chk(lib.aq_rope_kv8(p(Q), p(K), p(V), p(Q), T, hp.n_head, hp.n_rot, neox,
+                                            p(self.rope_cos), p(self.rope_sin), None, pos0, cache,
+                                            sv))
+                        chk(lib.aq_attention_kv8(p(Q), cache, T, hp.n_head, None, pos0, p(A), sv))
+                    else:
+                        kc, vc = self.kv[li, 0], self.kv[li, 1]
+                        chk(lib.aq_rope_kv(p(Q), p(K), p(V), T, hp.n_head, hp.n_kv, hp.head_dim,
+                                           hp.n_rot, neox, p(self.rope_cos), p(self.rope_sin),
+                                           None, pos0, self.n_ctx, p(kc), p(vc), sv))
+                        chk(lib.aq_attention_batch(p(Q), p(kc), p(vc), T, hp.n_head, hp.n_kv,
+                                                   hp.head_dim, self.n_ctx, None, pos0, p(A), sv))
                     ly["attn_output"].matmul_t_device(A.data_ptr(), T, O.data_ptr(), s, prec)
                     chk(lib.aq_add_rmsnorm(p(X), p(O), p(ly["ffn_norm"]), T, hp.n_embd, eps,
                                            p(H), sv))
@@ -505,7 +545,9 @@ class Model:
     def generate_greedy(self, prompt: list[int], n_gen: int, graph: bool = True,
                         timing: dict | None = None, batch_prefill: bool = True,
                         repeat_penalty: float = 1.0, repeat_last_n: int = 64,
-                        steps_per_graph: int = 16) -> list[int]:
+                        steps_per_graph: int = 16, presence_penalty: float = 0.0,
+                        frequency_penalty: float = 0.0, logit_bias: dict | None = None,
+                        allowed=None) -> list[int]:
         """Greedy continuation: n_gen tokens after `prompt` (the loop of
         smoke.py:743-755: logits = prefill(prompt); token = argmax(logits);
         logits = forward(token) ...).  Starts from an empty cache.  The
@@ -524,13 +566,22 @@ class Model:
         repeat_penalty other than 0 and 1 gives the decode loop of
         tests/bench.py:78-90 instead: a temperature-0 Sampler that accepts
         the prompt and every chosen token and penalizes the last
-        max(repeat_last_n, 1) of them (sample.py:31-45), on the device."""
+        max(repeat_last_n, 1) of them (sample.py:31-45), on the device.
+
+        presence_penalty and frequency_penalty are taken off the logits of
+        the window's tokens (the latter once for each time one is in it),
+        logit_bias ({token: bias}) is added, and tokens that `allowed` (n_vocab
+        truth values) leaves out are never chosen: with any of these the
+        logits of every step, the repetition penalty among the rest, go
+        through adjust_logits before the argmax (rounded to float32 there)."""
         torch = self.torch
         if not prompt or n_gen < 1:
             raise ValueError("need a non-empty prompt and n_gen >= 1")
         penalize = bool(repeat_penalty) and repeat_penalty != 1.0
         if penalize and not np.isfinite(repeat_penalty):
             raise ValueError("repeat_penalty must be finite")
+        if not (np.isfinite(presence_penalty) and np.isfinite(frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite")
         if len(prompt) + n_gen - 1 > self.n_ctx:
             raise RuntimeError(f"context window full ({self.n_ctx} tokens)")
         if min(prompt) < 0 or max(prompt) >= self.hp.n_vocab:
@@ -540,6 +591,12 @@ class Model:
         hist = torch.zeros(n_gen, dtype=torch.int64, device=self.dev)
         n_p = len(prompt)
         window = None
+        adjust = self._adjustment(presence_penalty, frequency_penalty, logit_bias, allowed)
+        if adjust is not None and (penalize or presence_penalty or frequency_penalty):
+            adjust["penalties"] = torch.tensor(
+                [[repeat_penalty if penalize else 1.0, presence_penalty, frequency_penalty]],
+                dtype=torch.float64, device=self.dev)
+            penalize = True
         if penalize:  # Sampler.accept of the prompt (tests/bench.py:78-80)
             last_n = max(int(repeat_last_n), 1)
             ring = np.zeros(1 + last_n, dtype=np.int64)
@@ -547,8 +604,14 @@ class Model:
                 ring[1 + i % last_n] = t
             ring[0] = n_p
             window = torch.zeros(1 + last_n, dtype=torch.int64, device=self.dev)
+            if adjust is not None:  # the advance below then only keeps the window
+                adjust["window"] = window.view(1, -1)
+                repeat_penalty = 1.0
 
         def advance():
+            if adjust is not None:
+                logits = self.logits.view(1, -1)
+                adjust_logits(logits, out=logits, **adjust)
             self._enqueue_advance(True, None, hist, window, repeat_penalty)
 
         def prompt_step():
@@ -637,6 +700,32 @@ class Model:
         out = [int(t) for t in hist.cpu().tolist()]
         self.n_past = n_p + n_gen - 1
         self.cached_ids = list(prompt) + out[:-1]
+        return out
+
+    def _adjustment(self, presence: float, frequency: float, bias, allowed) -> dict | None:
+        """adjust_logits' arguments for one row but the window and penalties;
+        None when there is nothing to adjust but a repetition penalty."""
+        torch, n = self.torch, self.hp.n_vocab
+        if not (presence or frequency or bias or allowed is not None):
+            return None
+        out = {}
+        if bias:
+            ids = [int(t) for t in bias]
+            if min(ids) < 0 or max(ids) >= n:
+                raise IndexError("logit_bias token out of range")
+            vals = np.array([float(v) for v in bias.values()], dtype=np.float32)
+            if np.isnan(vals).any():
+                raise ValueError("logit_bias must not be NaN")
+            out["bias"] = (torch.tensor(ids, dtype=torch.int64, device=self.dev),
+                           torch.from_numpy(vals).to(self.dev))
+        if allowed is not None:
+            ok = torch.as_tensor(np.asarray(
+                allowed.cpu() if isinstance(allowed, torch.Tensor) else allowed))
+            if ok.dtype != torch.bool or tuple(ok.shape) != (n,):
+                raise ValueError(f"allowed must hold {n} truth values")
+            if not bool(ok.any()):
+                raise ValueError("allowed leaves no token")
+            out["mask"] = pack_mask(ok.to(self.dev))
         return out
 
     def _capture(self, fn):
