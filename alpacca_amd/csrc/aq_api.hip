@@ -1232,7 +1232,7 @@ int aq_greedy_advance_penalized(const float *logits, int64_t n, aq_decode_state 
 namespace {
 int kv8_check(const aq_kv8 *c) {
   if (!c) return fail(AQ_ERR_VALUE, "cache is NULL");
-  if (c->n_kv <= 0 || c->n_ctx <= 0 || c->n_ctx > INT32_MAX)
+  if (c->n_kv <= 0 || c->n_kv > 65535 || c->n_ctx <= 0 || c->n_ctx > INT32_MAX)
     return fail(AQ_ERR_VALUE, "bad cache shape (n_kv %d, n_ctx %lld)", c->n_kv,
                 (long long)c->n_ctx);
   if (!aq::kv8_supported(c->head_dim))
@@ -1278,7 +1278,8 @@ extern "C" {
 
 int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *scales,
                  size_t *tail, size_t *scratch) {
-  if (n_kv <= 0 || n_ctx <= 0 || n_ctx > INT32_MAX || !aq::kv8_supported(head_dim))
+  if (n_kv <= 0 || n_kv > 65535 || n_ctx <= 0 || n_ctx > INT32_MAX ||
+      !aq::kv8_supported(head_dim))
     return fail(AQ_ERR_VALUE, "bad cache shape (n_kv %d, head_dim %d, n_ctx %lld)", n_kv,
                 head_dim, (long long)n_ctx);
   const size_t blocks = (size_t)n_kv * ((n_ctx + aq::kKv8Block - 1) / aq::kKv8Block);

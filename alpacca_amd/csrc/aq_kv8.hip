@@ -29,11 +29,6 @@ constexpr int kWG = 256;
 
 typedef float f4v __attribute__((ext_vector_type(4)));
 
-// byte of position row (0 .. 31) and dimension d in a V block
-__device__ __forceinline__ int v_byte(int row, int d) {
-  return (d >> 1) * 64 + ((row >> 2) & 3) * 16 + (d & 1) * 8 + (row >> 4) * 4 + (row & 3);
-}
-
 // positions p0 .. p0 + n of a call that lie in the cache (n = 0: none)
 struct Span {
   int64_t p0, n;
@@ -424,21 +419,48 @@ __global__ void __launch_bounds__(kStoreWG<HD>, HD == 256 ? 2 : 4)
 }
 
 // ---- read-back ---------------------------------------------------------------
-// out[kvh][p - start][d] = s c, one product rounded to fp32
+// out[kvh][p - start][d] = s c, one product rounded to fp32.  One workgroup per
+// block of K and of V; a thread turns units of 16 codes into four 16-byte stores
+// (K), or eight 8-byte ones to eight rows (V; 16 lanes fill 128 bytes of a row).
 template <int HD>
-__global__ void __launch_bounds__(kWG)
+__global__ void __launch_bounds__(kStoreWG<HD>)
     k_kv8_read(aq_kv8 c, int64_t start, int64_t n, float *__restrict__ ko,
                float *__restrict__ vo) {
-  const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  const int64_t total = (int64_t)c.n_kv * n * HD;
-  for (int64_t i = (int64_t)blockIdx.x * kWG + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * kWG) {
-    const int d = (int)(i % HD);
-    const int64_t pp = i / HD, kvh = pp / n, p = start + (pp - kvh * n);
-    const int64_t blk = kvh * n_blocks + p / kBlk;
-    const int row = (int)(p % kBlk);
-    ko[i] = c.k_scale[blk] * (float)c.k[blk * (kBlk * HD) + row * HD + d];
-    vo[i] = c.v_scale[blk] * (float)c.v[blk * (kBlk * HD) + v_byte(row, d)];
+  constexpr int NT = kStoreWG<HD>, UPT = BlockTokens<HD>::UNITS / NT;
+  const bool is_v = blockIdx.x & 1;
+  const int64_t b = start / kBlk + (blockIdx.x >> 1), n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
+  const int kvh = blockIdx.y;
+  const uint4 *src =
+      reinterpret_cast<const uint4 *>((is_v ? c.v : c.k) + (kvh * n_blocks + b) * (kBlk * HD));
+  const float s = (is_v ? c.v_scale : c.k_scale)[kvh * n_blocks + b];
+  // row r of the block is output row first + r, where lo <= r < hi
+  const int64_t first = b * kBlk - start, left = n - first;
+  const int lo = first < 0 ? (int)-first : 0, hi = left < kBlk ? (int)left : kBlk;
+  float *out = (is_v ? vo : ko) + (kvh * n + first) * HD;
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    const int u = threadIdx.x + NT * i;
+    const uint4 w = src[u];
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = s * (float)(int8_t)(ws[e >> 2] >> (8 * (e & 3)));
+    if (!is_v) {
+      const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
+      if (row < lo || row >= hi) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<f4u *>(out + row * HD + d0 + 4 * k) =
+            f4u{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int row = BlockTokens<HD>::v_row(u, k);
+      if (row < lo || row >= hi) continue;
+      typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+      *reinterpret_cast<f2u *>(out + row * HD + 2 * (u >> 2)) = f2u{x[k], x[8 + k]};
+    }
   }
 }
 
@@ -1251,11 +1273,11 @@ size_t kv8_scratch_bytes(int head_dim) {
   return (size_t)kScratchRows * (head_dim + 4) * sizeof(float);
 }
 
-#define AQ_HD(hd, CALL)                                   \
+#define AQ_HD(hd, ...)                                    \
   switch (hd) {                                           \
-    case 64: { constexpr int HD = 64; CALL; } break;      \
-    case 128: { constexpr int HD = 128; CALL; } break;    \
-    case 256: { constexpr int HD = 256; CALL; } break;    \
+    case 64: { constexpr int HD = 64; __VA_ARGS__; } break;      \
+    case 128: { constexpr int HD = 128; __VA_ARGS__; } break;    \
+    case 256: { constexpr int HD = 256; __VA_ARGS__; } break;    \
     default: return hipErrorInvalidValue;                 \
   }
 
@@ -1275,10 +1297,10 @@ hipError_t launch_rope_kv8(const float *q, const float *k, const float *v, float
 
 hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, float *v,
                            hipStream_t s) {
-  const int64_t total = (int64_t)c.n_kv * n * c.head_dim;
-  const int64_t wg = (total + kWG - 1) / kWG < 8192 ? (total + kWG - 1) / kWG : 8192;
-  AQ_HD(c.head_dim, hipLaunchKernelGGL(k_kv8_read<HD>, dim3((unsigned)wg), dim3(kWG), 0, s, c,
-                                       start, n, k, v))
+  const int64_t blocks = (start + n - 1) / kBlk - start / kBlk + 1;
+  AQ_HD(c.head_dim,
+        hipLaunchKernelGGL(k_kv8_read<HD>, dim3((unsigned)(2 * blocks), (unsigned)c.n_kv),
+                           dim3(kStoreWG<HD>), 0, s, c, start, n, k, v))
   return hipGetLastError();
 }
 

@@ -245,6 +245,29 @@ def test_store_leaves_other_blocks_and_strided_inputs():
 
 
 @gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_read_ranges(hd):
+    """Any range of positions, from and to the middle of blocks, and nothing
+    past it."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd)
+    _, k, v = inputs(rng, 100, 3, 3, hd)
+    cache = QuantKVCache(3, 101, hd)
+    cache.store(flat(k), flat(v), 0)
+    want = [values64(*coded(x)).astype(np.float32).transpose(1, 0, 2) for x in (k, v)]
+    for a, b in ((0, 100), (5, 6), (31, 33), (32, 64), (40, 41), (63, 100), (99, 100), (17, 17)):
+        for got, w in zip(cache.read(a, b), want):
+            assert np.array_equal(got.cpu().numpy(), w[:, a:b]), (a, b)
+    pad = torch.full((2, 3 * 7 * hd + 8), 9.0, device="cuda")
+    _lib.check(_lib.load().aq_kv8_read(cache.handle, 29, 7, pad[0, 3:].data_ptr(),
+                                       pad[1, 5:].data_ptr(), None))
+    for i, off in ((0, 3), (1, 5)):
+        row = pad[i].cpu().numpy()
+        assert np.array_equal(row[off:off + 21 * hd], want[i][:, 29:36].reshape(-1))
+        assert (row[:off] == 9).all() and (row[off + 21 * hd:] == 9).all()
+
+
+@gpu
 def test_store_nonfinite_blocks():
     """A block with an infinity or a NaN reads as NaN, its neighbours as
     they are; without it (gone back) the block is itself again."""
