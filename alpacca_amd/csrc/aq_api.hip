@@ -1285,7 +1285,8 @@ int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *s
   const size_t blocks = (size_t)n_kv * ((n_ctx + aq::kKv8Block - 1) / aq::kKv8Block);
   if (codes) *codes = blocks * aq::kKv8Block * head_dim;
   if (scales) *scales = blocks * sizeof(float);
-  if (tail) *tail = (size_t)n_kv * aq::kKv8Block * head_dim * sizeof(float);
+  // the fp32 block of every kv head, and its number
+  if (tail) *tail = ((size_t)n_kv * aq::kKv8Block * head_dim + (n_kv + 3) / 4 * 4) * sizeof(float);
   if (scratch) *scratch = aq::kv8_scratch_bytes(head_dim);
   return AQ_OK;
 }

@@ -6,6 +6,8 @@
 // s c.  The last block stored is kept in fp32 too (the tail), so a block that a
 // token joins is coded anew from its own values: the codes are a function of
 // the tokens alone, not of the calls that brought them, and no error adds up.
+// A call that goes back inside an earlier block, whose fp32 values are gone,
+// takes them from the codes (the tail's tag names the block it holds).
 //
 // Layouts (n_blocks = ceil(n_ctx / 32) per kv head):
 //   K codes [n_kv][n_blocks][32 positions][head_dim]
@@ -14,7 +16,8 @@
 //     side by side: what a lane of the matrix instructions takes as its operand
 //     (the scores' lanes hold the weights of these positions), two dimensions
 //     per 16-byte load
-//   scales [n_kv][n_blocks] fp32; tails [n_kv][32][head_dim] fp32.
+//   scales [n_kv][n_blocks] fp32; tails [n_kv][32][head_dim] fp32, and behind
+//   them the block that each kv head's tail holds, [n_kv] int32
 #include <math.h>
 
 #include <type_traits>
@@ -229,16 +232,28 @@ template <int HD>
 struct BlockTokens {
   static constexpr int UNITS = kBlk * HD / 16;
   bool is_v, by4;
-  float *tail;         // rows before the call's tokens
+  float *tail;         // rows before the call's tokens, if *tag is their block
+  int32_t *tag;
+  const uint4 *codes;  // the block's
+  const float *scale;
   const float *first;  // where the call's token of row 0 would be
   int64_t stride;      // from a token to the next
   int before, end;     // rows 0 .. before - 1 from the tail, before .. end - 1 the call's
   int64_t pos;         // the position of row 0
   Rope rope;
   // block b of a call's tokens sp at x (the head's vector of the first of them)
-  __device__ __forceinline__ BlockTokens(bool is_v, bool by4, const float *x, int64_t stride,
-                                         float *tail, const Span &sp, int64_t b, const Rope &rope)
-      : is_v(is_v), by4(by4), tail(tail), stride(stride), rope(rope) {
+  __device__ __forceinline__ BlockTokens(const aq_kv8 &c, int kvh, bool is_v, bool by4,
+                                         const float *x, const Span &sp, int64_t b,
+                                         const Rope &rope)
+      : is_v(is_v), by4(by4), stride((int64_t)c.n_kv * HD), rope(rope) {
+    const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
+    float *tails = is_v ? c.v_tail : c.k_tail;
+    tail = tails + (int64_t)kvh * kBlk * HD;
+    tag = reinterpret_cast<int32_t *>(tails + (int64_t)c.n_kv * kBlk * HD) + kvh;
+    codes = reinterpret_cast<const uint4 *>((is_v ? c.v : c.k) +
+                                            (kvh * n_blocks + b) * (kBlk * HD));
+    scale = (is_v ? c.v_scale : c.k_scale) + kvh * n_blocks + b;
+    x += kvh * HD;
     pos = b * kBlk;
     const int64_t lead = sp.p0 - pos, e = lead + sp.n;
     first = x - lead * stride;
@@ -284,14 +299,27 @@ struct BlockTokens {
       x[8 + k] = pick(live, v[k].y, 0.f);
     }
   }
+  // whether the rows before the call's are not in the tail
+  __device__ __forceinline__ bool gone() const { return before > 0 && *tag != pos / kBlk; }
+  // those rows from the codes (a unit is the 16 bytes that its thread writes later)
+  __device__ __forceinline__ void reopen(int u, float (&x)[16]) const {
+    const uint4 w = codes[u];
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    const float s = *scale;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = is_v ? v_row(u, e & 7) : u / (HD / 16);
+      if (row < before) x[e] = s * (float)(int8_t)(ws[e >> 2] >> (8 * (e & 3)));
+    }
+  }
   __device__ __forceinline__ static int v_row(int u, int k) {
     return 16 * (k >> 2) + 4 * (u & 3) + (k & 3);
   }
-  // the call's tokens of the block into the tail
-  __device__ __forceinline__ void keep(int u, const float (&x)[16]) const {
+  // rows from .. end - 1 of the block into the tail
+  __device__ __forceinline__ void keep(int u, int from, const float (&x)[16]) const {
     if (!is_v) {
       const int row = u / (HD / 16), d0 = 16 * (u % (HD / 16));
-      if (row < before || row >= end) return;
+      if (row < from || row >= end) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f4v *>(tail + row * HD + d0 + 4 * i) =
@@ -302,7 +330,7 @@ struct BlockTokens {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int row = v_row(u, k);
-      if (row >= before && row < end)
+      if (row >= from && row < end)
         *reinterpret_cast<float2 *>(tail + row * HD + d0) = make_float2(x[k], x[8 + k]);
     }
   }
@@ -385,20 +413,22 @@ __global__ void __launch_bounds__(kStoreWG<HD>, HD == 256 ? 2 : 4)
   const int64_t b = b0 + (int64_t)(blockIdx.x >> 1) / c.n_kv;
   if (b > bl) return;
   auto tokens = [&](int64_t bi) {
-    return BlockTokens<HD>(is_v, rope_by4(rope), (is_v ? v : k) + kvh * HD, (int64_t)c.n_kv * HD,
-                           (is_v ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, bi, rope);
+    return BlockTokens<HD>(c, kvh, is_v, rope_by4(rope), is_v ? v : k, sp, bi, rope);
   };
   BlockTokens<HD> blk = tokens(b);
   float x[UPT][16];
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) blk.load(tid + NT * i, x[i]);
+  const bool gone = blk.gone();
   uint32_t am = 0;
 #pragma unroll
   for (int i = 0; i < UPT; ++i) {
-    blk.load(tid + NT * i, x[i]);
+    if (gone) blk.reopen(tid + NT * i, x[i]);
     am = amax16(x[i], am);
   }
   am = wave_umax(am);
   if ((tid & 63) == 0) red[tid >> 6] = am;
-  __syncthreads();  // (and the tail has been read)
+  __syncthreads();  // (and the tail, its tag and the block's scale have been read)
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) am = max(am, red[w]);
   const float s = scale_of(am);
@@ -409,13 +439,16 @@ __global__ void __launch_bounds__(kStoreWG<HD>, HD == 256 ? 2 : 4)
 #pragma unroll
   for (int i = 0; i < UPT; ++i) dst[tid + NT * i] = code(x[i]);
   if (b != b0) return;
+  if (tid == 0) *blk.tag = (int32_t)bl;
+  int from = gone ? 0 : blk.before;
   if (bl != b0) {
     blk = tokens(bl);
+    from = 0;
 #pragma unroll
     for (int i = 0; i < UPT; ++i) blk.load(tid + NT * i, x[i]);
   }
 #pragma unroll
-  for (int i = 0; i < UPT; ++i) blk.keep(tid + NT * i, x[i]);
+  for (int i = 0; i < UPT; ++i) blk.keep(tid + NT * i, from, x[i]);
 }
 
 // ---- read-back ---------------------------------------------------------------
@@ -776,9 +809,7 @@ __global__ void __launch_bounds__(64 * kWaves)
       w = i / (UNITS / NT);
       u = threadIdx.x + NT * (i % (UNITS / NT));
     }
-    return BlockTokens<HD>(w == 1, true, (w ? vn : kn) + kvh * HD, (int64_t)c.n_kv * HD,
-                           (w ? c.v_tail : c.k_tail) + (int64_t)kvh * kBlk * HD, sp, (int64_t)nb,
-                           rope);
+    return BlockTokens<HD>(c, kvh, w == 1, true, w ? vn : kn, sp, (int64_t)nb, rope);
   };
   if constexpr (ROPE) {
     if (owner) {
@@ -842,7 +873,10 @@ __global__ void __launch_bounds__(64 * kWaves)
       for (int i = 0; i < UPT; ++i) {
         int u;
         const BlockTokens<HD> blk = tokens(i, u);
-        if (!blk.is_v) blk.keep(u, x[i]);  // (its own row; no other thread reads it)
+        const bool gone = blk.gone();
+        if (gone) blk.reopen(u, x[i]);
+        // (rows that no other thread reads; a token of V's below)
+        if (gone || !blk.is_v) blk.keep(u, gone ? 0 : blk.before, x[i]);
         const uint32_t a = amax16(x[i], 0);
         am[0] = max(am[0], blk.is_v ? 0u : a);
         am[1] = max(am[1], blk.is_v ? a : 0u);
@@ -859,7 +893,11 @@ __global__ void __launch_bounds__(64 * kWaves)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         sc[w] = scale_of(max(max(red[w][0], red[w][1]), max(red[w][2], red[w][3])));
-        if (threadIdx.x == 0) (w ? c.v_scale : c.k_scale)[kvh * n_blocks + nb] = sc[w];
+        if (threadIdx.x == 0) {
+          (w ? c.v_scale : c.k_scale)[kvh * n_blocks + nb] = sc[w];
+          reinterpret_cast<int32_t *>((w ? c.v_tail : c.k_tail) +
+                                      (int64_t)c.n_kv * kBlk * HD)[kvh] = nb;
+        }
       }
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {

@@ -139,9 +139,6 @@ class QuantKVCache:
             return
         if pos > self.length:
             raise ValueError(f"position {pos} leaves a gap after the {self.length} stored")
-        if pos % BLOCK and pos // BLOCK != (self.length - 1) // BLOCK and pos != self.length:
-            raise ValueError(f"position {pos} lies inside a block before the last one: go back "
-                             f"to {pos - pos % BLOCK}")
 
     def _call(self, fn, *args):
         """fn(*args, stream) with the cache's device current."""
@@ -159,8 +156,9 @@ class QuantKVCache:
         k rotated by cos / sin (positions, n_rot / 2; None: as it is), and
         rotate q (T, n_head * head_dim) into q_out (default: a new tensor;
         may be q), which is returned.  A position at or before the last
-        stored drops what followed; inside a block that is the last one only
-        (ValueError otherwise: start at a multiple of 32)."""
+        stored drops what followed: as if it had never been, inside the last
+        block and from a multiple of 32 on; inside an earlier block what stays
+        of it counts as its codes stand for it from then on."""
         torch = self._torch
         k, v = self._rows(k, "k", self.n_kv), self._rows(v, "v", self.n_kv)
         T = k.shape[0]

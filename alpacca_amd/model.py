@@ -410,7 +410,8 @@ class Model:
             n = max(0, len(tokens) - 1)
         if n != self.n_past:
             n = min(n, self.n_past)
-            # an 8-bit cache goes back inside its last block, or to a block's start
+            # an 8-bit cache goes back exactly inside its last block, or to a
+            # block's start (in between it would code coded values anew)
             if self.kv8 and n // KV_BLOCK != (self.n_past - 1) // KV_BLOCK:
                 n -= n % KV_BLOCK
             self.n_past = n

@@ -445,7 +445,8 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  * and stands for s c.  A block that holds an infinity or a NaN has a NaN scale
  * and reads as NaN.  The last block stored is also kept in fp32 (the tail), so a
  * token that joins it has it coded anew from the values themselves: the codes
- * do not depend on how many calls brought the tokens.
+ * do not depend on how many calls brought the tokens.  (A call that goes back
+ * inside an earlier block takes what stays of it as its codes stand for it.)
  *
  * The caller allocates the arrays (device memory, 16-byte aligned but for the
  * scales; sizes from aq_kv8_sizes; no initial content needed).  Calls on one
@@ -453,8 +454,8 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  * stream, or by events; so are replays of graphs that hold them.  q, k, v
  * and outputs are 16-byte aligned too (AQ_ERR_VALUE).  Layouts: K
  * codes [n_kv][n_blocks][32][head_dim], V codes [n_kv][n_blocks][head_dim / 2]
- * [4][2][8] (aq_kv8.hip), scales [n_kv][n_blocks], tails [n_kv][32][head_dim],
- * n_blocks = ceil(n_ctx / 32).  head_dim 64, 128 or 256.
+ * [4][2][8] (aq_kv8.hip), scales [n_kv][n_blocks], tails [n_kv][32][head_dim]
+ * and the block that each holds, n_blocks = ceil(n_ctx / 32).  head_dim 64, 128 or 256.
  */
 typedef struct aq_kv8 {
   int8_t *k, *v;            /* codes                                         */
@@ -474,11 +475,10 @@ int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *s
  * (which may be q; q NULL: no queries), k rotated and coded, v coded, at
  * positions p0 .. p0+T-1 (p0 = state->pos, or pos0 when state is NULL).  The
  * rotation is aq_rope_kv's bit for bit (n_rot 0: none; any even n_rot).  A call
- * that starts inside a block continues it: the block must be the last one
- * stored, and its positions before p0 stored (going back inside the last block
- * is fine, what followed is dropped; to go back further, start at a block's
- * first position).  Slots of the last block past p0+T-1 are cleared, blocks
- * after it left as they are.  AQ_ERR_VALUE when p0 + T > n_ctx (checked only for
+ * that starts inside a block continues it, and its positions before p0 must be
+ * stored; going back drops what followed (exactly, as if it had never been,
+ * inside the last block stored and to any block's first position).  Slots of
+ * the last block past p0+T-1 are cleared, blocks after it left as they are.  AQ_ERR_VALUE when p0 + T > n_ctx (checked only for
  * a host position; the kernels skip positions past the cache).  Enqueues only. */
 int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, int64_t T,
                 int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,

@@ -210,8 +210,6 @@ def test_store_goes_back():
     k[70] *= 50  # dropped below: must not leave its scale behind
     cache = QuantKVCache(2, 160, 64)
     cache.store(flat(k[:75]), flat(v[:75]), 0)
-    with pytest.raises(ValueError, match="go back to 32"):
-        cache.store(flat(k[:4]), flat(v[:4]), 40)
     k2, v2 = k[100:], v[100:]
     cache.store(flat(k2[:3]), flat(v2[:3]), 66)
     K, V = np.concatenate([k[:66], k2[:3]]), np.concatenate([v[:66], v2[:3]])
@@ -223,6 +221,40 @@ def test_store_goes_back():
     same_values(cache, (kc, vc), (ks, vs))
     with pytest.raises(ValueError, match="gap"):
         cache.store(flat(k[:1]), flat(v[:1]), 80)
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("how", ["store", "step", "tokens"])
+def test_store_goes_back_inside_an_earlier_block(hd, how):
+    """The positions that stay of an earlier block count as their codes stand
+    for them, also for tokens that join the block later."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd)
+    q, k, v = inputs(rng, 160, 4, 2, hd)
+    cache = QuantKVCache(2, 160, hd)
+    cache.store(flat(k[:100]), flat(v[:100]), 0)
+    at, n = 43, {"store": 40, "step": 1, "tokens": 5}[how]
+    K, V = ([values64(*coded(x[:100])).astype(np.float32)[:at], x[100:100 + n]] for x in (k, v))
+    K, V = np.concatenate(K), np.concatenate(V)
+    for i, p in enumerate(range(at, at + n)) if how != "store" else ():
+        if how == "step":
+            cache.step(flat(q[:1]), flat(k[100:101]), flat(v[100:101]), p)
+        else:
+            cache.store(flat(k[100 + i:101 + i]), flat(v[100 + i:101 + i]), p)
+    if how == "store":
+        cache.store(flat(k[100:140]), flat(v[100:140]), at)
+    # (blocks before are as they were: code them from their own tokens)
+    K[:B], V[:B] = k[:B], v[:B]
+    assert cache.length == at + n
+    (kc, ks), (vc, vs) = coded(K), coded(V)
+    same_values(cache, (kc, vc), (ks, vs))
+    # the same call again on what it left
+    if how == "store":
+        before = [x.clone() for x in cache.read()]
+        cache.store(flat(k[100:140]), flat(v[100:140]), at)
+        for x, y in zip(before, cache.read()):
+            assert (x - y).abs().max() <= 2.0 ** -22 * x.abs().max()
 
 
 @gpu
@@ -537,7 +569,8 @@ def test_sizes():
     for n_kv, hd, n_ctx in ((1, 64, 1), (8, 128, 131072), (5, 256, 33)):
         assert lib.aq_kv8_sizes(n_kv, hd, n_ctx, *map(ctypes.byref, out)) == 0
         blocks = n_kv * -(-n_ctx // B)
-        assert [o.value for o in out[:3]] == [blocks * B * hd, blocks * 4, n_kv * B * hd * 4]
+        assert [o.value for o in out[:3]] == [blocks * B * hd, blocks * 4,
+                                              (n_kv * B * hd + -(-n_kv // 4) * 4) * 4]
         assert out[3].value > 0
     for bad in ((0, 64, 10), (1, 96, 10), (1, 64, 0), (1, 64, 2 ** 31)):
         assert lib.aq_kv8_sizes(*bad, None, None, None, None) == _lib.AQ_ERR_VALUE
