@@ -299,8 +299,12 @@ struct BlockTokens {
       x[8 + k] = pick(live, v[k].y, 0.f);
     }
   }
-  // whether the rows before the call's are not in the tail
-  __device__ __forceinline__ bool gone() const { return before > 0 && *tag != pos / kBlk; }
+  // whether the rows before the call's are not in the tail (read before the
+  // workgroup, the only one to write the tag, does: a scalar load and a branch)
+  __device__ __forceinline__ bool gone() const {
+    const int32_t t = *(const __attribute__((address_space(4))) int32_t *)tag;
+    return before > 0 && t != (int32_t)(pos / kBlk);
+  }
   // those rows from the codes (a unit is the 16 bytes that its thread writes later)
   __device__ __forceinline__ void reopen(int u, float (&x)[16]) const {
     const uint4 w = codes[u];
@@ -746,23 +750,29 @@ struct OutScale {
 // takes the token's block, which it alone reads: it codes the block anew from
 // the tail and the token (k_kv8_store's codes, bit for bit), stores it and
 // attends to it from LDS, while the others go through the blocks before.
+//
+// (There a wave executes its few thousand instructions alone on its SIMD, 2 ns
+// each, so four waves code the block while a fifth makes q's pieces.)
 constexpr int kWaves = 4;
+constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves + 1 : kWaves; }
 template <int HD, bool ROPE>
-__global__ void __launch_bounds__(64 * kWaves)
+__global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     k_kv8_split(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
                 int64_t T, int G, float scale, float *__restrict__ part, float *__restrict__ out,
                 const float *__restrict__ kn, const float *__restrict__ vn, Rope rope) {
+  constexpr int NW = split_waves(HD, ROPE);
   constexpr int KJ = HD / 64, VJ = HD / 32, PS = HD + 4;
   constexpr int PARTS = HD == 256 ? 2 : 1, VP = VJ / PARTS;  // the merge's LDS: at most 32 KB
-  __shared__ f4v os[kWaves][2 * VP][64];
-  __shared__ float stat[kWaves][3][16];
+  __shared__ f4v os[NW][2 * VP][64];
+  __shared__ float stat[NW][3][16];
   __shared__ uint4 own[ROPE ? 2 : 1][ROPE ? BlockTokens<HD>::UNITS : 1];  // the token's block
   __shared__ uint32_t red[2][kWaves];
   const Span sp = span_of(st, pos0, T, c.n_ctx);
   const int j = blockIdx.x, S = gridDim.x, kvh = blockIdx.y, n_head = gridDim.y * G;
   const int id0 = blockIdx.z * 16, rows = (int)sp.n * G;  // at most 65535 x 16
   if (id0 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, cg = lane >> 4;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, cg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = id0 + r16, id_last = id0 + 15 < rows ? id0 + 15 : rows - 1;
   const bool live = id < rows;
   const int tok = live ? id / G : 0;
@@ -794,7 +804,7 @@ __global__ void __launch_bounds__(64 * kWaves)
   };
   Buf b0, b1;
   const bool owner = ROPE && j == 0;
-  int b = owner ? nb : (ROPE ? j - 1 : j) * kWaves + wave;
+  int b = owner ? nb : (ROPE ? j - 1 : j) * NW + wave;
   if (!owner) load(b, b0);
   // the owner's tokens: on their way before q's are waited for
   constexpr int UNITS = BlockTokens<HD>::UNITS, NT = 64 * kWaves;
@@ -811,19 +821,23 @@ __global__ void __launch_bounds__(64 * kWaves)
     }
     return BlockTokens<HD>(c, kvh, w == 1, true, w ? vn : kn, sp, (int64_t)nb, rope);
   };
+  bool gone[2] = {false, false};  // K's and V's block
+  const bool coding = owner && wave < kWaves, asking = owner && wave == NW - 1;
   if constexpr (ROPE) {
-    if (owner) {
+    if (coding) {
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
         int u;
         const BlockTokens<HD> blk = tokens(i, u);
+        gone[blk.is_v] = blk.gone();
         blk.load(u, x[i]);
       }
     }
   }
   QRow<HD> qr;
-  qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, sp.p0,
-                         rope);
+  if (!coding || asking)
+    qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, sp.p0,
+                           rope);
   RowState<HD> s;
   s.clear();
   auto compute = [&](int blk, Buf &x, auto mask) {
@@ -868,25 +882,29 @@ __global__ void __launch_bounds__(64 * kWaves)
   };
   if constexpr (ROPE) {
     if (owner) {
-      uint32_t am[2] = {0, 0};  // of K's and V's units (a wave's units are of one each)
+      if (coding) {
+        uint32_t am[2] = {0, 0};  // of K's and V's units (a wave's units are of one each)
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        int u;
-        const BlockTokens<HD> blk = tokens(i, u);
-        const bool gone = blk.gone();
-        if (gone) blk.reopen(u, x[i]);
-        // (rows that no other thread reads; a token of V's below)
-        if (gone || !blk.is_v) blk.keep(u, gone ? 0 : blk.before, x[i]);
-        const uint32_t a = amax16(x[i], 0);
-        am[0] = max(am[0], blk.is_v ? 0u : a);
-        am[1] = max(am[1], blk.is_v ? a : 0u);
-      }
-      for (int d = threadIdx.x; d < HD; d += NT)  // V's tail row: the token's values
-        c.v_tail[((int64_t)kvh * kBlk + sp.p0 % kBlk) * HD + d] = vn[kvh * HD + d];
+        for (int i = 0; i < UPT; ++i) {
+          int u;
+          const BlockTokens<HD> blk = tokens(i, u);
+          if (gone[blk.is_v]) {
+            blk.reopen(u, x[i]);
+            blk.keep(u, 0, x[i]);
+          } else if (!blk.is_v) {
+            blk.keep(u, blk.before, x[i]);  // (its own row; no other thread reads it)
+          }
+          const uint32_t a = amax16(x[i], 0);
+          am[0] = max(am[0], blk.is_v ? 0u : a);
+          am[1] = max(am[1], blk.is_v ? a : 0u);
+        }
+        for (int d = threadIdx.x; d < HD; d += NT)  // V's tail row: the token's values
+          c.v_tail[((int64_t)kvh * kBlk + sp.p0 % kBlk) * HD + d] = vn[kvh * HD + d];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        am[w] = wave_umax(am[w]);
-        if (lane == 0) red[w][wave] = am[w];
+        for (int w = 0; w < 2; ++w) {
+          am[w] = wave_umax(am[w]);
+          if (lane == 0) red[w][wave] = am[w];
+        }
       }
       __syncthreads();
       float sc[2];
@@ -899,17 +917,19 @@ __global__ void __launch_bounds__(64 * kWaves)
                                       (int64_t)c.n_kv * kBlk * HD)[kvh] = nb;
         }
       }
+      if (coding) {
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        int u;
-        const BlockTokens<HD> blk = tokens(i, u);
-        const int w = blk.is_v ? 1 : 0;
-        const uint4 cd = Coder(w ? sc[1] : sc[0])(x[i]);
-        own[w][u] = cd;
-        reinterpret_cast<uint4 *>((w ? c.v : c.k) + (kvh * n_blocks + nb) * (kBlk * HD))[u] = cd;
+        for (int i = 0; i < UPT; ++i) {
+          int u;
+          const BlockTokens<HD> blk = tokens(i, u);
+          const int w = blk.is_v ? 1 : 0;
+          const uint4 cd = Coder(w ? sc[1] : sc[0])(x[i]);
+          own[w][u] = cd;
+          reinterpret_cast<uint4 *>((w ? c.v : c.k) + (kvh * n_blocks + nb) * (kBlk * HD))[u] = cd;
+        }
       }
       __syncthreads();
-      if (wave == 0) {
+      if (asking) {
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
@@ -925,7 +945,7 @@ __global__ void __launch_bounds__(64 * kWaves)
       }
     }
   }
-  const int stride = (ROPE ? S - 1 : S) * kWaves;
+  const int stride = (ROPE ? S - 1 : S) * NW;
   constexpr auto mask = std::integral_constant<bool, !ROPE>();  // (full blocks before the token's)
   while (b < nb) {
     load(b + stride, b1);
@@ -944,7 +964,7 @@ __global__ void __launch_bounds__(64 * kWaves)
   }
   float *dst = S == 1 ? out + ((int64_t)tok * n_head + kvh * G + g) * HD
                       : part + (((int64_t)kvh * T * G + id) * S + j) * PS;
-  float M = -INFINITY, R = kLow, den = 0.f, fo[kWaves];
+  float M = -INFINITY, R = kLow, den = 0.f, fo[NW];
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
     if (h) __syncthreads();
@@ -953,25 +973,25 @@ __global__ void __launch_bounds__(64 * kWaves)
     __syncthreads();
     if (h == 0) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         M = fmaxf(M, stat[w][0][r16]);
         R = fmaxf(R, stat[w][1][r16]);
       }
       const float mref = M == -INFINITY ? 0.f : M;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < NW; ++w) {
         den = fmaf(stat[w][2][r16], exp2_(stat[w][0][r16] - mref), den);
         fo[w] = exp2_(stat[w][1][r16] - R);
       }
     }
     const OutScale fin(R, M, den);
-    for (int i = wave; i < VP; i += kWaves) {
+    for (int i = wave; i < VP; i += NW) {
       f4v a[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         a[e] = os[0][2 * i + e][lane] * fo[0];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) a[e] += os[w][2 * i + e][lane] * fo[w];
+        for (int w = 1; w < NW; ++w) a[e] += os[w][2 * i + e][lane] * fo[w];
         if (S == 1) a[e] = fin(a[e]);
       }
       f4v *o4 = reinterpret_cast<f4v *>(dst + 32 * (VP * h + i) + 8 * cg);
@@ -1348,9 +1368,9 @@ hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, 
 //
 // The split kernel: about two workgroups per CU, no more than give every wave a
 // block of a full cache, nor than the scratch holds (the step has one more).
-int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows) {
+int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves) {
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
-  int64_t S = (n_blocks + kWaves - 1) / kWaves;
+  int64_t S = (n_blocks + waves - 1) / waves;
   const int64_t fill = (kMaxSplits - 1 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
   const int64_t room = kScratchRows / rows - 1;
   S = S < fill ? S : fill;
@@ -1386,7 +1406,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
   int S;
   if (rows <= kSplitRows) {
     const int64_t tiles = (rows + 15) / 16;
-    S = kv8_splits(c, tiles, T * n_head);
+    S = kv8_splits(c, tiles, T * n_head, kWaves);
     AQ_HD(c.head_dim,
           hipLaunchKernelGGL((k_kv8_split<HD, false>),
                              dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
@@ -1427,10 +1447,11 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      float *out, hipStream_t s) {
   const float scale = (float)(1.0 / sqrt((double)c.head_dim));
   const int G = n_head / c.n_kv;
-  const int S = kv8_splits(c, 1, n_head) + 1;
   AQ_HD(c.head_dim,
+        constexpr int NW = split_waves(HD, true);
+        const int S = kv8_splits(c, 1, n_head, NW) + 1;
         hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
-                           dim3(64 * kWaves), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
+                           dim3(64 * NW), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
                            c.scratch, out, k, v, Rope{cos_t, sin_t, n_rot, neox});
         hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)G, (unsigned)c.n_kv), dim3(kWG), 0, s,
                            c.scratch, st, pos0, c.n_ctx, (int64_t)1, G, S, out))
