@@ -366,6 +366,10 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 // the last token are cleared.  The workgroup of the call's first block also keeps
 // the tail: it alone reads it (before), and writes the tokens of the last block
 // (after), so no two workgroups meet there.  The rest rotate q, a token each.
+//
+// One pass over memory, one barrier a block: 2048 tokens, 32 / 8
+// heads of 128 20.3 us (50 MB in, 38 out: 4.3 TB/s; a large copy 5.15), one
+// token of 32 / 8 heads of 64 5.0 us (its chain: position, tail, tables, maximum).
 template <int HD>
 constexpr int kStoreWG = HD == 64 ? 128 : 256;
 template <int HD>
@@ -459,6 +463,8 @@ __global__ void __launch_bounds__(kStoreWG<HD>, HD == 256 ? 2 : 4)
 // out[kvh][p - start][d] = s c, one product rounded to fp32.  One workgroup per
 // block of K and of V; a thread turns units of 16 codes into four 16-byte stores
 // (K), or eight 8-byte ones to eight rows (V; 16 lanes fill 128 bytes of a row).
+// Bound by its stores: 2048 positions of 8 heads of 128, 21 MB in 7.5 us; one
+// position 2.4.
 template <int HD>
 __global__ void __launch_bounds__(kStoreWG<HD>)
     k_kv8_read(aq_kv8 c, int64_t start, int64_t n, float *__restrict__ ko,
@@ -745,14 +751,20 @@ struct OutScale {
 // under way while one is computed; the waves' states meet in LDS, the splits'
 // in k_kv8_combine.  One split writes the output itself.
 //
+// Bound by the codes' bytes, for short caches by one wave's chain.  One token of
+// 32 / 8 heads of 128: 30000 positions 13.7 us (61 MB: 4.5 TB/s), 131072 42
+// (268 MB: 6.4); 32 / 8 heads of 64, 2176 positions 4.5; 5 tokens of 28 / 4
+// heads of 128 at 7001 12.4 (three tiles of rows, each reading the codes).
+//
 // ROPE: one token, whose q, k and v are not rotated yet.  Every workgroup
 // rotates its q rows in registers; one more workgroup per kv head (the first)
 // takes the token's block, which it alone reads: it codes the block anew from
 // the tail and the token (k_kv8_store's codes, bit for bit), stores it and
-// attends to it from LDS, while the others go through the blocks before.
-//
-// (There a wave executes its few thousand instructions alone on its SIMD, 2 ns
-// each, so four waves code the block while a fifth makes q's pieces.)
+// attends to it from LDS, while the others go through the blocks before.  There
+// a wave executes its few thousand instructions alone on its SIMD, 2 ns each,
+// so four waves code the block while a fifth makes q's pieces: 32 / 8 heads of
+// 128 at 3800 positions 8.3 us (four waves 10.2; the store's launch alone 5),
+// 32 / 8 heads of 64 at 99 6.0 (6.4).  At 256 dimensions five waves spill: four.
 constexpr int kWaves = 4;
 constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves + 1 : kWaves; }
 template <int HD, bool ROPE>
@@ -1007,7 +1019,8 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
 
 // One workgroup per query row merges the splits' states: HD / 4 threads of 16
 // bytes a split, all of a chunk's loads (and the m, R, l of every split) in
-// flight at once.
+// flight at once.  Bound by a launch's start and two trips to memory: 3.0-3.9 us
+// at 18 to 64 splits (loads one after the other: 31 at 64).
 constexpr int kMaxSplits = 512;
 template <int HD>
 __global__ void __launch_bounds__(kWG)
@@ -1088,7 +1101,9 @@ __global__ void __launch_bounds__(kWG)
 }
 
 // The merge of up to kFewSplits splits of many rows: HD / 4 threads per row, all
-// its loads in flight at once, no LDS.
+// its loads in flight at once, no LDS.  Bound by the states' bytes: 256 tokens
+// of 32 heads of 128 in 4 splits (17 MB in, 4 out, from the last-level cache)
+// 5.3 us (through k_kv8_combine the whole call took 95 us, not 85).
 constexpr int kFewSplits = 8;
 template <int HD>
 __global__ void __launch_bounds__(kWG)
@@ -1129,12 +1144,20 @@ __global__ void __launch_bounds__(kWG)
 // ---- many rows: tiles of rows over all positions they see -------------------------
 // One workgroup of four waves per 64 rows (16 per wave) of a kv head and split of
 // the positions (gridDim.y of them; one writes the output, several their states
-// for k_kv8_combine).  The chunks of two blocks are converted to fp16 in operand order in LDS once for all waves
-// (each lane's 16 bytes at its place: no conflicts).  A wave's pass over chunk ch
-// forms the scores of chunk ch + 1 while the softmax of chunk ch runs (the matrix
-// and the vector instructions of one pass do not wait for each other), then adds
-// the values of chunk ch; K of chunk ch + 2 and V of chunk ch + 1 go to LDS
-// meanwhile, the codes after them are on their way, and one barrier ends it.
+// for the merge).  The chunks of two blocks are converted to fp16 in operand
+// order in LDS once for all waves (each lane's 16 bytes at its place: no
+// conflicts).  A wave's pass over chunk ch forms the scores of chunk ch + 1 while
+// the softmax of chunk ch runs (the matrix and the vector instructions of one
+// pass do not wait for each other), then adds the values of chunk ch; K of chunk
+// ch + 2 and V of chunk ch + 1 go to LDS meanwhile, the codes after them are on
+// their way, and one barrier ends it.
+//
+// Bound by issue, matrix and vector instructions together (matrix cores busy 34 %
+// and 38 % of the time; each useful product is two, of two pieces).  2048 tokens of
+// 32 / 8 heads of 64 from the start 55 us (17.2 useful GFLOP: 0.31 PFLOP/s, 0.62
+// with both pieces); 777 of 32 / 8 heads of 128 behind 2901 127 us (0.33, 0.66).
+// Slower: two row tiles per wave (74 and 182 against 66 and 146 then), eight waves
+// (57 and 143), q's pieces from LDS, rescaling always (61 against 57).
 template <int HD>
 __global__ void __launch_bounds__(64 * kWaves)
     k_kv8_tiles(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
@@ -1142,8 +1165,8 @@ __global__ void __launch_bounds__(64 * kWaves)
                 float *__restrict__ out) {
   constexpr int KJ = HD / 64, VJ = HD / 32, KS = HD / 32;
   constexpr int NU = HD / 64;  // 1 KB units of a chunk's K (and of its V) per wave
-  // 128 dimensions and more have the registers to read four operands ahead (146
-  // against 134 us below; at 64 it costs: 56 against 59)
+  // 128 dimensions and more have the registers to read four operands ahead (127 us,
+  // one ahead 134); at 64 it costs (59, one ahead 56)
   constexpr int AHEAD = HD >= 128 ? 4 : 1;
   extern __shared__ __attribute__((aligned(16))) h8 lds[];
   auto kl = reinterpret_cast<h8(*)[4 * KS][64]>(lds);                // [2][position tile, k step][lane]
