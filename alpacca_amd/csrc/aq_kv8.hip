@@ -299,10 +299,12 @@ struct BlockTokens {
       x[8 + k] = pick(live, v[k].y, 0.f);
     }
   }
-  // whether the rows before the call's are not in the tail (read before the
-  // workgroup, the only one to write the tag, does: a scalar load and a branch)
+  // whether the rows before the call's are not in the tail.  A scalar load and a
+  // branch, before the workgroup, the only one to write the tag, does; the empty
+  // statement holds the value, which is not to be loaded again after that.
   __device__ __forceinline__ bool gone() const {
-    const int32_t t = *(const __attribute__((address_space(4))) int32_t *)tag;
+    int32_t t = *(const __attribute__((address_space(4))) int32_t *)tag;
+    asm volatile("" : "+s"(t));
     return before > 0 && t != (int32_t)(pos / kBlk);
   }
   // those rows from the codes (a unit is the 16 bytes that its thread writes later)
@@ -367,9 +369,9 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 // the tail: it alone reads it (before), and writes the tokens of the last block
 // (after), so no two workgroups meet there.  The rest rotate q, a token each.
 //
-// One pass over memory, one barrier a block: 2048 tokens, 32 / 8
-// heads of 128 20.3 us (50 MB in, 38 out: 4.3 TB/s; a large copy 5.15), one
-// token of 32 / 8 heads of 64 5.0 us (its chain: position, tail, tables, maximum).
+// One pass over memory, one barrier a block: 2048 tokens, 32 / 8 heads of 128
+// 20.3 us (50 MB in, 38 out: 4.3 TB/s; a large copy 5.15), one token of 32 / 8
+// heads of 64 5.0 us (its chain: position, tail, tables, maximum).
 template <int HD>
 constexpr int kStoreWG = HD == 64 ? 128 : 256;
 template <int HD>
@@ -763,7 +765,7 @@ struct OutScale {
 // attends to it from LDS, while the others go through the blocks before.  There
 // a wave executes its few thousand instructions alone on its SIMD, 2 ns each,
 // so four waves code the block while a fifth makes q's pieces: 32 / 8 heads of
-// 128 at 3800 positions 8.3 us (four waves 10.2; the store's launch alone 5),
+// 128 at 3800 positions 7.8 us (four waves 10.2; the store's launch alone 5),
 // 32 / 8 heads of 64 at 99 6.0 (6.4).  At 256 dimensions five waves spill: four.
 constexpr int kWaves = 4;
 constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves + 1 : kWaves; }
@@ -840,9 +842,13 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
         int u;
+        tokens(i, u).load(u, x[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {  // (awaited when all loads are on their way)
+        int u;
         const BlockTokens<HD> blk = tokens(i, u);
         gone[blk.is_v] = blk.gone();
-        blk.load(u, x[i]);
       }
     }
   }
