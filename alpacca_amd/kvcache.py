@@ -236,11 +236,11 @@ class QuantKVCache:
             raise ValueError(f"positions {start}..{stop - 1} of {self.length} stored")
         kv = torch.empty((2, self.n_kv, stop - start, self.head_dim), dtype=torch.float32,
                          device=self.device)
-        k, v = kv[0], kv[1]
         if stop > start:
-            self._call(self._lib.aq_kv8_read, self._ref, start, stop - start, k.data_ptr(),
-                       v.data_ptr())
-        return k, v
+            p = kv.data_ptr()
+            self._call(self._lib.aq_kv8_read, self._ref, start, stop - start, p,
+                       p + 4 * self.n_kv * (stop - start) * self.head_dim)
+        return kv.unbind()
 
 
 __all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "QuantKVCache"]
