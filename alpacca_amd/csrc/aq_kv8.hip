@@ -521,10 +521,10 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
 //     operand as it holds them (the V layout stores positions in that order).
 // The block's K scale enters as the factor of its raw scores, its V scale in
 // the weights: P = 2^(z - m) s_V, formed relative to the largest such product
-// the row has met, 2^R, so the pieces hold 24 bits of whatever counts and no
-// magnitude of V over- or underflows them.  m and R are rounded up to whole
-// numbers, so every rescaling is an exact power of two.  The sum of 2^(z - m)
-// is kept per lane.
+// the row has met, 2^D (of the same 2^m), so the pieces hold 24 bits of whatever
+// counts and no magnitude of V over- or underflows them.  m and D are rounded up
+// to whole numbers, so every rescaling is an exact power of two; D stays a small
+// number however large the scores are.  The sum of 2^(z - m) is kept per lane.
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f2v __attribute__((ext_vector_type(2)));
@@ -532,7 +532,8 @@ typedef unsigned int u4v __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kTop = 14.f;      // weights reach 2^14 in the pieces
-constexpr float kLow = -1e30f;    // R before any weight
+constexpr float kLow = -1e30f;    // D before any weight
+constexpr float kFine = 0x1p20f;  // exponents up to here are off by less than 2^-4
 
 template <int OFF>
 __device__ __forceinline__ float2 lane_pair(float v) {
@@ -655,52 +656,82 @@ struct QRow {
   }
 };
 
-// The running softmax of a lane's row: maximum m and reference R (both whole
-// exponents of two, the same in the row's four lanes), the lane's part of the
-// sum l, and the numerators, o[2 j + e][rr] at dimension 32 j + 8 cg + 2 rr + e,
-// which stand for o 2^(R - m - kTop).
+// The running softmax of a lane's row: maximum m and, counted from it, the
+// reference D (both whole exponents of two, the same in the row's four lanes), the
+// lane's part of the sum l, and the numerators, o[2 j + e][rr] at dimension
+// 32 j + 8 cg + 2 rr + e, which stand for o 2^(D - kTop).
 template <int HD>
 struct RowState {
-  float m, R, l;
+  float m, D, l;
   f4v o[HD / 16];
   __device__ __forceinline__ void clear() {
-    m = -INFINITY, R = kLow, l = 0.f;
+    m = -INFINITY, D = kLow, l = 0.f;
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) o[i] = f4v{0.f, 0.f, 0.f, 0.f};
   }
 };
+// differences are taken from m, 0 where the row has seen nothing
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+// a reference D counted from m, counted from ref >= m
+__device__ __forceinline__ float moved(float D, float m, float ref) {
+  return fmaxf(D + (m - ref), kLow);
+}
 
 // NB blocks' raw scores sc (two tiles of positions each) to weights in pieces,
-// with their K and V scales: m, R, l and o of the row move on.  MASK: only
+// with their K and V scales: m, D, l and o of the row move on.  MASK: only
 // positions up to last[b], counted from the lane's first one in block b, exist.
+//
+// An exponent is one fma, whose product is not rounded while the maximum's is:
+// past kFine that would show (weights above what fp16 holds, or the largest one
+// lost), so there the scores are rounded products first, for the whole wave.
 template <int HD, int NB, bool MASK>
 __device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB], float f,
                                              const float (&ks)[NB], const float (&vs)[NB],
                                              const int (&last)[NB], h8 (&ph)[NB], h8 (&pl)[NB]) {
-  float c[NB], t[NB], ve[NB], mn = st.m, R = st.R;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    c[b] = ks[b] * f;
+  float c[NB], t[NB], ve[NB], mn = st.m, reach = 0.f;
+  auto largest = [&](int b) {  // of the row's scores in a block, -infinity for none
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = sc[2 * b + (i >> 2)][i & 3];
       mx = !MASK || 16 * (i >> 2) + (i & 3) <= last[b] ? fmaxf(mx, x) : mx;
     }
-    mx = row_max(mx);
-    t[b] = mx == -INFINITY ? mx : ceilf(mx * c[b]);  // (not through a masked block's scale)
-    mn = fmaxf(mn, t[b]);
-    ve[b] = (float)__builtin_amdgcn_frexp_expf(vs[b]);
-    if (vs[b] > 0.f) R = fmaxf(R, t[b] + ve[b]);
+    return row_max(mx);
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    c[b] = ks[b] * f;
+    const float mx = largest(b);
+    const bool none = MASK && mx == -INFINITY;  // (not through a masked block's scale)
+    t[b] = none ? mx : ceilf(mx * c[b]);
+    reach += none ? 0.f : fabsf(t[b]);
   }
-  const float mref = mn == -INFINITY ? 0.f : mn;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(reach < kFine)) != 0, 0)) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      c[b] = c[b] > 0x1.fffffep127f ? 0x1.fffffep127f : c[b];  // (no 0 x infinity; a NaN stays)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sc[2 * b + (i >> 2)][i & 3] *= c[b];
+      t[b] = ceilf(largest(b));
+      c[b] = 1.f;
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) mn = fmaxf(mn, t[b]);
+  const float mref = finite_ref(mn), old = moved(st.D, st.m, mref);
+  float D = old;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    ve[b] = (float)__builtin_amdgcn_frexp_expf(vs[b]);
+    if (vs[b] > 0.f) D = fmaxf(D, (t[b] - mref) + ve[b]);
+  }
   // (whole exponents: an integer conversion and a ldexp, a quarter of exp2's time)
-  const float corr = ldexpf(1.f, (int)(st.m - mref)), corr_o = ldexpf(1.f, (int)(st.R - R));
+  const float corr = ldexpf(1.f, (int)(st.m - mref)), corr_o = ldexpf(1.f, (int)(old - D));
   float sum = 0.f;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const float g = ldexpf(__builtin_amdgcn_frexp_mantf(vs[b]),
-                           (int)fminf(ve[b] + mref - R + kTop, 120.f));
+                           (int)fminf(ve[b] - D + kTop, 120.f));
     u4v h, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -722,20 +753,20 @@ __device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB]
   }
   st.l = fmaf(st.l, corr, sum);
   st.m = mn;
-  // (R moves in whole powers of two, so seldom)
-  if (__any(R != st.R)) {
+  // (whole powers of two, so seldom)
+  if (__builtin_amdgcn_ballot_w64(D != old)) {
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) st.o[i] *= corr_o;
   }
-  st.R = R;
+  st.D = D;
 }
 
-// v 2^(R - m - kTop) / den, the power in two whole parts so that neither leaves
+// v 2^(D - kTop) / den, the power in two whole parts so that neither leaves
 // the range
 struct OutScale {
   float a, b;
-  __device__ __forceinline__ OutScale(float R, float m, float den) {
-    const float x = R - m - kTop, h = floorf(0.5f * x);
+  __device__ __forceinline__ OutScale(float D, float den) {
+    const float x = D - kTop, h = floorf(0.5f * x);
     a = exp2_(h);
     b = exp2_(x - h);
     inv = 1.f / den;
@@ -744,6 +775,14 @@ struct OutScale {
   template <class V>
   __device__ __forceinline__ V operator()(V v) const {
     return v * a * inv * b;
+  }
+};
+// two states' references joined
+struct Ref {
+  float m, D;
+  __device__ __forceinline__ Ref join(const Ref &o) const {
+    const float n = fmaxf(m, o.m), ref = finite_ref(n);
+    return {n, fmaxf(moved(D, m, ref), moved(o.D, o.m, ref))};
   }
 };
 
@@ -977,12 +1016,13 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
   s.l = row_sum(s.l);
   if (cg == 0) {
     stat[wave][0][r16] = s.m;
-    stat[wave][1][r16] = s.R;
+    stat[wave][1][r16] = s.D;
     stat[wave][2][r16] = s.l;
   }
   float *dst = S == 1 ? out + ((int64_t)tok * n_head + kvh * G + g) * HD
                       : part + (((int64_t)kvh * T * G + id) * S + j) * PS;
-  float M = -INFINITY, R = kLow, den = 0.f, fo[NW];
+  Ref all{-INFINITY, kLow};
+  float den = 0.f, fo[NW];
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
     if (h) __syncthreads();
@@ -991,18 +1031,15 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     __syncthreads();
     if (h == 0) {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        M = fmaxf(M, stat[w][0][r16]);
-        R = fmaxf(R, stat[w][1][r16]);
-      }
-      const float mref = M == -INFINITY ? 0.f : M;
+      for (int w = 0; w < NW; ++w) all = all.join({stat[w][0][r16], stat[w][1][r16]});
+      const float mref = finite_ref(all.m);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         den = fmaf(stat[w][2][r16], exp2_(stat[w][0][r16] - mref), den);
-        fo[w] = exp2_(stat[w][1][r16] - R);
+        fo[w] = exp2_(moved(stat[w][1][r16], stat[w][0][r16], mref) - all.D);
       }
     }
-    const OutScale fin(R, M, den);
+    const OutScale fin(all.D, den);
     for (int i = wave; i < VP; i += NW) {
       f4v a[2];
 #pragma unroll
@@ -1020,11 +1057,11 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     }
   }
   if (S > 1 && live && wave == 0 && cg == 0)
-    *reinterpret_cast<f4v *>(dst + HD) = f4v{M, R, den, 0.f};
+    *reinterpret_cast<f4v *>(dst + HD) = f4v{all.m, all.D, den, 0.f};
 }
 
 // One workgroup per query row merges the splits' states: HD / 4 threads of 16
-// bytes a split, all of a chunk's loads (and the m, R, l of every split) in
+// bytes a split, all of a chunk's loads (and the m, D, l of every split) in
 // flight at once.  Bound by a launch's start and two trips to memory: 3.0-3.9 us
 // at 18 to 64 splits (loads one after the other: 31 at 64).
 constexpr int kMaxSplits = 512;
@@ -1045,7 +1082,7 @@ __global__ void __launch_bounds__(kWG)
     const int s = grp + NG * u;
     x[u] = *reinterpret_cast<const f4v *>(p + (s < S ? s : 0) * PS + 4 * d4);
   }
-  f4v e[2];  // m, R, l of splits tid and tid + 256
+  f4v e[2];  // m, D, l of splits tid and tid + 256
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int s = tid + kWG * i;
@@ -1054,27 +1091,23 @@ __global__ void __launch_bounds__(kWG)
   }
   const Span sp = span_of(st, pos0, T, n_ctx);
   if (t >= sp.n) return;
-  float M = fmaxf(e[0][0], e[1][0]), R = fmaxf(e[0][1], e[1][1]);
+  Ref all = Ref{e[0][0], e[0][1]}.join({e[1][0], e[1][1]});
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    M = fmaxf(M, __shfl_xor(M, off));
-    R = fmaxf(R, __shfl_xor(R, off));
-  }
+  for (int off = 32; off > 0; off >>= 1)
+    all = all.join({__shfl_xor(all.m, off), __shfl_xor(all.D, off)});
   if ((tid & 63) == 0) {
-    red[0][tid >> 6] = M;
-    red[1][tid >> 6] = R;
+    red[0][tid >> 6] = all.m;
+    red[1][tid >> 6] = all.D;
   }
   __syncthreads();
+  all = {red[0][0], red[1][0]};
 #pragma unroll
-  for (int w = 0; w < kWG / 64; ++w) {
-    M = fmaxf(M, red[0][w]);
-    R = fmaxf(R, red[1][w]);
-  }
-  const float mref = M == -INFINITY ? 0.f : M;
+  for (int w = 1; w < kWG / 64; ++w) all = all.join({red[0][w], red[1][w]});
+  const float mref = finite_ref(all.m);
   float den = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (tid + kWG * i < S) fo[tid + kWG * i] = exp2_(e[i][1] - R);
+    if (tid + kWG * i < S) fo[tid + kWG * i] = exp2_(moved(e[i][1], e[i][0], mref) - all.D);
     den = fmaf(e[i][2], exp2_(e[i][0] - mref), den);
   }
 #pragma unroll
@@ -1102,7 +1135,7 @@ __global__ void __launch_bounds__(kWG)
   if (tid >= LP) return;
 #pragma unroll
   for (int w = 1; w < NG; ++w) o += acc[w][d4];
-  const OutScale fin(R, M, den);
+  const OutScale fin(all.D, den);
   reinterpret_cast<f4v *>(out + ((int64_t)t * n_head + kvh * G + (id - t * G)) * HD)[d4] = fin(o);
 }
 
@@ -1121,29 +1154,27 @@ __global__ void __launch_bounds__(kWG)
   const Span sp = span_of(st, pos0, T, n_ctx);
   if (t >= sp.n) return;
   const float *p = part + ((int64_t)kvh * T * G + id) * S * PS;
-  f4v x[kFewSplits], e[kFewSplits];  // numerators; m, R, l
+  f4v x[kFewSplits], e[kFewSplits];  // numerators; m, D, l
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
     const float *ps = p + (s < S ? s : 0) * PS;
     x[s] = *reinterpret_cast<const f4v *>(ps + 4 * d4);
     e[s] = *reinterpret_cast<const f4v *>(ps + HD);
   }
-  float M = -INFINITY, R = kLow;
+  Ref all{e[0][0], e[0][1]};
 #pragma unroll
-  for (int s = 0; s < kFewSplits; ++s) {  // (repeats of the first split change no maximum)
-    M = fmaxf(M, e[s][0]);
-    R = fmaxf(R, e[s][1]);
-  }
-  const float mref = M == -INFINITY ? 0.f : M;
+  for (int s = 1; s < kFewSplits; ++s)  // (repeats of the first split change nothing)
+    all = all.join({e[s][0], e[s][1]});
+  const float mref = finite_ref(all.m);
   f4v o = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
     if (s >= S) break;
-    o += x[s] * exp2_(e[s][1] - R);
+    o += x[s] * exp2_(moved(e[s][1], e[s][0], mref) - all.D);
     den = fmaf(e[s][2], exp2_(e[s][0] - mref), den);
   }
-  const OutScale fin(R, M, den);
+  const OutScale fin(all.D, den);
   reinterpret_cast<f4v *>(out + ((int64_t)t * n_head + kvh * G + (id - t * G)) * HD)[d4] = fin(o);
 }
 
@@ -1165,7 +1196,7 @@ __global__ void __launch_bounds__(kWG)
 // Slower: two row tiles per wave (74 and 182 against 66 and 146 then), eight waves
 // (57 and 143), q's pieces from LDS, rescaling always (61 against 57).
 template <int HD>
-__global__ void __launch_bounds__(64 * kWaves)
+__global__ void __launch_bounds__(64 * kWaves, HD == 64 ? 4 : 1)
     k_kv8_tiles(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
                 int64_t T, int G, float scale, int tiles, int layer, float *__restrict__ part,
                 float *__restrict__ out) {
@@ -1203,7 +1234,8 @@ __global__ void __launch_bounds__(64 * kWaves)
   const int id = id0 + wave * 16 + r16;
   const bool live = id < rows;
   const int tok = live ? id / G : 0, g = live ? id - tok * G : 0;
-  const int64_t lim = sp.p0 + tok, qo = ((int64_t)tok * n_head + kvh * G + g) * HD;
+  const int lim = (int)sp.p0 + tok;  // the row's last position
+  const int64_t qo = ((int64_t)tok * n_head + kvh * G + g) * HD;
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
   const int8_t *kb = c.k + kvh * n_blocks * (kBlk * HD) + r16 * HD + 16 * cg;
   const int8_t *vb = c.v + kvh * n_blocks * (kBlk * HD) + r16 * 64 + 16 * cg;
@@ -1278,8 +1310,8 @@ __global__ void __launch_bounds__(64 * kWaves)
     if constexpr (MASK) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int64_t d = lim - ((int64_t)(2 * ch + u) * kBlk + 4 * cg);
-        last[u] = (int)(d > 64 ? 64 : d < -1 ? -1 : d);
+        const int d = lim - ((2 * ch + u) * kBlk + 4 * cg);
+        last[u] = d > 64 ? 64 : d < -1 ? -1 : d;
       }
     }
     softmax_step<HD, 2, MASK>(s, sc, qr.f, ks, vs, last, ph, pl);
@@ -1331,9 +1363,9 @@ __global__ void __launch_bounds__(64 * kWaves)
   }
   const float den = row_sum(s.l);
   if (!live) return;
-  const OutScale fin(s.R, s.m, den);
+  const OutScale fin(s.D, den);
   float *dst = S == 1 ? out + qo : part + (((int64_t)kvh * T * G + id) * S + split) * (HD + 4);
-  if (S > 1 && cg == 0) *reinterpret_cast<f4v *>(dst + HD) = f4v{s.m, s.R, den, 0.f};
+  if (S > 1 && cg == 0) *reinterpret_cast<f4v *>(dst + HD) = f4v{s.m, s.D, den, 0.f};
 #pragma unroll
   for (int i = 0; i < VJ; ++i) {
     f4v a = s.o[2 * i], b = s.o[2 * i + 1];

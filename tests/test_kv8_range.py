@@ -1,0 +1,152 @@
+"""Attention over the 8-bit KV cache with scores far from one: sizes of queries
+and keys whose products reach 2^24 and far beyond, equal scores among them, very
+small queries against very large keys and the other way round, V scales of each
+block their own; every form (split, tiles, step) against a float64 softmax over
+the coded values, within bounds derived below."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from tests.test_kv8 import B, coded, flat, inputs, values64
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def softmax_bound(q, K, V, amax, pos):
+    """q (T, n_head, hd), K / V (n, n_kv, hd) float64, amax (n, n_kv) the largest
+    |V| of each position's block: outputs and the bound of their error.
+
+    Scores are off by at most dz: hd products and their sums as a random walk
+    of six standard deviations, each step 2^-24 of the largest sum of
+    magnitudes, and the exponent's own rounding.  Each normalised weight w then
+    lies between w e^-2dz and min(1, w e^2dz), and as weights sum to one the
+    output moves by at most sum |w' - w| |v - out|.  The sums' and the last
+    roundings (n of 2^-24 as a random walk, 2^-22) go by the products that
+    enter them."""
+    T, n_head, hd = q.shape
+    G = n_head // K.shape[1]
+    out, tol = np.empty((2, T, n_head, hd))
+    for t in range(T):
+        n = pos + t + 1
+        for h in range(n_head):
+            k, v, am = K[:n, h // G], V[:n, h // G], amax[:n, h // G]
+            z = k @ q[t, h] / math.sqrt(hd)
+            logw = z - z.max() - math.log(np.exp(z - z.max()).sum())
+            out[t, h] = np.exp(logw) @ v
+            mag = (np.abs(k) @ np.abs(q[t, h])).max() / math.sqrt(hd)
+            dz = 6 * math.sqrt(hd) * 2.0 ** -24 * mag + 2.0 ** -24 * min(z.max() - z.min(), 100)
+            up, dn = np.exp(np.minimum(logw + 2 * dz, 0.0)), np.exp(logw - 2 * dz)
+            tol[t, h] = ((up - dn)[:, None] * np.abs(v - out[t, h])).sum(0)
+            tol[t, h] += (6 * math.sqrt(n) * 2.0 ** -24 + 2.0 ** -22) * (up * am).sum()
+    return out, tol
+
+
+def block_amax(v):
+    """(n, n_kv): the largest magnitude of each position's block."""
+    n = v.shape[0]
+    m = np.stack([np.abs(v[b:b + B]).max((0, 2)) for b in range(0, n, B)])
+    return np.repeat(m, B, axis=0)[:n].astype(np.float64)
+
+
+def scaled_blocks(rng, v, spread):
+    """v with a power of two of its own for each block, up to 2^spread either way."""
+    e = np.repeat(rng.integers(-spread, spread + 1, -(-v.shape[0] // B)), B)[:v.shape[0]]
+    return (v * np.exp2(e)[:, None, None]).astype(np.float32)
+
+
+def compare(got, q, k, v, pos, hd):
+    want, tol = softmax_bound(q.astype(np.float64), values64(*coded(k)), values64(*coded(v)),
+                              block_amax(v), pos)
+    got = got.cpu().numpy().reshape(want.shape).astype(np.float64)
+    assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:5]
+    err = np.abs(got - want)
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("hd,n_kv,G", [(64, 2, 4), (128, 1, 7), (256, 1, 2)])
+@pytest.mark.parametrize("size", [30.0, 300.0, 3e3, 1e4, 1e5, 1e8, 1e13, 1e18])
+def test_large_scores(hd, n_kv, G, T, size):
+    """q and k of this size each, so scores of about its square."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd + T)
+    n = 330
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    q, k = (q * np.float32(size)).astype(np.float32), (k * np.float32(size)).astype(np.float32)
+    v = scaled_blocks(rng, v, 20)
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    pos = n - T
+    compare(cache.attend(flat(q[pos:]), pos), q[pos:], k, v, pos, hd)
+
+
+@pytest.mark.parametrize("hd,n_kv,G", [(64, 2, 4), (128, 1, 7), (256, 1, 2)])
+@pytest.mark.parametrize("size", [3e3, 1e5, 1e18])
+def test_large_scores_of_a_step(hd, n_kv, G, size):
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd)
+    n = 200
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    q, k = (q * np.float32(size)).astype(np.float32), (k * np.float32(size)).astype(np.float32)
+    v = scaled_blocks(rng, v, 20)
+    cache = QuantKVCache(n_kv, n, hd)
+    for p in (0, 1, 31, 32, 150, 199):
+        if p > cache.length:
+            cache.store(flat(k[:p]), flat(v[:p]), 0)
+        got = cache.step(flat(q[p:p + 1]), flat(k[p:p + 1]), flat(v[p:p + 1]), p)
+        compare(got, q[p:p + 1], k[:p + 1], v[:p + 1], p, hd)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("size", [1.0, 300.0, 3e3, 1e4, 1e5, 1e9, 1e18])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_equal_large_scores(hd, size, T):
+    """Every block holds the same keys, so the scores of a position are equal
+    in every block, whatever their roundings, and whole blocks weigh alike;
+    their V scales differ.  Within a block the largest score leads by far
+    more than the roundings (asserted), so from size 300 on the output is the
+    mean of the blocks' values at that position."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(7 * hd + T)
+    nb, n_kv, G = 11, 2, 2
+    n = nb * B
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    # a leading position in each block: a key along the direction that the
+    # group's queries share but for a little noise; the rest small
+    q = (np.repeat(q[:1, ::G], G, axis=1) + 0.01 * q).astype(np.float32)
+    k = np.repeat(0.1 * k[:1], B, axis=0) * rng.uniform(0.1, 1, (B, 1, 1))
+    for h in range(n_kv):
+        k[5, h] = 2 * q[0, h * G]
+    k = np.tile(k, (nb, 1, 1))
+    q, k = ((x * size).astype(np.float32) for x in (q, k))
+    v = scaled_blocks(rng, v, 12)
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    pos = n - T
+    got = cache.attend(flat(q[pos:]), pos).cpu().numpy().reshape(T, n_kv * G, hd)
+    K, V = values64(*coded(k)), values64(*coded(v))
+    am = block_amax(v)
+    for t in range(T):
+        for h in range(n_kv * G):
+            seen = pos + t + 1
+            z = K[:B, h // G] @ q[pos + t, h].astype(np.float64) / math.sqrt(hd)  # of a block
+            mag = (np.abs(K[:B, h // G]) @ np.abs(q[pos + t, h]).astype(np.float64)).max()
+            dz = 6 * 2.0 ** -24 * mag + 2.0 ** -17
+            zs = np.resize(z, seen)
+            w = np.exp(zs - zs.max())
+            top = np.sort(z)
+            if size >= 300:
+                assert top[-1] - top[-2] > 2 * dz + 60
+                spread = 0.0  # (the others weigh nothing, the leading ones are equal)
+            else:
+                spread = math.expm1(2 * dz)
+            w /= w.sum()
+            want = w @ V[:seen, h // G]
+            tol = spread * (w[:, None] * np.abs(V[:seen, h // G] - want)).sum(0)
+            tol = tol + (6 * math.sqrt(seen) * 2.0 ** -24 + 2.0 ** -22) * (w * am[:seen, h // G]).sum()
+            err = np.abs(got[t, h] - want)
+            assert (err <= tol).all(), (t, h, (err / tol).max())
