@@ -598,17 +598,18 @@ __device__ __forceinline__ void pieces2(float a, float b, uint32_t &hi, uint32_t
 }
 
 // A lane's part of one query row: 8 dimensions 64 jj + 16 cg + 8 half .. per k
-// step ks = 2 jj + half, in pieces, and the factor that turns raw scores into
-// exponents of two (less the K scale).  A row with an infinity or a NaN gets
-// the factor NaN.
+// step ks = 2 jj + half, in pieces of the row times 2^-back.  back stays apart: as
+// part of a factor it would fall among the subnormals for small rows, whose keys
+// may be large.  The pieces of a row with an infinity or a NaN are NaN, and with
+// them its raw scores.
 template <int HD>
 struct QRow {
   h8 hi[HD / 32], lo[HD / 32];
-  float f;
+  int back;
   // ROPE: q is rotated for position pos on the way
   template <bool ROPE>
-  __device__ __forceinline__ void load(const float *__restrict__ q, bool live, int cg, float scale,
-                                       int64_t pos, const Rope &rope) {
+  __device__ __forceinline__ void load(const float *__restrict__ q, bool live, int cg, int64_t pos,
+                                       const Rope &rope) {
     float v[HD / 64][16];
     const uint32_t exists = ones_if(live);
     uint32_t am = 0;  // the largest magnitude, as bits (infinity's and NaNs' above all)
@@ -637,15 +638,16 @@ struct QRow {
     am = max(t[0], t[1]);
     const bool bad = am >= 0x7F800000u;
     const int up = am > 0 && !bad ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(am)) : 0;
-    f = bad ? __uint_as_float(0x7FC00000u) : ldexpf(scale * kLog2e, -up);
+    back = -up;
+    const float nan = __uint_as_float(0x7FC00000u);
     const uint32_t good = ones_if(!bad);
 #pragma unroll
     for (int ks = 0; ks < HD / 32; ++ks) {
       u4v h, l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i], up), 0.f);
-        const float b = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i + 1], up), 0.f);
+        const float a = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i], up), nan);
+        const float b = pick(good, ldexpf(v[ks >> 1][8 * (ks & 1) + 2 * i + 1], up), nan);
         uint32_t hh, ll;
         pieces2(a, b, hh, ll);
         h[i] = hh, l[i] = ll;
@@ -678,14 +680,16 @@ __device__ __forceinline__ float moved(float D, float m, float ref) {
 }
 
 // NB blocks' raw scores sc (two tiles of positions each) to weights in pieces,
-// with their K and V scales: m, D, l and o of the row move on.  MASK: only
-// positions up to last[b], counted from the lane's first one in block b, exist.
+// with their K and V scales: m, D, l and o of the row move on.  f, and 2^back of
+// the row: what turns raw scores into exponents of two (but for the K scale).
+// MASK: only positions up to last[b], counted from the lane's first one in block
+// b, exist.
 //
 // An exponent is one fma, whose product is not rounded while the maximum's is:
 // past kFine that would show (weights above what fp16 holds, or the largest one
 // lost), so there the scores are rounded products first, for the whole wave.
 template <int HD, int NB, bool MASK>
-__device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB], float f,
+__device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB], float f, int back,
                                              const float (&ks)[NB], const float (&vs)[NB],
                                              const int (&last)[NB], h8 (&ph)[NB], h8 (&pl)[NB]) {
   float c[NB], t[NB], ve[NB], mn = st.m, reach = 0.f;
@@ -700,7 +704,7 @@ __device__ __forceinline__ void softmax_step(RowState<HD> &st, f4v (&sc)[2 * NB]
   };
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    c[b] = ks[b] * f;
+    c[b] = ldexpf(ks[b], back) * f;
     const float mx = largest(b);
     const bool none = MASK && mx == -INFINITY;  // (not through a masked block's scale)
     t[b] = none ? mx : ceilf(mx * c[b]);
@@ -811,7 +815,7 @@ constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves 
 template <int HD, bool ROPE>
 __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     k_kv8_split(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
-                int64_t T, int G, float scale, float *__restrict__ part, float *__restrict__ out,
+                int64_t T, int G, float f, float *__restrict__ part, float *__restrict__ out,
                 const float *__restrict__ kn, const float *__restrict__ vn, Rope rope) {
   constexpr int NW = split_waves(HD, ROPE);
   constexpr int KJ = HD / 64, VJ = HD / 32, PS = HD + 4;
@@ -893,8 +897,7 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
   }
   QRow<HD> qr;
   if (!coding || asking)
-    qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, scale, sp.p0,
-                           rope);
+    qr.template load<ROPE>(q + ((int64_t)tok * n_head + kvh * G + g) * HD, live, cg, sp.p0, rope);
   RowState<HD> s;
   s.clear();
   auto compute = [&](int blk, Buf &x, auto mask) {
@@ -919,10 +922,10 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     if (MASK && first + kBlk - 1 > lim0) {  // (uniform) some row ends inside it or before
       const int64_t d = lim - first - 4 * cg;
       const int last[1] = {(int)(d > 64 ? 64 : d < -1 ? -1 : d)};
-      softmax_step<HD, 1, true>(s, sc, qr.f, ks, vs, last, ph, pl);
+      softmax_step<HD, 1, true>(s, sc, f, qr.back, ks, vs, last, ph, pl);
     } else {
       const int last[1] = {0};
-      softmax_step<HD, 1, false>(s, sc, qr.f, ks, vs, last, ph, pl);
+      softmax_step<HD, 1, false>(s, sc, f, qr.back, ks, vs, last, ph, pl);
     }
 #pragma unroll
     for (int i = 0; i < VJ; ++i) {
@@ -1198,7 +1201,7 @@ __global__ void __launch_bounds__(kWG)
 template <int HD>
 __global__ void __launch_bounds__(64 * kWaves, HD == 64 ? 4 : 1)
     k_kv8_tiles(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
-                int64_t T, int G, float scale, int tiles, int layer, float *__restrict__ part,
+                int64_t T, int G, float f, int tiles, int layer, float *__restrict__ part,
                 float *__restrict__ out) {
   constexpr int KJ = HD / 64, VJ = HD / 32, KS = HD / 32;
   constexpr int NU = HD / 64;  // 1 KB units of a chunk's K (and of its V) per wave
@@ -1314,7 +1317,7 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 64 ? 4 : 1)
         last[u] = d > 64 ? 64 : d < -1 ? -1 : d;
       }
     }
-    softmax_step<HD, 2, MASK>(s, sc, qr.f, ks, vs, last, ph, pl);
+    softmax_step<HD, 2, MASK>(s, sc, f, qr.back, ks, vs, last, ph, pl);
     const h8 (*v)[64] = vl[odd];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -1340,7 +1343,7 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 64 ? 4 : 1)
   fetch_k(c0);
   fetch_v(c0);
   scales(c0, ks, vs);
-  qr.template load<false>(q + qo, live, cg, scale, 0, Rope{});
+  qr.template load<false>(q + qo, live, cg, 0, Rope{});
   stage(rk, kl[0]);
   stage(rv, vl[0]);
   fetch_k(c0 + 1);
@@ -1458,10 +1461,13 @@ int kv8_tile_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int cus) {
   return pick;
 }
 
+// scores to exponents of two
+static float score_factor(int head_dim) { return (float)(1.0 / sqrt((double)head_dim)) * kLog2e; }
+
 hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int n_head,
                                 const aq_decode_state *st, int64_t pos0, float *out,
                                 hipStream_t s) {
-  const float scale = (float)(1.0 / sqrt((double)c.head_dim));
+  const float f = score_factor(c.head_dim);
   const int G = n_head / c.n_kv;
   const int64_t rows = T * G;
   int S;
@@ -1471,7 +1477,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
     AQ_HD(c.head_dim,
           hipLaunchKernelGGL((k_kv8_split<HD, false>),
                              dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
-                             dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, scale, c.scratch, out,
+                             dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, f, c.scratch, out,
                              nullptr, nullptr, Rope{}))
   } else {
     int dev = 0;
@@ -1485,7 +1491,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
           if (hipError_t e = set_dynamic_lds(reinterpret_cast<const void *>(k_kv8_tiles<HD>), lds))
             return e;
           hipLaunchKernelGGL(k_kv8_tiles<HD>, dim3((unsigned)(tiles * c.n_kv), (unsigned)S),
-                             dim3(64 * kWaves), lds, s, q, c, st, pos0, T, G, scale, (int)tiles,
+                             dim3(64 * kWaves), lds, s, q, c, st, pos0, T, G, f, (int)tiles,
                              layer, c.scratch, out))
   }
   if (S > 1 && S <= kFewSplits) {
@@ -1506,13 +1512,13 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      int n_rot, int neox, const float *cos_t, const float *sin_t,
                                      const aq_decode_state *st, int64_t pos0, const aq_kv8 &c,
                                      float *out, hipStream_t s) {
-  const float scale = (float)(1.0 / sqrt((double)c.head_dim));
+  const float f = score_factor(c.head_dim);
   const int G = n_head / c.n_kv;
   AQ_HD(c.head_dim,
         constexpr int NW = split_waves(HD, true);
         const int S = kv8_splits(c, 1, n_head, NW) + 1;
         hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
-                           dim3(64 * NW), 0, s, q, c, st, pos0, (int64_t)1, G, scale,
+                           dim3(64 * NW), 0, s, q, c, st, pos0, (int64_t)1, G, f,
                            c.scratch, out, k, v, Rope{cos_t, sin_t, n_rot, neox});
         hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)G, (unsigned)c.n_kv), dim3(kWG), 0, s,
                            c.scratch, st, pos0, c.n_ctx, (int64_t)1, G, S, out))

@@ -10,7 +10,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_kv8 import B, coded, flat, inputs, values64
+from tests.test_kv8 import B, attention64, coded, flat, inputs, values64
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -150,3 +150,72 @@ def test_equal_large_scores(hd, size, T):
             tol = tol + (6 * math.sqrt(seen) * 2.0 ** -24 + 2.0 ** -22) * (w * am[:seen, h // G]).sum()
             err = np.abs(got[t, h] - want)
             assert (err <= tol).all(), (t, h, (err / tol).max())
+
+
+UNIT = 2.0 ** -149  # of the subnormal numbers
+
+
+def of_units(u):
+    """Whole units 2^-149 (magnitudes below 2^24) as float32 on the GPU, from
+    their bits: a CPU that flushes subnormals does not show."""
+    a = np.abs(u)
+    # (below 2^24 the units are the bits: the first binade has the subnormals' unit)
+    bits = (a | np.where(u < 0, 1 << 31, 0)).astype(np.uint32)
+    return torch.from_numpy(np.ascontiguousarray(bits).view(np.int32)).cuda().view(torch.float32)
+
+
+def signed(rng, lo, hi, shape):
+    return rng.uniform(lo, hi, shape) * rng.choice([-1.0, 1.0], shape)
+
+
+def within(got, want, tol):
+    got = got.cpu().numpy().reshape(want.shape)
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("hd,n_kv,G", [(64, 2, 4), (128, 1, 7), (256, 1, 2)])
+@pytest.mark.parametrize("q_units,ks", [(2.0 ** 24, 1e37), (2.0 ** 22, 1e38), (2.0 ** 14, 3e38)])
+def test_small_queries_and_large_keys(hd, n_kv, G, T, q_units, ks):
+    """Queries of up to q_units 2^-149 (2e-38, the first two rows about the
+    border of the subnormals, the last far below it), keys near the largest
+    float: scores of about 1, 1 and 0.1."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd + T)
+    n = 230
+    u = np.rint(signed(rng, 0.25 * q_units, 0.99 * q_units, (n, n_kv * G, hd))).astype(np.int64)
+    k = signed(rng, 0.25 * ks, ks, (n, n_kv, hd)).astype(np.float32)
+    v = signed(rng, 0.25, 1, (n, n_kv, hd)).astype(np.float32)
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    pos = n - T
+    want, tol = attention64(u[pos:] * UNIT, values64(*coded(k)), values64(*coded(v)), pos)
+    within(cache.attend(of_units(u[pos:].reshape(T, -1)), pos), want, tol)
+    if T == 1:
+        got = cache.step(of_units(u[pos:].reshape(T, -1)), flat(k[pos:]), flat(v[pos:]), pos)
+        within(got, want, tol)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("hd,n_kv,G", [(64, 2, 4), (128, 1, 7), (256, 1, 2)])
+@pytest.mark.parametrize("k_units,qs", [(127.0, 3e38), (127.0 * 7, 3e38), (127.0 * 30000, 1e38)])
+def test_large_queries_and_small_keys(hd, n_kv, G, T, k_units, qs):
+    """Queries near the largest float, keys of up to k_units 2^-149, whose
+    scales are a few units themselves."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd + T)
+    n = 230
+    q = signed(rng, 0.25 * qs, qs, (n, n_kv * G, hd)).astype(np.float32)
+    u = np.rint(signed(rng, 0.1 * k_units, k_units, (n, n_kv, hd))).astype(np.int64)
+    v = signed(rng, 0.25, 1, (n, n_kv, hd)).astype(np.float32)
+    s = np.stack([np.rint(np.abs(u[b:b + B]).max((0, 2)) / 127) for b in range(0, n, B)])
+    s = np.repeat(s, B, axis=0)[:n, :, None]
+    K = np.clip(np.rint(u / s), -127, 127) * s * UNIT
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(of_units(u.reshape(n, -1)), flat(v), 0)
+    pos = n - T
+    want, tol = attention64(q[pos:].astype(np.float64), K, values64(*coded(v)), pos)
+    within(cache.attend(flat(q[pos:]), pos), want, tol)
+    if T == 1:
+        got = cache.step(flat(q[pos:]), of_units(u[pos:].reshape(1, -1)), flat(v[pos:]), pos)
+        within(got, want, tol)
