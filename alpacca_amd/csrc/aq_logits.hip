@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kWG)
   const int64_t *w = window ? window + row * (1 + last_n) : nullptr;
   int64_t tok[kAhead], id[kAhead];
   int64_t a = bias_off && n_bias ? bias_off[row] : 0, b = bias_off && n_bias ? bias_off[row + 1] : n_bias;
-  a = a > 0 ? a : 0;
+  a = a < 0 ? 0 : a < n_bias ? a : n_bias;  // (also: a + j below does not wrap)
   b = b < n_bias ? b : n_bias;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {

@@ -201,3 +201,17 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             bad()
     assert adjust_logits(x[:0]).shape == (0, 40)
+
+
+@gpu
+def test_bias_offsets_past_the_list():
+    """Offsets are clipped to the list, the largest 64-bit ones too: such a row
+    owns no entry, or all from its start on."""
+    big = 2 ** 63 - 1
+    rows, n = 5, 1500
+    x = np.linspace(-2, 2, rows * n, dtype=np.float32).reshape(rows, n)
+    ids = np.arange(0, 1200, 2, dtype=np.int64)
+    val = np.linspace(-1, 1, 600, dtype=np.float32)
+    for off in ([big, big, big - 300, 590, big, big], [-big - 1, big, 0, 3, big, -big - 1],
+                [590, big, 599, big - 1200, 600, 601]):
+        check(x, None, None, (ids, val, np.array(off, np.int64)), None)
