@@ -191,7 +191,7 @@ struct Coder {
   // the sum's low bits
   __device__ __forceinline__ uint4 operator()(const float (&x)[16]) const {
     uint32_t t[16], w[4];
-    if (!(s >= 0.f)) return make_uint4(0, 0, 0, 0);
+    if (!(s > 0.f)) return make_uint4(0, 0, 0, 0);  // (0 or NaN)
     float far = lift - 1.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {

@@ -164,6 +164,34 @@ def of_units(u):
     return torch.from_numpy(np.ascontiguousarray(bits).view(np.int32)).cuda().view(torch.float32)
 
 
+def test_codes_of_a_zero_scale():
+    """A block whose largest magnitude is below 64 units 2^-149 has the scale
+    0, and then every code is 0 and every value +0, in the store and in the
+    step, also where a later token gives the block a scale."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(12)
+    n_kv, hd = 2, 64
+    for top in (1, 5, 63):
+        u = rng.integers(-top, top + 1, (40, n_kv * hd))
+        u[::B, ::hd] = -top
+        x = of_units(u)
+        cache = QuantKVCache(n_kv, 64, hd)
+        cache.store(x, x, 0)
+        q = torch.ones(1, n_kv * hd, device="cuda")
+        assert (cache.attend(q, 39) == 0).all()
+        for p in (None, 40):
+            if p:
+                cache.step(q, x[39:], x[39:], p)
+            for t in (cache.k, cache.v):
+                assert (t == 0).all()
+            for t in (*cache.read(), cache.k_scale, cache.v_scale):
+                assert (t.view(torch.int32) == 0).all()  # (no -0 either)
+        cache.step(q, torch.ones_like(q), torch.ones_like(q), 41)
+        for t in cache.read():
+            assert (t[:, :41].view(torch.int32) & 0x7FFFFFFF == 0).all()
+            assert (t[:, 41] == np.float32(1) / np.float32(127) * 127).all()
+
+
 def signed(rng, lo, hi, shape):
     return rng.uniform(lo, hi, shape) * rng.choice([-1.0, 1.0], shape)
 
