@@ -212,6 +212,7 @@ class Model:
         self.stream.wait_stream(torch.cuda.current_stream(self.dev))
         self.n_past = 0
         self.cached_ids: list[int] = []
+        self._kv_end = 0  # the position after the one that was stored last
         # batched prefill: chunk size (ALPACCA_PREFILL_CHUNK, model.py:630-634)
         # and matmul precision (fp32: the reference's f32 products).  The
         # reference's 256 bounds host memory; here the chunk only sets how
@@ -388,6 +389,7 @@ class Model:
             self._enqueue_advance(False)
         self.stream.synchronize()
         self.n_past += 1
+        self._kv_end = self.n_past
         self.cached_ids.append(token)
         return self.logits.cpu().numpy()
 
@@ -410,9 +412,9 @@ class Model:
             n = max(0, len(tokens) - 1)
         if n != self.n_past:
             n = min(n, self.n_past)
-            # an 8-bit cache goes back exactly inside its last block, or to a
-            # block's start (in between it would code coded values anew)
-            if self.kv8 and n // KV_BLOCK != (self.n_past - 1) // KV_BLOCK:
+            # an 8-bit cache goes back exactly inside the block stored last, or
+            # to a block's start (in between it would code coded values anew)
+            if self.kv8 and n // KV_BLOCK != (self._kv_end - 1) // KV_BLOCK:
                 n -= n % KV_BLOCK
             self.n_past = n
             del self.cached_ids[n:]
@@ -514,6 +516,7 @@ class Model:
                     else:
                         chk(lib.aq_add(p(X), p(O), T * hp.n_embd, sv))
                 self.n_past += T
+                self._kv_end = self.n_past
             self.x.copy_(X[T - 1])
             self._enqueue_head()
         self.cached_ids.extend(tokens)
@@ -541,6 +544,7 @@ class Model:
                 self._enqueue_advance(False, prompt)
         self.stream.synchronize()
         self.n_past += len(tokens)
+        self._kv_end = self.n_past
         self.cached_ids.extend(tokens)
 
     def generate_greedy(self, prompt: list[int], n_gen: int, graph: bool = True,
@@ -699,7 +703,7 @@ class Model:
             timing["steps"] = n_gen - 1
             timing["prefill_ms"] = t_pf * 1e3  # host wall clock, synchronized
         out = [int(t) for t in hist.cpu().tolist()]
-        self.n_past = n_p + n_gen - 1
+        self.n_past = self._kv_end = n_p + n_gen - 1
         self.cached_ids = list(prompt) + out[:-1]
         return out
 
