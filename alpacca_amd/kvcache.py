@@ -27,6 +27,15 @@ HEAD_DIMS = (64, 128, 256)
 MAX_GROUP = 16  # query heads per kv head
 
 
+def check_heads(n_head: int, n_kv: int, head_dim: int) -> None:
+    """ValueError for heads that the 8-bit cache's attention does not take."""
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"the 8-bit KV cache takes head_dim {HEAD_DIMS}, got {head_dim}")
+    if n_kv < 1 or n_head < 1 or n_head % n_kv or n_head // n_kv > MAX_GROUP:
+        raise ValueError(f"the 8-bit KV cache takes 1 to {MAX_GROUP} query heads per kv head, "
+                         f"got {n_head} for {n_kv}")
+
+
 class QuantKVCache:
     """n_ctx positions of n_kv heads of head_dim, on `device` (default: the
     current one).  ValueError for an unsupported shape.  `scratch`: another
@@ -243,4 +252,4 @@ class QuantKVCache:
         return kv.unbind()
 
 
-__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "QuantKVCache"]
+__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "QuantKVCache", "check_heads"]

@@ -38,7 +38,7 @@ import numpy as np
 
 from . import _lib
 from .kvcache import BLOCK as KV_BLOCK
-from .kvcache import QuantKVCache
+from .kvcache import QuantKVCache, check_heads
 from .logits import adjust_logits, pack_mask
 from .qmatrix import (DENSE_DTYPES, MIXABLE_DTYPES, DenseMatrix, QuantMatrix,
                       interleave_rows, matvec_fused_device, matvec_multi_device,
@@ -96,6 +96,8 @@ class Model:
         import torch
         if kv_dtype not in ("f32", "q8"):
             raise ValueError(f"unknown kv_dtype {kv_dtype!r} (f32, q8)")
+        if kv_dtype == "q8":
+            check_heads(hp.n_head, hp.n_kv, hp.head_dim)
         if not torch.cuda.is_available():
             raise RuntimeError("alpacca_amd.model.Model needs a HIP device (gfx950)")
         _lib.ensure_device()
