@@ -580,7 +580,9 @@ class Model:
         logit_bias ({token: bias}) is added, and tokens that `allowed` (n_vocab
         truth values) leaves out are never chosen: with any of these the
         logits of every step, the repetition penalty among the rest, go
-        through adjust_logits before the argmax (rounded to float32 there)."""
+        through adjust_logits before the argmax (rounded to float32 there).
+        ValueError where every allowed token's bias is -inf, RuntimeError
+        (and an empty cache) where a step left no allowed logit above -inf."""
         torch = self.torch
         if not prompt or n_gen < 1:
             raise ValueError("need a non-empty prompt and n_gen >= 1")
@@ -598,7 +600,8 @@ class Model:
         hist = torch.zeros(n_gen, dtype=torch.int64, device=self.dev)
         n_p = len(prompt)
         window = None
-        adjust = self._adjustment(presence_penalty, frequency_penalty, logit_bias, allowed)
+        adjust, permitted = self._adjustment(presence_penalty, frequency_penalty, logit_bias,
+                                             allowed)
         if adjust is not None and (penalize or presence_penalty or frequency_penalty):
             adjust["penalties"] = torch.tensor(
                 [[repeat_penalty if penalize else 1.0, presence_penalty, frequency_penalty]],
@@ -705,24 +708,34 @@ class Model:
             timing["steps"] = n_gen - 1
             timing["prefill_ms"] = t_pf * 1e3  # host wall clock, synchronized
         out = [int(t) for t in hist.cpu().tolist()]
+        # (among logits that are all -inf the argmax is the lowest token)
+        if permitted is not None and not permitted[out].all():
+            self.reset()
+            raise RuntimeError("no allowed token's logit is above -inf at generated token "
+                               f"{int(np.argmin(permitted[out]))}")
         self.n_past = self._kv_end = n_p + n_gen - 1
         self.cached_ids = list(prompt) + out[:-1]
         return out
 
-    def _adjustment(self, presence: float, frequency: float, bias, allowed) -> dict | None:
-        """adjust_logits' arguments for one row but the window and penalties;
-        None when there is nothing to adjust but a repetition penalty."""
+    def _adjustment(self, presence: float, frequency: float, bias, allowed) -> tuple:
+        """adjust_logits' arguments for one row but the window and penalties
+        (None when there is nothing to adjust but a repetition penalty), and
+        the allowed tokens as a host array, or None."""
         torch, n = self.torch, self.hp.n_vocab
         if not (presence or frequency or bias or allowed is not None):
-            return None
-        out = {}
+            return None, None
+        out, permitted, banned = {}, None, []
         if bias:
             ids = [int(t) for t in bias]
             if min(ids) < 0 or max(ids) >= n:
                 raise IndexError("logit_bias token out of range")
-            vals = np.array([float(v) for v in bias.values()], dtype=np.float32)
-            if np.isnan(vals).any():
+            wide = np.array([float(v) for v in bias.values()])
+            if np.isnan(wide).any():
                 raise ValueError("logit_bias must not be NaN")
+            if (np.isfinite(wide) & (np.abs(wide) > np.finfo(np.float32).max)).any():
+                raise ValueError("logit_bias past float32's range")
+            vals = wide.astype(np.float32)
+            banned = [t for t, v in zip(ids, wide) if v == -np.inf]
             out["bias"] = (torch.tensor(ids, dtype=torch.int64, device=self.dev),
                            torch.from_numpy(vals).to(self.dev))
         if allowed is not None:
@@ -732,8 +745,11 @@ class Model:
                 raise ValueError(f"allowed must hold {n} truth values")
             if not bool(ok.any()):
                 raise ValueError("allowed leaves no token")
+            permitted = ok.numpy()
+            if permitted.sum() == permitted[banned].sum():
+                raise ValueError("every allowed token's logit_bias is -inf")
             out["mask"] = pack_mask(ok.to(self.dev))
-        return out
+        return out, permitted
 
     def _capture(self, fn):
         """One eager run of fn (sizes the library's per-stream workspace

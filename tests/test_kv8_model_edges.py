@@ -35,3 +35,43 @@ def test_going_back_after_a_refused_prompt(batch, cut):
             a.length = b.length = len(new)
             for x, y in zip(a.read(), b.read()):
                 assert torch.equal(x, y), keep
+
+
+def test_allowed_tokens_that_are_banned():
+    """A token outside the mask is never returned: refused before the first
+    step where every allowed token's bias is -inf, and a RuntimeError where
+    the penalties leave no allowed logit above -inf."""
+    hp, tensors = tiny()
+    m = model(hp, tensors)
+    ban = float("-inf")
+
+    def only(*ids):
+        a = np.zeros(hp.n_vocab, bool)
+        a[list(ids)] = True
+        return a
+    for graph in (True, False):
+        with pytest.raises(ValueError, match="allowed"):
+            m.generate_greedy([1, 2], 4, graph=graph, allowed=only(5), logit_bias={5: ban})
+        with pytest.raises(ValueError, match="allowed"):
+            m.generate_greedy([1, 2], 4, graph=graph, allowed=only(5, 9),
+                              logit_bias={9: ban, 5: ban, 3: 1.0})
+        assert m.generate_greedy([1, 2], 4, graph=graph, allowed=only(5, 9),
+                                 logit_bias={9: ban}) == [5] * 4
+        # each said token falls to -inf: two steps leave nothing, one token more fails
+        kw = dict(graph=graph, allowed=only(5, 9), presence_penalty=1e39)
+        assert sorted(m.generate_greedy([1, 2], 2, **kw)) == [5, 9]
+        with pytest.raises(RuntimeError, match="allowed"):
+            m.generate_greedy([1, 2], 3, **kw)
+        assert m.n_past == 0 and m.cached_ids == []
+    # the model is as it was
+    want = model(hp, tensors).generate_greedy([1, 2], 6)
+    assert m.generate_greedy([1, 2], 6) == want
+
+
+def test_biases_past_float32():
+    hp, tensors = tiny()
+    m = model(hp, tensors)
+    for v in (1e39, -1e39):
+        with pytest.raises(ValueError, match="float32"):
+            m.generate_greedy([1, 2], 2, logit_bias={3: v})
+    assert m.generate_greedy([1, 2], 2, logit_bias={3: float("inf")}) == [3, 3]
