@@ -215,3 +215,58 @@ def test_bias_offsets_past_the_list():
     for off in ([big, big, big - 300, 590, big, big], [-big - 1, big, 0, 3, big, -big - 1],
                 [590, big, 599, big - 1200, 600, 601]):
         check(x, None, None, (ids, val, np.array(off, np.int64)), None)
+
+
+def batch_inputs(rng, rows, n, last_n):
+    x = (3 * rng.standard_normal((rows, n))).astype(np.float32)
+    window = np.empty((rows, 1 + last_n), np.int64)
+    window[:, 0] = rng.integers(0, 2 * last_n + 1, rows)
+    window[:, 1:] = (n * rng.random((rows, last_n)) ** 3).astype(np.int64)
+    pen = np.stack([rng.uniform(0.8, 1.4, rows), rng.uniform(-1, 1, rows),
+                    rng.uniform(-0.5, 0.5, rows)], axis=1)
+    off = np.concatenate([[0], np.cumsum(rng.integers(0, 1500, rows))]).astype(np.int64)
+    ids = rng.integers(0, n, off[-1]).astype(np.int64)
+    val = (4 * rng.standard_normal(off[-1])).astype(np.float32)
+    allowed = rng.random((rows, n)) < 0.6
+    allowed[rows // 2] = False
+    return x, window, pen, (ids, val, off), allowed
+
+
+@gpu
+@pytest.mark.parametrize("rows,n,last_n", [(64, 32771, 700), (33, 65537, 1500), (1025, 1999, 40),
+                                           (1024, 2048, 70), (512, 2049, 70), (16, 131073, 64)])
+def test_adjust_large_batches(rows, n, last_n):
+    """From 1024 slices of 2048 logits on (rows x n): windows, ragged biases of
+    more entries than a workgroup has threads, a mask per row that leaves one
+    with nothing."""
+    rng = np.random.default_rng(rows + n)
+    assert rows * -(-n // 2048) >= 1024
+    x, window, pen, bias, allowed = batch_inputs(rng, rows, n, last_n)
+    x[:, ::97] = np.inf
+    x[:, 5::89] = np.nan
+    check(x, window, pen, bias, allowed)
+    check(x, None, None, bias, allowed[0])
+    check(x, window, pen, None, None)
+
+
+@gpu
+@pytest.mark.parametrize("n", [32771, 4099])
+def test_adjust_rows_alone_and_in_batches(n):
+    """A row's logits are the same bits in a batch on either side of the border
+    between the slices' sizes, and alone."""
+    from alpacca_amd.logits import adjust_logits, pack_mask
+    words = -(-n // 2048)
+    above = -(-1024 // words)
+    rng = np.random.default_rng(n)
+    x, window, pen, (ids, val, off), allowed = batch_inputs(rng, above, n, 200)
+
+    def run(rows, out_of_place):
+        xd = dev(x[:rows])
+        return adjust_logits(xd, window=dev(window[:rows]), penalties=dev(pen[:rows]),
+                             bias=(dev(ids), dev(val), dev(off[:rows + 1])),
+                             mask=pack_mask(dev(allowed[:rows])),
+                             out=None if out_of_place else xd).view(torch.int32)
+    assert above * words >= 1024 > (above - 1) * words
+    for fresh in (True, False):
+        many, fewer, one = (run(rows, fresh) for rows in (above, above - 1, 1))
+        assert torch.equal(many[:-1], fewer) and torch.equal(many[:1], one)
