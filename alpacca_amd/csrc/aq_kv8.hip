@@ -1388,8 +1388,8 @@ constexpr int64_t kScratchRows = 65536;
 // most rows per kv head for the split kernel: it converts every block once per
 // tile of 16 rows, the tiles kernel once per 64, but by way of LDS and barriers.
 // 32/8 heads of 128 after 8000 positions, split against tiles: 32 rows 14.8 / 20.5
-// us, 64 18.2 / 20.6, 128 24.1 / 26.3, 256 36.0 / 38.9; heads of 256 (groups of 2):
-// 64 rows 24.9 / 26.1, 128 30.7 / 30.2.
+// us, 64 18.2 / 20.6, 128 24.1 / 26.3, 256 36.0 / 38.9; 16/8 heads of 256: 64 rows
+// 26.4 / 52.9, 128 38.2 / 53.7, 256 62.0 / 56.0.
 constexpr int64_t kSplitRows = 256;
 size_t kv8_scratch_bytes(int head_dim) {
   return (size_t)kScratchRows * (head_dim + 4) * sizeof(float);
@@ -1430,12 +1430,20 @@ hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, 
 // position, which the host may not know: a call gives the same bits however it
 // is told where it is.
 //
-// The split kernel: about two workgroups per CU, no more than give every wave a
-// block of a full cache, nor than the scratch holds (the step has one more).
-int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves) {
-  const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
+// Workgroups of the split and of the tiles kernel that a CU has the registers for
+// at once: heads of 256 take more than half of a SIMD's per wave (and the tiles
+// 128 KB of LDS), so one; a second turn is then no faster than a second launch.
+constexpr int kv8_residents(int head_dim) { return head_dim == 256 ? 1 : 2; }
+// The split kernel: as many workgroups as 256 CUs hold (but one, at most one more
+// for heads up to 128), no more than give every wave a block of a full cache, nor
+// than the scratch holds.  more: workgroups per kv head beside them (the step's).
+// Heads of 256, 8 kv heads, 32767 positions: 32 splits 28.8 us, 64 33.4; 4 kv
+// heads: 64 splits 20.6, 128 27.2; the step of 8 kv heads: TODO.
+int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves, int more) {
+  const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk, groups = c.n_kv * tiles;
   int64_t S = (n_blocks + waves - 1) / waves;
-  const int64_t fill = (kMaxSplits - 1 + c.n_kv * tiles - 1) / (c.n_kv * tiles);
+  const int64_t fill = kv8_residents(c.head_dim) == 1 ? (256 - more * c.n_kv) / groups
+                                                      : (kMaxSplits - 2 + groups) / groups;
   const int64_t room = kScratchRows / rows - 1;
   S = S < fill ? S : fill;
   S = S < room ? S : room;
@@ -1447,11 +1455,12 @@ int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves) {
 // tokens at 8000 172 us whole, 85 split; 64 of heads of 256 (groups of 2) at 1000 56, 27.
 int kv8_tile_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int cus) {
   const double chunks = (double)((c.n_ctx + 2 * kBlk - 1) / (2 * kBlk));
+  const double beside = kv8_residents(c.head_dim) == 1 ? 1.0 : 0.65;
   double best = 0.0;
   int pick = 1;
   for (int S = 1; S <= kFewSplits && S <= chunks && (S == 1 || rows * S <= kScratchRows); ++S) {
     const double turns = ceil((double)(tiles * c.n_kv * S) / cus);
-    const double t = ceil(chunks / S) * (c.head_dim / 96.0) * (turns > 1 ? 0.65 * turns : 1.0) +
+    const double t = ceil(chunks / S) * (c.head_dim / 96.0) * (turns > 1 ? beside * turns : 1.0) +
                      (S > 1 ? 4.0 + (double)rows * S * (c.head_dim + 4) * 8 / 4e6 : 0.0);
     if (S == 1 || t < best) {
       best = t;
@@ -1473,7 +1482,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
   int S;
   if (rows <= kSplitRows) {
     const int64_t tiles = (rows + 15) / 16;
-    S = kv8_splits(c, tiles, T * n_head, kWaves);
+    S = kv8_splits(c, tiles, T * n_head, kWaves, 0);
     AQ_HD(c.head_dim,
           hipLaunchKernelGGL((k_kv8_split<HD, false>),
                              dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
@@ -1516,7 +1525,7 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
   const int G = n_head / c.n_kv;
   AQ_HD(c.head_dim,
         constexpr int NW = split_waves(HD, true);
-        const int S = kv8_splits(c, 1, n_head, NW) + 1;
+        const int S = kv8_splits(c, 1, n_head, NW, 1) + 1;
         hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
                            dim3(64 * NW), 0, s, q, c, st, pos0, (int64_t)1, G, f,
                            c.scratch, out, k, v, Rope{cos_t, sin_t, n_rot, neox});
