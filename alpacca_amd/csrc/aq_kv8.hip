@@ -553,6 +553,16 @@ __device__ __forceinline__ float row_sum(float v) {
   p = lane_pair<32>(p.x + p.y);
   return p.x + p.y;
 }
+__device__ __forceinline__ float wave_max(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __uint_as_float(dppu<decltype(ctrl)::value>(__float_as_uint(x)));
+  };
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0xB1>()));   // quad_perm [1,0,3,2]
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4E>()));   // quad_perm [2,3,0,1]
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
+  return row_max(v);
+}
 // a float that no store of this kernel reaches, at a wave's common place: a
 // scalar load
 __device__ __forceinline__ float load_const(const float *p) {
@@ -781,14 +791,20 @@ struct OutScale {
     return v * a * inv * b;
   }
 };
-// two states' references joined
+// the maximum and the reference of N states joined: m(i), D(i) of each
 struct Ref {
   float m, D;
-  __device__ __forceinline__ Ref join(const Ref &o) const {
-    const float n = fmaxf(m, o.m), ref = finite_ref(n);
-    return {n, fmaxf(moved(D, m, ref), moved(o.D, o.m, ref))};
-  }
 };
+template <int N, class M, class R>
+__device__ __forceinline__ Ref joined(M m, R D) {
+  Ref all{m(0), kLow};
+#pragma unroll
+  for (int i = 1; i < N; ++i) all.m = fmaxf(all.m, m(i));
+  const float ref = finite_ref(all.m);
+#pragma unroll
+  for (int i = 0; i < N; ++i) all.D = fmaxf(all.D, moved(D(i), m(i), ref));
+  return all;
+}
 
 // ---- few rows: the positions split over workgroups -------------------------------
 // Workgroup (split j, kv head, tile of 16 rows): wave w takes blocks 4 j + w, + 4 S
@@ -1033,8 +1049,8 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     for (int i = 0; i < 2 * VP; ++i) os[wave][i][lane] = s.o[2 * VP * h + i];
     __syncthreads();
     if (h == 0) {
-#pragma unroll
-      for (int w = 0; w < NW; ++w) all = all.join({stat[w][0][r16], stat[w][1][r16]});
+      all = joined<NW>([&](int w) { return stat[w][0][r16]; },
+                       [&](int w) { return stat[w][1][r16]; });
       const float mref = finite_ref(all.m);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
@@ -1094,18 +1110,16 @@ __global__ void __launch_bounds__(kWG)
   }
   const Span sp = span_of(st, pos0, T, n_ctx);
   if (t >= sp.n) return;
-  Ref all = Ref{e[0][0], e[0][1]}.join({e[1][0], e[1][1]});
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    all = all.join({__shfl_xor(all.m, off), __shfl_xor(all.D, off)});
+  // (the wave's maximum, then its reference counted from it, then the waves')
+  const float wm = wave_max(fmaxf(e[0][0], e[1][0])), wref = finite_ref(wm);
+  const float wd = wave_max(fmaxf(moved(e[0][1], e[0][0], wref), moved(e[1][1], e[1][0], wref)));
   if ((tid & 63) == 0) {
-    red[0][tid >> 6] = all.m;
-    red[1][tid >> 6] = all.D;
+    red[0][tid >> 6] = wm;
+    red[1][tid >> 6] = wd;
   }
   __syncthreads();
-  all = {red[0][0], red[1][0]};
-#pragma unroll
-  for (int w = 1; w < kWG / 64; ++w) all = all.join({red[0][w], red[1][w]});
+  const Ref all = joined<kWG / 64>([&](int w) { return red[0][w]; },
+                                   [&](int w) { return red[1][w]; });
   const float mref = finite_ref(all.m);
   float den = 0.f;
 #pragma unroll
@@ -1164,10 +1178,9 @@ __global__ void __launch_bounds__(kWG)
     x[s] = *reinterpret_cast<const f4v *>(ps + 4 * d4);
     e[s] = *reinterpret_cast<const f4v *>(ps + HD);
   }
-  Ref all{e[0][0], e[0][1]};
-#pragma unroll
-  for (int s = 1; s < kFewSplits; ++s)  // (repeats of the first split change nothing)
-    all = all.join({e[s][0], e[s][1]});
+  // (repeats of the first split change nothing)
+  const Ref all = joined<kFewSplits>([&](int s) { return e[s][0]; },
+                                     [&](int s) { return e[s][1]; });
   const float mref = finite_ref(all.m);
   f4v o = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
