@@ -1,7 +1,8 @@
 """QuantKVCache: the keys and values of one attention layer in 8 bits, in HBM.
 
 A quarter of the fp32 cache's bytes (the reference keeps fp32,
-alpacca/model.py:368-371).  Blocks of 32 positions of one kv head share a
+alpacca/model.py:368-371), and a scratch of 18, 35 or 68 MB (head_dim 64, 128,
+256) that a model's layers share.  Blocks of 32 positions of one kv head share a
 scale, K and V apart; attention has float32 accuracy over the coded values
 (include/alpacca_amd.h, aq_kv8, has the exact rules).
 
@@ -40,7 +41,8 @@ class QuantKVCache:
     """n_ctx positions of n_kv heads of head_dim, on `device` (default: the
     current one).  ValueError for an unsupported shape.  `scratch`: another
     cache whose scratch this one shares (same head_dim and device), for caches
-    whose calls are ordered, like a model's layers."""
+    whose calls are ordered, like a model's layers; without it the cache makes
+    its own (scratch_nbytes), which for a short context is more than the cache."""
 
     def __init__(self, n_kv: int, n_ctx: int, head_dim: int, device=None, scratch=None):
         import torch
@@ -86,6 +88,10 @@ class QuantKVCache:
         return sum(t.numel() * t.element_size()
                    for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail,
                              self.v_tail))
+
+    def scratch_nbytes(self) -> int:
+        """Bytes of the attention's scratch, which caches may share."""
+        return self._scratch.numel() * self._scratch.element_size()
 
     def reset(self) -> None:
         """Forget what is stored."""

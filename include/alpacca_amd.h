@@ -466,8 +466,9 @@ typedef struct aq_kv8 {
   int32_t n_kv, head_dim;
 } aq_kv8;
 
-/* Bytes of each codes array, each scales array, each tail and the scratch.
- * Host only.  AQ_ERR_VALUE for an unsupported shape. */
+/* Bytes of each codes array, each scales array, each tail and the scratch (18,
+ * 35 or 68 MB for head_dim 64, 128, 256; caches whose calls are ordered may share
+ * one).  Host only.  AQ_ERR_VALUE for an unsupported shape. */
 int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *scales,
                  size_t *tail, size_t *scratch);
 

@@ -75,3 +75,19 @@ def test_biases_past_float32():
         with pytest.raises(ValueError, match="float32"):
             m.generate_greedy([1, 2], 2, logit_bias={3: v})
     assert m.generate_greedy([1, 2], 2, logit_bias={3: float("inf")}) == [3, 3]
+
+
+def test_scratch_is_shared_and_counted():
+    """A model's layers share one scratch; a cache of its own has another."""
+    from alpacca_amd.kvcache import QuantKVCache
+    hp, tensors = tiny(n_layer=3)
+    kv8 = model(hp, tensors, kv_dtype="q8").kv8
+    assert len({c._scratch.data_ptr() for c in kv8}) == 1
+    for hd, mb in ((64, 18), (128, 35), (256, 68)):
+        a = QuantKVCache(2, 40, hd)
+        b = QuantKVCache(1, 70, hd, scratch=a)
+        assert a.scratch_nbytes() == b.scratch_nbytes() == 65536 * (hd + 4) * 4
+        assert round(a.scratch_nbytes() / 1e6) == mb
+        assert a.storage_nbytes() == 2 * (2 * 2 * 32 * hd + 2 * 2 * 4 + 2 * 32 * hd * 4 + 16)
+        assert a._scratch.data_ptr() == b._scratch.data_ptr() != QuantKVCache(
+            2, 40, hd)._scratch.data_ptr()
