@@ -829,7 +829,7 @@ __device__ __forceinline__ Ref joined(M m, R D) {
 constexpr int kWaves = 4;
 constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves + 1 : kWaves; }
 template <int HD, bool ROPE>
-__global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
+__global__ void __launch_bounds__(64 * split_waves(HD, ROPE), HD == 64 ? 3 : 1)
     k_kv8_split(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
                 int64_t T, int G, float f, float *__restrict__ part, float *__restrict__ out,
                 const float *__restrict__ kn, const float *__restrict__ vn, Rope rope) {
@@ -850,8 +850,8 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
   const bool live = id < rows;
   const int tok = live ? id / G : 0;
   const int g = live ? id - tok * G : 0;
-  const int64_t lim = sp.p0 + tok;              // the row's last position
-  const int64_t lim0 = sp.p0 + id0 / G;         // the tile's first row's
+  const int lim = (int)sp.p0 + tok;             // the row's last position
+  const int lim0 = (int)sp.p0 + id0 / G;        // the tile's first row's
   const int nb_all = (int)((sp.p0 + id_last / G) / kBlk) + 1;  // blocks the tile sees
   const int nb = ROPE ? nb_all - 1 : nb_all;                   // of them from memory
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk;
@@ -934,10 +934,10 @@ __global__ void __launch_bounds__(64 * split_waves(HD, ROPE))
     }
     h8 ph[1], pl[1];
     const float ks[1] = {x.ks}, vs[1] = {x.vs};
-    const int64_t first = (int64_t)blk * kBlk;
-    if (MASK && first + kBlk - 1 > lim0) {  // (uniform) some row ends inside it or before
-      const int64_t d = lim - first - 4 * cg;
-      const int last[1] = {(int)(d > 64 ? 64 : d < -1 ? -1 : d)};
+    const int first = blk * kBlk;  // (below n_ctx, and with it 2^31)
+    if (MASK && first > lim0 - (kBlk - 1)) {  // (uniform) some row ends inside it or before
+      const int d = lim - first - 4 * cg;
+      const int last[1] = {d > 64 ? 64 : d < -1 ? -1 : d};
       softmax_step<HD, 1, true>(s, sc, f, qr.back, ks, vs, last, ph, pl);
     } else {
       const int last[1] = {0};

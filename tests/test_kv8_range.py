@@ -247,3 +247,53 @@ def test_large_queries_and_small_keys(hd, n_kv, G, T, k_units, qs):
     if T == 1:
         got = cache.step(flat(q[pos:]), of_units(u[pos:].reshape(1, -1)), flat(v[pos:]), pos)
         within(got, want, tol)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("wide", [1e4, 1e7, 1e9, 1e10])
+def test_queries_of_a_wide_range(hd, T, wide):
+    """Two dimensions of the queries are large where every key is zero, so the
+    others make the scores.  The two fp16 pieces of a row scaled to a largest
+    value of 2^14 or more leave at most 2^-25 (half a unit of the second one),
+    2^-39 of the row's largest magnitude; a score is off by that times the sum
+    of its key's magnitudes, beside float32's own roundings."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(hd + T)
+    n, n_kv, G = 230, 2, 4
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    k[..., 3] = k[..., hd // 2 + 1] = 0
+    q[..., 3], q[..., hd // 2 + 1] = wide, -0.7 * wide
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    pos = n - T
+    K, V = values64(*coded(k)), values64(*coded(v))
+    want, tol = attention64(q[pos:].astype(np.float64), K, V, pos)
+    for t in range(T):
+        for h in range(n_kv * G):
+            most = np.abs(K[:pos + t + 1, h // G]).sum(1).max()
+            dz = 2.0 ** -39 * wide * most / math.sqrt(hd)
+            tol[t, h] += 2 * np.abs(V[:pos + t + 1, h // G]).max() * math.expm1(2 * dz)
+    within(cache.attend(flat(q[pos:]), pos), want, tol)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_scores_stay_finite_beside_products_past_float32(T):
+    """Where every key is zero in the one dimension that holds a query's
+    largest value, a block's scale times that value may pass float32: outputs
+    stay means of values."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(T)
+    n, n_kv, G, hd = 230, 2, 4, 64
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    k *= np.float32(1e30)
+    k[..., 3] = 0
+    q *= np.float32(1e-30)
+    q[..., 3] = 3e38
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    V = values64(*coded(v))
+    got = cache.attend(flat(q[n - T:]), n - T).cpu().numpy().reshape(T, n_kv, G, hd)
+    assert np.isfinite(got).all()
+    top = np.abs(V).max(0)[None, :, None] * (1 + 2.0 ** -20)
+    assert (np.abs(got) <= top).all()
