@@ -1447,25 +1447,31 @@ hipError_t launch_kv8_read(const aq_kv8 &c, int64_t start, int64_t n, float *k, 
 // at once: heads of 256 take more than half of a SIMD's per wave (and the tiles
 // 128 KB of LDS), so one; a second turn is then no faster than a second launch.
 constexpr int kv8_residents(int head_dim) { return head_dim == 256 ? 1 : 2; }
-// The split kernel: as many workgroups as 256 CUs hold (but one, at most one more
-// for heads up to 128), no more than give every wave a block of a full cache, nor
-// than the scratch holds.  more: workgroups per kv head beside them (the step's).
-// Heads of 256, 8 kv heads, 32767 positions: 32 splits 28.8 us, 64 33.4; 4 kv
-// heads: 64 splits 20.6, 128 27.2; the step of 8 kv heads: TODO.
+// The split kernel: as many workgroups as 256 CUs hold (rounded up to whole splits
+// where that is two each and there are no others), no more than give every wave a
+// block of a full cache, nor than the scratch holds.  more: workgroups per kv head
+// beside them (the step's), which would else leave some for a second turn: the step
+// of 32 / 8 heads of 128 at 32128 positions, 64 + 1 splits a kv head 27.8 us, 63 + 1
+// 23.6.  Heads of 256, 32767 positions, 8 kv heads: 32 splits 28.8, 64 33.4; 4 kv
+// heads: 64 splits 20.6, 128 27.2; the step, 8 kv heads: 31 + 1 31.4, 64 + 1 43.4.
 int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves, int more) {
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk, groups = c.n_kv * tiles;
+  const int64_t hold = 256 * kv8_residents(c.head_dim);
   int64_t S = (n_blocks + waves - 1) / waves;
-  const int64_t fill = kv8_residents(c.head_dim) == 1 ? (256 - more * c.n_kv) / groups
-                                                      : (kMaxSplits - 2 + groups) / groups;
+  int64_t fill = (hold - more * c.n_kv) / groups;
+  if (hold > 256 && !more) fill = (hold - 2 + groups) / groups;
   const int64_t room = kScratchRows / rows - 1;
   S = S < fill ? S : fill;
   S = S < room ? S : room;
   return (int)(S < 1 ? 1 : S);
 }
 // The tiles kernel: the smallest estimate.  A workgroup takes about head_dim / 96
-// us per chunk, two on a CU 1.3 times that, more in turn; the splits' states go
-// through memory once each way, in a launch of its own.  32/8 heads of 128: 256
-// tokens at 8000 172 us whole, 85 split; 64 of heads of 256 (groups of 2) at 1000 56, 27.
+// us per chunk, two on a CU 1.3 times that, where a CU holds two, else and beyond
+// in turn; the splits' states go through memory once each way, in a launch of its
+// own.  32/8 heads of 128: 256 tokens at 8000 172 us whole, 85 in four splits.
+// Heads of 256, groups of 4: 700 tokens of 5 kv heads at 3396 (220 workgroups) 162
+// whole, 166 in two; 512 of 4 at 3000 (128) 137, in two 84, in four 90; 256 (64)
+// 128, in four 50, in eight 62.
 int kv8_tile_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int cus) {
   const double chunks = (double)((c.n_ctx + 2 * kBlk - 1) / (2 * kBlk));
   const double beside = kv8_residents(c.head_dim) == 1 ? 1.0 : 0.65;
