@@ -823,19 +823,19 @@ __device__ __forceinline__ Ref joined(M m, R D) {
 // the tail and the token (k_kv8_store's codes, bit for bit), stores it and
 // attends to it from LDS, while the others go through the blocks before.  There
 // a wave executes its few thousand instructions alone on its SIMD, 2 ns each,
-// so four waves code the block while a fifth makes q's pieces: 32 / 8 heads of
-// 128 at 3800 positions 7.8 us (four waves 10.2; the store's launch alone 5),
-// 32 / 8 heads of 64 at 99 6.0 (6.4).  At 256 dimensions five waves spill: four.
+// so four waves code the block while a fifth makes q's pieces, as long as a CU
+// has one workgroup (several of five waves each load its SIMDs unevenly).  Whole
+// calls, five waves against four: 32 / 8 heads of 64 at 4094 positions 9.7 us
+// (10.0), at 32766 14.0 (13.0); of 128 at 4094 10.9 (11.4), at 8190 15.4 (12.9), at
+// 32766 23.9 (18.9).  At 256 dimensions five waves spill: four.
 constexpr int kWaves = 4;
-constexpr int split_waves(int hd, bool rope) { return rope && hd < 256 ? kWaves + 1 : kWaves; }
-template <int HD, bool ROPE>
-__global__ void __launch_bounds__(64 * split_waves(HD, ROPE), HD == 64 ? 3 : 1)
+template <int HD, bool ROPE, int NW>
+__global__ void __launch_bounds__(64 * NW, HD == 64 ? 3 : 1)
     k_kv8_split(const float *__restrict__ q, aq_kv8 c, const aq_decode_state *st, int64_t pos0,
                 int64_t T, int G, float f, float *__restrict__ part, float *__restrict__ out,
                 const float *__restrict__ kn, const float *__restrict__ vn, Rope rope) {
-  constexpr int NW = split_waves(HD, ROPE);
   constexpr int KJ = HD / 64, VJ = HD / 32, PS = HD + 4;
-  constexpr int PARTS = HD == 256 ? 2 : 1, VP = VJ / PARTS;  // the merge's LDS: at most 32 KB
+  constexpr int PARTS = HD == 256 ? 2 : 1, VP = VJ / PARTS;  // the merge's LDS: at most 40 KB
   __shared__ f4v os[NW][2 * VP][64];
   __shared__ float stat[NW][3][16];
   __shared__ uint4 own[ROPE ? 2 : 1][ROPE ? BlockTokens<HD>::UNITS : 1];  // the token's block
@@ -1451,8 +1451,8 @@ constexpr int kv8_residents(int head_dim) { return head_dim == 256 ? 1 : 2; }
 // where that is two each and there are no others), no more than give every wave a
 // block of a full cache, nor than the scratch holds.  more: workgroups per kv head
 // beside them (the step's), which would else leave some for a second turn: the step
-// of 32 / 8 heads of 128 at 32128 positions, 64 + 1 splits a kv head 27.8 us, 63 + 1
-// 23.6.  Heads of 256, 32767 positions, 8 kv heads: 32 splits 28.8, 64 33.4; 4 kv
+// of 32 / 8 heads of 128 at 32128 positions, 64 + 1 splits a kv head 20.3 us, 63 + 1
+// 17.8.  Heads of 256, 32767 positions, 8 kv heads: 32 splits 28.8, 64 33.4; 4 kv
 // heads: 64 splits 20.6, 128 27.2; the step, 8 kv heads: 31 + 1 31.4, 64 + 1 43.4.
 int kv8_splits(const aq_kv8 &c, int64_t tiles, int64_t rows, int waves, int more) {
   const int64_t n_blocks = (c.n_ctx + kBlk - 1) / kBlk, groups = c.n_kv * tiles;
@@ -1503,7 +1503,7 @@ hipError_t launch_attention_kv8(const float *q, const aq_kv8 &c, int64_t T, int 
     const int64_t tiles = (rows + 15) / 16;
     S = kv8_splits(c, tiles, T * n_head, kWaves, 0);
     AQ_HD(c.head_dim,
-          hipLaunchKernelGGL((k_kv8_split<HD, false>),
+          hipLaunchKernelGGL((k_kv8_split<HD, false, kWaves>),
                              dim3((unsigned)S, (unsigned)c.n_kv, (unsigned)tiles),
                              dim3(64 * kWaves), 0, s, q, c, st, pos0, T, G, f, c.scratch, out,
                              nullptr, nullptr, Rope{}))
@@ -1542,12 +1542,18 @@ hipError_t launch_attention_rope_kv8(const float *q, const float *k, const float
                                      float *out, hipStream_t s) {
   const float f = score_factor(c.head_dim);
   const int G = n_head / c.n_kv;
+  // five waves where a CU gets one workgroup
+  const bool five =
+      c.head_dim < 256 && (kv8_splits(c, 1, n_head, kWaves + 1, 1) + 1) * c.n_kv <= 256;
+  const int waves = five ? kWaves + 1 : kWaves, S = kv8_splits(c, 1, n_head, waves, 1) + 1;
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)S, (unsigned)c.n_kv, 1u), dim3(64 * waves), 0, s, q, c,
+                       st, pos0, (int64_t)1, G, f, c.scratch, out, k, v,
+                       Rope{cos_t, sin_t, n_rot, neox});
+  };
   AQ_HD(c.head_dim,
-        constexpr int NW = split_waves(HD, true);
-        const int S = kv8_splits(c, 1, n_head, NW, 1) + 1;
-        hipLaunchKernelGGL((k_kv8_split<HD, true>), dim3((unsigned)S, (unsigned)c.n_kv, 1u),
-                           dim3(64 * NW), 0, s, q, c, st, pos0, (int64_t)1, G, f,
-                           c.scratch, out, k, v, Rope{cos_t, sin_t, n_rot, neox});
+        if (five) go(k_kv8_split<HD, true, HD < 256 ? kWaves + 1 : kWaves>);
+        else go(k_kv8_split<HD, true, kWaves>);
         hipLaunchKernelGGL(k_kv8_combine<HD>, dim3((unsigned)G, (unsigned)c.n_kv), dim3(kWG), 0, s,
                            c.scratch, st, pos0, c.n_ctx, (int64_t)1, G, S, out))
   return hipGetLastError();
