@@ -814,8 +814,10 @@ __device__ __forceinline__ Ref joined(M m, R D) {
 //
 // Bound by the codes' bytes, for short caches by one wave's chain.  One token of
 // 32 / 8 heads of 128: 30000 positions 13.7 us (61 MB: 4.5 TB/s), 131072 42
-// (268 MB: 6.4); 32 / 8 heads of 64, 2176 positions 4.5; 5 tokens of 28 / 4
-// heads of 128 at 7001 12.4 (three tiles of rows, each reading the codes).
+// (268 MB: 6.4); 32 / 8 heads of 64, 2176 positions 4.4; 16 / 8 heads of 256, 3800
+// 7.7, 32766 24.6 (134 MB: 5.5); 5 tokens of 28 / 4 heads of 128 at 7001 12.9
+// (three tiles of rows, one or two blocks a wave, 3.2 MB of states beside 7.2 of
+// codes; which of these bounds it was not measured).
 //
 // ROPE: one token, whose q, k and v are not rotated yet.  Every workgroup
 // rotates its q rows in registers; one more workgroup per kv head (the first)
@@ -1207,8 +1209,9 @@ __global__ void __launch_bounds__(kWG)
 //
 // Bound by issue, matrix and vector instructions together (matrix cores busy 34 %
 // and 38 % of the time; each useful product is two, of two pieces).  2048 tokens of
-// 32 / 8 heads of 64 from the start 55 us (17.2 useful GFLOP: 0.31 PFLOP/s, 0.62
-// with both pieces); 777 of 32 / 8 heads of 128 behind 2901 127 us (0.33, 0.66).
+// 32 / 8 heads of 64 from the start 50-52 us a call in a row of calls, 55 traced
+// (17.2 useful GFLOP: 0.33 PFLOP/s, 0.66 with both pieces); 777 of 32 / 8 heads of
+// 128 behind 2901 113 us, 125 traced (0.37, 0.74).
 // Slower: two row tiles per wave (74 and 182 against 66 and 146 then), eight waves
 // (57 and 143), q's pieces from LDS, rescaling always (61 against 57).
 template <int HD>

@@ -4,7 +4,9 @@ A quarter of the fp32 cache's bytes (the reference keeps fp32,
 alpacca/model.py:368-371), and a scratch of 18, 35 or 68 MB (head_dim 64, 128,
 256) that a model's layers share.  Blocks of 32 positions of one kv head share a
 scale, K and V apart; attention has float32 accuracy over the coded values
-(include/alpacca_amd.h, aq_kv8, has the exact rules).
+(include/alpacca_amd.h, aq_kv8, has the exact rules).  A position's code depends
+on the later tokens of its block too, once they are stored: a prompt's row sees
+values coded with up to 31 tokens that come after it.
 
 * ``store(k, v, pos, cos, sin, neox, q)`` - rotate and code T tokens at
   positions ``pos`` ..; returns the rotated queries, if any were given
@@ -14,7 +16,8 @@ scale, K and V apart; attention has float32 accuracy over the coded values
 
 Inputs are float32 tensors on the cache's device (made contiguous where they
 are not); the calls only enqueue on that device's current stream.  Calls on one
-cache are ordered as its stores are: on one stream, or by events.
+cache, its construction among them, are ordered as its stores are: on one stream,
+or by events.
 ``alpacca_amd.model.Model(..., kv_dtype="q8")`` runs its layers on these.
 """
 from __future__ import annotations

@@ -218,9 +218,11 @@ class Model:
         # batched prefill: chunk size (ALPACCA_PREFILL_CHUNK, model.py:630-634)
         # and matmul precision (fp32: the reference's f32 products).  The
         # reference's 256 bounds host memory; here the chunk only sets how
-        # many rows each matmul_t launch gets (the results are bit-identical
-        # for every chunk size: a product's K order does not depend on M and
-        # attention merges fixed 64-position chunks), and 256-row launches
+        # many rows each matmul_t launch gets (over the fp32 cache the results
+        # are bit-identical for every chunk size: a product's K order does not
+        # depend on M and attention merges fixed 64-position chunks; over the
+        # 8-bit one a row also sees how its block's later tokens of the same
+        # chunk were coded), and 256-row launches
         # leave most CUs idle (1B model, 2048 tokens: 298 ms at 256, 70 ms
         # at 2048).
         import os
@@ -401,7 +403,9 @@ class Model:
         repeats the cached prefix reuses it as the reference does.  batch=True
         runs the suffix through the batched step (forward_batch, in chunks of
         prefill_chunk tokens); batch=False runs it through the decode step
-        one token at a time (the same function)."""
+        one token at a time: the same function over the fp32 cache.  Over the
+        8-bit cache a row of a chunk sees its block coded with the chunk's
+        later tokens as well, a single token with those up to its own."""
         if not tokens:
             return None
         if len(tokens) > self.n_ctx:

@@ -443,7 +443,10 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  * scale is s = fl32(amax / 127), a value x is coded as the whole number c
  * nearest to x / s (ties to even, at most 127 in magnitude; 0 where s is 0),
  * and stands for s c.  A block that holds an infinity or a NaN has a NaN scale
- * and reads as NaN.  The last block stored is also kept in fp32 (the tail), so a
+ * and reads as NaN.  (So a value's code depends on up to 31 later tokens of its
+ * block, once they are stored, and an infinity among them makes the whole block
+ * NaN for every query that attends to any of it.)
+ * The last block stored is also kept in fp32 (the tail), so a
  * token that joins it has it coded anew from the values themselves: the codes
  * do not depend on how many calls brought the tokens.  (A call that goes back
  * inside an earlier block takes what stays of it as its codes stand for it.)
@@ -479,8 +482,9 @@ int aq_kv8_sizes(int n_kv, int head_dim, int64_t n_ctx, size_t *codes, size_t *s
  * that starts inside a block continues it, and its positions before p0 must be
  * stored; going back drops what followed (exactly, as if it had never been,
  * inside the last block stored and to any block's first position).  Slots of
- * the last block past p0+T-1 are cleared, blocks after it left as they are.  AQ_ERR_VALUE when p0 + T > n_ctx (checked only for
- * a host position; the kernels skip positions past the cache).  Enqueues only. */
+ * the last block past p0+T-1 are cleared, blocks after it left as they are.
+ * AQ_ERR_VALUE when p0 + T > n_ctx (checked only for a host position; the kernels
+ * skip positions past the cache).  Enqueues only. */
 int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, int64_t T,
                 int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
                 const aq_decode_state *state, int64_t pos0, const aq_kv8 *cache, void *stream);
@@ -488,7 +492,13 @@ int aq_rope_kv8(const float *q, const float *k, const float *v, float *q_out, in
 /* Causal attention of T query tokens (q [T][n_head * head_dim], rotated) at
  * positions p0 .. p0+T-1, all stored, over the cache's values: token t attends
  * to positions 0 .. p0+t.  out [T][n_head * head_dim].  float32 accuracy over the
- * values the codes stand for.  Groups n_head / n_kv of 1 to 16; T up to 65535.
+ * values the codes stand for, for scores of any size that float32 holds: beside
+ * float32's own roundings of its products and sums a score is off by at most 2^-39
+ * of the query's largest magnitude times the sum of the key's magnitudes, and a
+ * weight times its block's V scale by at most 2^-37 of the row's largest such
+ * product.  The values are those of every
+ * token stored, also of a block's tokens after p0+t (see the scale above).  Groups
+ * n_head / n_kv of 1 to 16; T up to 65535.
  * A query with an infinity or a NaN gives NaN.  Enqueues only, and allocates
  * nothing. */
 int aq_attention_kv8(const float *q, const aq_kv8 *cache, int64_t T, int n_head,

@@ -297,3 +297,28 @@ def test_scores_stay_finite_beside_products_past_float32(T):
     assert np.isfinite(got).all()
     top = np.abs(V).max(0)[None, :, None] * (1 + 2.0 ** -20)
     assert (np.abs(got) <= top).all()
+
+
+@pytest.mark.parametrize("T", [1, 40, 90])
+@pytest.mark.parametrize("in_v", [False, True])
+def test_an_infinity_reaches_its_whole_block(T, in_v):
+    """Stored with the tokens of positions 64 .. 95, an infinity at 80 makes
+    every row from 64 on NaN, those before it too, and no row before 64."""
+    from alpacca_amd.kvcache import QuantKVCache
+    rng = np.random.default_rng(T)
+    n, n_kv, G, hd = 100, 2, 4, 64
+    q, k, v = inputs(rng, n, n_kv * G, n_kv, hd)
+    clean = values64(*coded(k)), values64(*coded(v))
+    (v if in_v else k)[80, 1, 9] = -np.inf
+    cache = QuantKVCache(n_kv, n, hd)
+    cache.store(flat(k), flat(v), 0)
+    for pos in sorted({0, 63 - T + 1 if T < 64 else 0, 64, n - T}):
+        if pos < 0 or pos + T > n:
+            continue
+        want, tol = attention64(q[pos:pos + T].astype(np.float64), *clean, pos)
+        got = cache.attend(flat(q[pos:pos + T]), pos).cpu().numpy().reshape(want.shape)
+        for t in range(T):
+            bad = slice(4, 8) if pos + t >= 64 else slice(8, 8)
+            assert np.isnan(got[t, bad]).all(), (pos, t)
+            good = got[t, :bad.start], want[t, :bad.start], tol[t, :bad.start]
+            assert (np.abs(good[0] - good[1]) <= good[2]).all(), (pos, t)
