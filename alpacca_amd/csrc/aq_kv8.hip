@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
 // Both kernels below work on tiles of 16 query rows of one kv head (row id =
 // token * G + head in the group, any G up to 16) with
 // v_mfma_f32_16x16x32_f16, the codes as exact fp16 operands and every fp32
-// operand in two fp16 pieces (x = hi + lo, 24 bits where lo is normal):
+// operand in two fp16 pieces (x = hi + lo, 23 bits where lo is normal):
 //   S^T (positions x rows) = C_K Q^T, Q's row scaled by a power of two to a
 //     largest value in [2^14, 2^15): lane l holds row l % 16's scores at
 //     positions 16 pt + 4 (l / 16) + r of a block (pt = 0, 1; r = 0 .. 3);
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kStoreWG<HD>)
 //     operand as it holds them (the V layout stores positions in that order).
 // The block's K scale enters as the factor of its raw scores, its V scale in
 // the weights: P = 2^(z - m) s_V, formed relative to the largest such product
-// the row has met, 2^D (of the same 2^m), so the pieces hold 24 bits of whatever
+// the row has met, 2^D (of the same 2^m), so the pieces hold 23 bits of whatever
 // counts and no magnitude of V over- or underflows them.  m and D are rounded up
 // to whole numbers, so every rescaling is an exact power of two; D stays a small
 // number however large the scores are.  The sum of 2^(z - m) is kept per lane.
