@@ -109,8 +109,8 @@ def test_few_tokens(hd, n_kv, G, n, T):
     compare(cache.attend(flat(q), n - T), want, tol)
 
 
-# the step's splits take what lies before the token's block: 1 to 3 blocks per
-# wave, and 40 / 314 splits of one kv head
+# the step's splits take what lies before the token's block: 63 of 8 kv heads (31 of
+# heads of 256), so 2 to 5 blocks per wave, and 40 / 391 of one kv head
 @pytest.mark.parametrize("hd,n_kv,G,n_ctx,at,n_rot,neox", [
     (64, 8, 4, 28001, (10240, 10271, 20500, 28000), 64, False),
     (128, 8, 4, 24001, (10250, 24000), 128, True), (256, 1, 2, 4999, (4100, 4998), 64, True),
