@@ -79,6 +79,14 @@ SIGNATURES = {
     "aq_attention_rope_kv8": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp,
                                      _vp, _vp]),
     "aq_kv8_read": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
+    "aq_sample": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "aq_paged_sizes": (_i32, [_vp, _c.POINTER(_sz)]),
+    "aq_rope_paged": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp,
+                             _i64, _i64, _vp, _vp, _i64, _vp, _vp]),
+    "aq_attention_paged": (_i32, [_vp, _vp, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _vp, _i64,
+                                  _i64, _vp, _sz, _vp, _vp]),
+    "aq_attention_paged_scratch": (_i32, [_vp, _i64, _i32, _i64, _i64, _c.POINTER(_sz)]),
+    "aq_paged_read": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
     "aq_stream_read": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _vp]),
 }
 
@@ -94,6 +102,13 @@ class KV8(ctypes.Structure):
                 ("v_tail", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
                 ("n_ctx", ctypes.c_int64), ("n_kv", ctypes.c_int32),
                 ("head_dim", ctypes.c_int32)]
+
+
+class Paged(ctypes.Structure):
+    """aq_paged: the arrays and the shape of one layer's paged KV cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("n_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 _lib = None

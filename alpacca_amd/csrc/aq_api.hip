@@ -1387,3 +1387,151 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
 }
 
 }  // extern "C"
+
+// ---- sampling ------------------------------------------------------------------------
+
+extern "C" {
+
+int aq_sample(const float *logits, int64_t rows, int64_t n, const double *u,
+              const double *params, int64_t params_ld, int64_t *out, float *logp, void *stream) {
+  if (rows < 0 || n < 0 || params_ld < 0) return fail(AQ_ERR_VALUE, "negative shape");
+  if (rows > 65535) return fail(AQ_ERR_VALUE, "at most 65535 rows per call");
+  if (n > INT32_MAX) return fail(AQ_ERR_VALUE, "too many logits");
+  if (params_ld && params_ld < 4)
+    return fail(AQ_ERR_VALUE, "a row's params are 4 numbers, not %lld", (long long)params_ld);
+  if (rows == 0) return AQ_OK;
+  if (n == 0) return fail(AQ_ERR_VALUE, "no logits to choose from");
+  if (!logits || !u || !params || !out) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  hipError_t e = aq::launch_sample(logits, rows, n, u, params, params_ld, out, logp,
+                                   static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "sampling launch");
+}
+
+}  // extern "C"
+
+// ---- paged 16-bit KV cache -------------------------------------------------------
+
+namespace {
+int paged_shape(const aq_paged *c) {
+  if (!c) return fail(AQ_ERR_VALUE, "cache is NULL");
+  if (c->n_kv <= 0 || c->n_kv > 65535 || c->n_pages <= 0 || c->n_pages > INT32_MAX)
+    return fail(AQ_ERR_VALUE, "bad cache shape (n_kv %d, n_pages %lld)", c->n_kv,
+                (long long)c->n_pages);
+  if (c->page_size <= 0 || c->page_size % 32 || c->page_size > 65536)
+    return fail(AQ_ERR_VALUE, "pages hold a multiple of 32 positions up to 65536 (got %d)",
+                c->page_size);
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(AQ_ERR_VALUE, "the paged cache takes head_dim 64, 128 or 256 (got %d)",
+                c->head_dim);
+  if (c->dtype != AQ_F16 && c->dtype != AQ_BF16)
+    return fail(AQ_ERR_VALUE, "the paged cache holds F16 or BF16 (got type %d)", c->dtype);
+  if (c->n_pages * c->page_size > ((int64_t)1 << 40) / c->n_kv)
+    return fail(AQ_ERR_VALUE, "the paged cache is too large");
+  return AQ_OK;
+}
+
+int paged_check(const aq_paged *c) {
+  if (int rc = paged_shape(c)) return rc;
+  if (!c->k || !c->v) return fail(AQ_ERR_VALUE, "NULL array in the cache");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16)
+    return fail(AQ_ERR_VALUE, "the cache's arrays must be 16-byte aligned");
+  return AQ_OK;
+}
+
+int paged_tokens(const aq_paged *c, int64_t N, const int32_t *table, int64_t seqs, int64_t width,
+                 const int64_t *pos, int64_t start) {
+  if (N < 0) return fail(AQ_ERR_VALUE, "negative token count");
+  if (N > ((int64_t)1 << 24)) return fail(AQ_ERR_VALUE, "%lld tokens are too many for one call",
+                                          (long long)N);
+  if (seqs < 0 || width < 0 || start < 0 || seqs > INT32_MAX || width > INT32_MAX)
+    return fail(AQ_ERR_VALUE, "bad table shape (%lld rows of %lld pages, start %lld)",
+                (long long)seqs, (long long)width, (long long)start);
+  if (N && (!pos || (seqs && width && !table))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  return AQ_OK;
+}
+
+int paged_attention_shape(const aq_paged *c, int64_t N, int n_head, int64_t width, int64_t start) {
+  if (int rc = paged_shape(c)) return rc;
+  if (n_head <= 0 || n_head % c->n_kv || n_head / c->n_kv > 16)
+    return fail(AQ_ERR_VALUE, "bad attention shape (n_head %d, n_kv %d): groups of 1 to 16",
+                n_head, c->n_kv);
+  if (N < 0 || N > ((int64_t)1 << 24) / n_head)
+    return fail(AQ_ERR_VALUE, "%lld query rows of %d heads are too many for one call",
+                (long long)N, n_head);
+  if (width < 0 || start < 0 || width > INT32_MAX || start > ((int64_t)1 << 40))
+    return fail(AQ_ERR_VALUE, "bad table width %lld or start %lld", (long long)width,
+                (long long)start);
+  return AQ_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int aq_paged_sizes(const aq_paged *cache, size_t *bytes) {
+  if (int rc = paged_shape(cache)) return rc;
+  if (bytes)
+    *bytes = (size_t)cache->n_pages * cache->page_size * cache->n_kv * cache->head_dim * 2;
+  return AQ_OK;
+}
+
+int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, int64_t N,
+                  int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
+                  int64_t n_pos, const int32_t *table, int64_t seqs, int64_t width,
+                  const int64_t *seq, const int64_t *pos, int64_t start, const aq_paged *cache,
+                  void *stream) {
+  if (int rc = paged_check(cache)) return rc;
+  if (int rc = paged_tokens(cache, N, table, seqs, width, pos, start)) return rc;
+  if (n_rot < 0 || n_rot > cache->head_dim || n_rot % 2)
+    return fail(AQ_ERR_VALUE, "n_rot %d must be even and <= head_dim %d", n_rot, cache->head_dim);
+  if (n_rot && (!cos_tab || !sin_tab || n_pos < 0)) return fail(AQ_ERR_VALUE, "NULL rotation table");
+  if (q && (n_head <= 0 || n_head > 65535)) return fail(AQ_ERR_VALUE, "bad n_head %d", n_head);
+  if (N && (!k || !v || (q && !q_out))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(q, k, v, q_out)) return rc;
+  if (N == 0) return AQ_OK;
+  hipError_t e = aq::launch_rope_paged(q, k, v, q_out, N, n_head, n_rot, neox ? 1 : 0, cos_tab,
+                                       sin_tab, n_pos, {table, seqs, width, seq, pos, start},
+                                       *cache, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache append launch");
+}
+
+int aq_attention_paged_scratch(const aq_paged *cache, int64_t N, int n_head, int64_t width,
+                               int64_t start, size_t *bytes) {
+  if (int rc = paged_attention_shape(cache, N, n_head, width, start)) return rc;
+  if (bytes) *bytes = 0;
+  return AQ_OK;
+}
+
+int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
+                       const int32_t *table, int64_t seqs, int64_t width, const int64_t *seq,
+                       const int64_t *pos, const int32_t *prefix, int64_t n_prefix,
+                       int64_t start, void *scratch, size_t scratch_bytes, float *out,
+                       void *stream) {
+  if (int rc = paged_check(cache)) return rc;
+  if (int rc = paged_tokens(cache, N, table, seqs, width, pos, start)) return rc;
+  if (int rc = paged_attention_shape(cache, N, n_head, width, start)) return rc;
+  if (n_prefix < 0 || n_prefix > INT32_MAX || start > n_prefix * cache->page_size)
+    return fail(AQ_ERR_VALUE, "a prefix of %lld pages of %d holds fewer than %lld positions",
+                (long long)n_prefix, cache->page_size, (long long)start);
+  if (N && (!q || !out || (start && !prefix))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(q, out, scratch, nullptr)) return rc;
+  if (N == 0) return AQ_OK;
+  hipError_t e = aq::launch_attention_paged(q, N, n_head, {table, seqs, width, seq, pos, start},
+                                            {prefix, 1, n_prefix, nullptr, nullptr, start}, *cache,
+                                            out, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache attention launch");
+}
+
+int aq_paged_read(const aq_paged *cache, int64_t N, const int32_t *table, int64_t seqs,
+                  int64_t width, const int64_t *seq, const int64_t *pos, int64_t start, void *k,
+                  void *v, void *stream) {
+  if (int rc = paged_check(cache)) return rc;
+  if (int rc = paged_tokens(cache, N, table, seqs, width, pos, start)) return rc;
+  if (N && (!k || !v)) return fail(AQ_ERR_VALUE, "NULL pointer argument");
+  if (int rc = kv8_aligned(k, v, nullptr, nullptr)) return rc;
+  if (N == 0) return AQ_OK;
+  hipError_t e = aq::launch_paged_read(N, {table, seqs, width, seq, pos, start}, *cache, k, v,
+                                       static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache read launch");
+}
+
+}  // extern "C"

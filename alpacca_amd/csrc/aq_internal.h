@@ -238,4 +238,28 @@ hipError_t launch_logits_adjust(const float *logits, int64_t rows, int64_t n,
                                 const int64_t *bias_off, int64_t n_bias, const uint32_t *mask,
                                 int64_t mask_ld, float *out, hipStream_t s);
 
+// One token for each row of logits (aq_sample.hip).
+hipError_t launch_sample(const float *logits, int64_t rows, int64_t n, const double *u,
+                         const double *params, int64_t params_ld, int64_t *out, float *logp,
+                         hipStream_t s);
+
+// Paged 16-bit KV cache (aq_paged.hip).  The places of a call's tokens: pos and
+// seq of each, and the table of pages whose slot 0 is position start.
+struct PagedTable {
+  const int32_t *pages;  // [seqs][width]
+  int64_t seqs, width;
+  const int64_t *seq, *pos;  // seq NULL: row i
+  int64_t start;
+};
+hipError_t launch_rope_paged(const float *q, const float *k, const float *v, float *q_out,
+                             int64_t N, int n_head, int n_rot, int neox, const float *cos_t,
+                             const float *sin_t, int64_t n_pos, const PagedTable &tab,
+                             const aq_paged &c, hipStream_t s);
+hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c, void *k, void *v,
+                             hipStream_t s);
+// pre: one row, the prefix's pages; its start is the prefix's length
+hipError_t launch_attention_paged(const float *q, int64_t N, int n_head, const PagedTable &tab,
+                                  const PagedTable &pre, const aq_paged &c, float *out,
+                                  hipStream_t s);
+
 }  // namespace aq

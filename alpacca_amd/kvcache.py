@@ -1,4 +1,7 @@
-"""QuantKVCache: the keys and values of one attention layer in 8 bits, in HBM.
+"""The KV caches of one attention layer beside the fp32 one, in HBM: in 8 bits
+(QuantKVCache) and, for many sequences, paged in 16 bits (PagedKVCache).
+
+QuantKVCache: the keys and values of one sequence in 8 bits.
 
 A quarter of the fp32 cache's bytes (the reference keeps fp32,
 alpacca/model.py:368-371), and a scratch of 18, 35 or 68 MB (head_dim 64, 128,
@@ -19,6 +22,16 @@ are not); the calls only enqueue on that device's current stream.  Calls on one
 cache, its construction among them, are ordered as its stores are: on one stream,
 or by events.
 ``alpacca_amd.model.Model(..., kv_dtype="q8")`` runs its layers on these.
+
+PagedKVCache: the keys and values of one layer for many sequences, in fp16 or
+bf16, in pages that the caller hands out (include/alpacca_amd.h, aq_paged, has the
+exact rules).  Sequences may share a prefix, which attention reads once for all.
+
+* ``append(k, v, table, pos, ...)`` - rotate tokens' queries and keys and put keys
+  and values into their pages
+* ``attend(q, table, pos, ..., prefix=pages, start=its length)`` - attention of a
+  query a row over the prefix and the row's own pages
+* ``read(table, pos, ...)`` - the values back, in the cache's type
 """
 from __future__ import annotations
 
@@ -40,7 +53,60 @@ def check_heads(n_head: int, n_kv: int, head_dim: int) -> None:
                          f"got {n_head} for {n_kv}")
 
 
-class QuantKVCache:
+class _Heads:
+    """What the caches' calls have in common: their arguments, rows of heads of
+    head_dim on the cache's device."""
+
+    def _rows(self, x, name: str, heads=None):
+        """x as a contiguous float32 [T, heads * head_dim] on the device."""
+        torch = self._torch
+        if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32:
+            raise ValueError(f"{name} must be a float32 tensor")
+        if x.device != self.device:
+            raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
+        dim = x.dim()
+        if dim == 1:
+            x = x.unsqueeze(0)
+        elif dim == 3:
+            if x.shape[2] != self.head_dim:
+                raise ValueError(f"{name} has shape {tuple(x.shape)}, head_dim is {self.head_dim}")
+            x = x.reshape(x.shape[0], x.shape[1] * x.shape[2])
+        elif dim != 2:
+            raise ValueError(f"{name} must be (T, heads * head_dim), got {tuple(x.shape)}")
+        if heads is not None and x.shape[1] != heads * self.head_dim:
+            raise ValueError(f"{name} has {x.shape[1]} values per token, expected "
+                             f"{heads} x {self.head_dim}")
+        x = x.contiguous()
+        return x if x.data_ptr() % 16 == 0 else x.clone()  # (the kernels load 16 bytes)
+
+    def _query_heads(self, q) -> int:
+        n, rem = divmod(q.shape[1], self.head_dim)
+        if rem or n == 0 or n % self.n_kv or n // self.n_kv > MAX_GROUP:
+            raise ValueError(f"q has {q.shape[1]} values per token: not a multiple of "
+                             f"{self.n_kv} kv heads x head_dim {self.head_dim} of at most "
+                             f"{MAX_GROUP} query heads each")
+        return n
+
+    def _call(self, fn, *args):
+        """fn(*args, stream) with the cache's device current."""
+        cuda = self._torch.cuda
+        if cuda.current_device() == self.device.index:
+            _lib.check(fn(*args, _lib.current_stream(self.device.index)))
+        else:
+            with cuda.device(self.device):
+                _lib.check(fn(*args, _lib.current_stream(self.device.index)))
+
+    def _out(self, out, q, qc):
+        if out is None:
+            out = self._torch.empty_like(qc)
+            return out if q.dim() == 2 else out.view(q.shape)
+        if (out.dtype != self._torch.float32 or out.numel() != qc.numel()
+                or out.device != self.device or not out.is_contiguous()):
+            raise ValueError("out must be a contiguous float32 tensor of q's size")
+        return out
+
+
+class QuantKVCache(_Heads):
     """n_ctx positions of n_kv heads of head_dim, on `device` (default: the
     current one).  ValueError for an unsupported shape.  `scratch`: another
     cache whose scratch this one shares (same head_dim and device), for caches
@@ -102,36 +168,6 @@ class QuantKVCache:
 
     # ---- arguments -----------------------------------------------------------
 
-    def _rows(self, x, name: str, heads=None):
-        """x as a contiguous float32 [T, heads * head_dim] on the device."""
-        torch = self._torch
-        if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32:
-            raise ValueError(f"{name} must be a float32 tensor")
-        if x.device != self.device:
-            raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
-        dim = x.dim()
-        if dim == 1:
-            x = x.unsqueeze(0)
-        elif dim == 3:
-            if x.shape[2] != self.head_dim:
-                raise ValueError(f"{name} has shape {tuple(x.shape)}, head_dim is {self.head_dim}")
-            x = x.reshape(x.shape[0], x.shape[1] * x.shape[2])
-        elif dim != 2:
-            raise ValueError(f"{name} must be (T, heads * head_dim), got {tuple(x.shape)}")
-        if heads is not None and x.shape[1] != heads * self.head_dim:
-            raise ValueError(f"{name} has {x.shape[1]} values per token, expected "
-                             f"{heads} x {self.head_dim}")
-        x = x.contiguous()
-        return x if x.data_ptr() % 16 == 0 else x.clone()  # (the kernels load 16 bytes)
-
-    def _query_heads(self, q) -> int:
-        n, rem = divmod(q.shape[1], self.head_dim)
-        if rem or n == 0 or n % self.n_kv or n // self.n_kv > MAX_GROUP:
-            raise ValueError(f"q has {q.shape[1]} values per token: not a multiple of "
-                             f"{self.n_kv} kv heads x head_dim {self.head_dim} of at most "
-                             f"{MAX_GROUP} query heads each")
-        return n
-
     def _tables(self, cos, sin, last: int):
         """n_rot and the tables' pointers; `last`: rows the call reads."""
         if cos is None and sin is None:
@@ -157,15 +193,6 @@ class QuantKVCache:
             return
         if pos > self.length:
             raise ValueError(f"position {pos} leaves a gap after the {self.length} stored")
-
-    def _call(self, fn, *args):
-        """fn(*args, stream) with the cache's device current."""
-        cuda = self._torch.cuda
-        if cuda.current_device() == self.device.index:
-            _lib.check(fn(*args, _lib.current_stream(self.device.index)))
-        else:
-            with cuda.device(self.device):
-                _lib.check(fn(*args, _lib.current_stream(self.device.index)))
 
     # ---- operators -----------------------------------------------------------
 
@@ -236,15 +263,6 @@ class QuantKVCache:
         self.length = pos + 1
         return out
 
-    def _out(self, out, q, qc):
-        if out is None:
-            out = self._torch.empty_like(qc)
-            return out if q.dim() == 2 else out.view(q.shape)
-        if (out.dtype != self._torch.float32 or out.numel() != qc.numel()
-                or out.device != self.device or not out.is_contiguous()):
-            raise ValueError("out must be a contiguous float32 tensor of q's size")
-        return out
-
     def read(self, start: int = 0, stop: int | None = None):
         """The values of positions start .. stop - 1 (default: all stored) as
         two float32 tensors (n_kv, stop - start, head_dim)."""
@@ -261,4 +279,173 @@ class QuantKVCache:
         return kv.unbind()
 
 
-__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "QuantKVCache", "check_heads"]
+class PagedKVCache(_Heads):
+    """n_pages pages of page_size (a multiple of 32) positions of n_kv heads of
+    head_dim in dtype (torch.float16 or torch.bfloat16), on `device` (default: the
+    current one).  ValueError for an unsupported shape.
+
+    Which pages a sequence has is the caller's: a call's ``table`` (seqs, width),
+    int32, holds a row of page numbers for each sequence, in the order of its
+    positions.  Where sequences share a prefix, its positions 0 .. start - 1 lie in
+    pages of its own and a row's first page begins with position ``start``.  Token i
+    of a call is at position pos[i] (int64) of row seq[i] (int64; None: row i).
+    A token without a place (a position below 0 or below start, a row, page or
+    page number out of range) is left out, as padding is: nothing is stored for it.
+
+    The calls only enqueue on the device's current stream; those on one cache, its
+    construction among them, are ordered by the caller."""
+
+    def __init__(self, n_kv: int, n_pages: int, head_dim: int, page_size: int = 64, dtype=None,
+                 device=None):
+        import torch
+        dtype = torch.float16 if dtype is None else dtype
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"the paged cache holds float16 or bfloat16, not {dtype}")
+        name = "F16" if dtype == torch.float16 else "BF16"
+        self._c = _lib.Paged(None, None, n_pages, page_size, n_kv, head_dim,
+                             _lib.DTYPE_IDS[name])
+        self._ref = ctypes.addressof(self._c)
+        size = ctypes.c_size_t()
+        _lib.check(_lib.load().aq_paged_sizes(self._ref, ctypes.byref(size)))
+        self._lib = _lib.ensure_device()
+        self._torch = torch
+        self.device = torch.device("cuda" if device is None else device)
+        if self.device.type != "cuda":
+            raise ValueError(f"the cache lives on a GPU, not {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.n_kv, self.n_pages, self.head_dim = n_kv, n_pages, head_dim
+        self.page_size, self.dtype = page_size, dtype
+        self.k, self.v = (torch.zeros(size.value // 2, dtype=dtype, device=self.device)
+                          for _ in range(2))
+        self._c.k, self._c.v = self.k.data_ptr(), self.v.data_ptr()
+
+    @property
+    def handle(self) -> int:
+        """The aq_paged* of the C ABI (for device-resident callers)."""
+        return self._ref
+
+    def storage_nbytes(self) -> int:
+        """Bytes of HBM that hold the pages."""
+        return 2 * (self.k.numel() + self.v.numel())
+
+    # ---- arguments -----------------------------------------------------------
+
+    def _index(self, x, name: str, dtype, dim: int):
+        """x as a contiguous tensor of dtype on the device."""
+        if (not isinstance(x, self._torch.Tensor) or x.dtype != dtype or x.dim() != dim
+                or x.device != self.device):
+            have = (f"{x.dtype} {tuple(x.shape)} on {x.device}"
+                    if isinstance(x, self._torch.Tensor) else type(x).__name__)
+            raise ValueError(f"{name} must be {dtype} of {dim} dimension(s) on {self.device}, "
+                             f"got {have}")
+        return x.contiguous()
+
+    def _places(self, table, pos, seq, start: int, n=None):
+        """The checked descriptors of a call's tokens (kept alive by the caller)
+        and their C arguments but start."""
+        i64 = self._torch.int64
+        table = self._index(table, "table", self._torch.int32, 2)
+        pos = self._index(pos, "pos", i64, 1)
+        if n is not None and pos.shape[0] != n:
+            raise ValueError(f"{n} tokens, but pos has {pos.shape[0]}")
+        if seq is not None:
+            seq = self._index(seq, "seq", i64, 1)
+            if seq.shape != pos.shape:
+                raise ValueError(f"seq has {seq.shape[0]} tokens, pos {pos.shape[0]}")
+        if start < 0:
+            raise ValueError(f"start {start} is below 0")
+        return (table, pos, seq), (table.data_ptr(), table.shape[0], table.shape[1],
+                                   None if seq is None else seq.data_ptr(), pos.data_ptr())
+
+    # ---- operators -----------------------------------------------------------
+
+    def append(self, k, v, table, pos, seq=None, start: int = 0, cos=None, sin=None,
+               neox: bool = False, q=None, q_out=None):
+        """Put the N tokens k, v (N, n_kv * head_dim) into their places, k rotated
+        by cos / sin (positions, n_rot / 2; None: as it is), and rotate q
+        (N, n_head * head_dim) into q_out (default: a new tensor; may be q), which
+        is returned.  A token whose position is below 0 or past the tables is left
+        out, its row of q_out as it was (a new tensor's: undefined).  Two tokens in one place leave it undefined
+        whose values it holds."""
+        torch = self._torch
+        k, v = self._rows(k, "k", self.n_kv), self._rows(v, "v", self.n_kv)
+        N = k.shape[0]
+        if v.shape[0] != N:
+            raise ValueError(f"k has {N} tokens, v {v.shape[0]}")
+        keep, place = self._places(table, pos, seq, start, N)
+        n_head, qp, op = 1, None, None
+        if q is not None:
+            shape = q.shape
+            q = self._rows(q, "q")
+            n_head = self._query_heads(q)
+            if q.shape[0] != N:
+                raise ValueError(f"k has {N} tokens, q {q.shape[0]}")
+            if q_out is None:
+                q_out = torch.empty_like(q)
+                if len(shape) != 2:
+                    q_out = q_out.view(shape)
+            elif (q_out.dtype != torch.float32 or q_out.numel() != q.numel()
+                  or q_out.device != self.device or not q_out.is_contiguous()):
+                raise ValueError("q_out must be a contiguous float32 tensor of q's size")
+            qp, op = q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        n_rot, cp, sp, n_pos = 0, None, None, 0
+        if cos is not None or sin is not None:
+            for x, name in ((cos, "cos"), (sin, "sin")):
+                if (not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.dim() != 2
+                        or x.device != self.device or not x.is_contiguous()):
+                    raise ValueError(f"{name} must be a contiguous float32 (positions, "
+                                     f"n_rot / 2) tensor on {self.device}")
+            if cos.shape != sin.shape:
+                raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must agree")
+            n_rot, n_pos = 2 * cos.shape[1], cos.shape[0]
+            cp, sp = cos.data_ptr(), sin.data_ptr()
+        if N:
+            self._call(self._lib.aq_rope_paged, qp, k.data_ptr(), v.data_ptr(), op, N, n_head,
+                       n_rot, 1 if neox else 0, cp, sp, n_pos, *place, start, self._ref)
+        return q_out
+
+    def attend(self, q, table, pos, seq=None, start: int = 0, prefix=None, out=None):
+        """Attention of the query rows q (N, n_head * head_dim, rotated), row i over
+        positions 0 .. pos[i] of its sequence: those below `start` in the pages
+        `prefix` (int32, all rows share them), the others in its row of the table; as
+        q.  A row whose position is below 0, or that has no place to attend to,
+        gives 0."""
+        torch = self._torch
+        qc = self._rows(q, "q")
+        n_head, N = self._query_heads(qc), qc.shape[0]
+        keep, place = self._places(table, pos, seq, start, N)
+        pp, n_prefix = None, 0
+        if prefix is not None:
+            prefix = self._index(prefix, "prefix", torch.int32, 1)
+            pp, n_prefix = prefix.data_ptr(), prefix.shape[0]
+        if start > n_prefix * self.page_size:
+            raise ValueError(f"a prefix of {n_prefix} pages of {self.page_size} holds fewer than "
+                             f"{start} positions")
+        out = self._out(out, q, qc)
+        if N:
+            size = ctypes.c_size_t()
+            _lib.check(self._lib.aq_attention_paged_scratch(self._ref, N, n_head, place[2], start,
+                                                            ctypes.byref(size)))
+            # of this call alone: calls on other streams, and graphs, have their own
+            scratch = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+            self._call(self._lib.aq_attention_paged, qc.data_ptr(), self._ref, N, n_head, *place,
+                       pp, n_prefix, start, scratch.data_ptr(), size.value, out.data_ptr())
+        return out
+
+    def read(self, table, pos, seq=None, start: int = 0):
+        """The values that the tokens' places hold, as two tensors (N, n_kv *
+        head_dim) of the cache's type; 0 for a token without a place."""
+        torch = self._torch
+        keep, place = self._places(table, pos, seq, start)
+        N, width = pos.shape[0], self.n_kv * self.head_dim
+        k, v = (torch.empty((N, width), dtype=self.dtype, device=self.device) for _ in range(2))
+        if N:
+            self._call(self._lib.aq_paged_read, self._ref, N, *place, start, k.data_ptr(),
+                       v.data_ptr())
+        return k, v
+
+
+__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "PagedKVCache", "QuantKVCache", "check_heads"]

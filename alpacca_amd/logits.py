@@ -1,9 +1,13 @@
-"""Adjustment of logits before a token is chosen: penalties for tokens already
-said, per-token biases and a grammar's mask, for the rows of a batch in one
-launch (include/alpacca_amd.h, aq_logits_adjust, has the exact rules).  The
-repetition penalty is the reference sampler's (alpacca/sample.py:36-45).
+"""From a batch's logits to its tokens (include/alpacca_amd.h, aq_logits_adjust
+and aq_sample, has the exact rules).
 
-``Model.generate_greedy`` runs it between the head and the choice of the token.
+* ``adjust_logits`` - penalties for tokens already said, per-token biases and a
+  grammar's mask, for the rows of a batch in one launch.  The repetition penalty is
+  the reference sampler's (alpacca/sample.py:36-45).  ``Model.generate_greedy``
+  runs it between the head and the choice of the token.
+* ``sample_logits`` - a token for each row with temperature, top-k, top-p and
+  min-p, from given random numbers (alpacca/sample.py:44-76); the settings from
+  ``sampling_params``.
 """
 from __future__ import annotations
 
@@ -97,13 +101,83 @@ def adjust_logits(logits, *, window=None, penalties=None, bias=None, mask=None, 
         return None if t is None else t.data_ptr()
     args = (x.data_ptr(), rows, n, p(window), last_n, p(penalties), p(ids), p(val), p(off), n_bias,
             p(mask), mask_ld, out.data_ptr())
-    fn, index = _lib.ensure_device().aq_logits_adjust, dev.index
-    if torch.cuda.current_device() == index:
-        _lib.check(fn(*args, _lib.current_stream(index)))
-    else:
-        with torch.cuda.device(dev):
-            _lib.check(fn(*args, _lib.current_stream(index)))
+    _call(_lib.ensure_device().aq_logits_adjust, dev, args)
     return out
 
 
-__all__ = ["adjust_logits", "pack_mask"]
+def _call(fn, dev, args):
+    """fn(*args, stream) with `dev` current."""
+    import torch
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(fn(*args, _lib.current_stream(dev.index)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, _lib.current_stream(dev.index)))
+
+
+def sampling_params(rows=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, device=None):
+    """The settings of sample_logits as float64 (rows, 4), or (4,) for every
+    row (rows None): each a number, or one for each row.
+
+    temperature  0 (or less): the largest logit's token
+    top_k        how many tokens are kept (0: all)
+    top_p        the share of the weights that is kept (1: all)
+    min_p        the least weight that is kept, the largest counting 1 (0: all)"""
+    import torch
+    cols = []
+    for x, name in ((temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"),
+                    (min_p, "min_p")):
+        x = torch.as_tensor(x, dtype=torch.float64).cpu()
+        if x.dim() > 1 or (x.dim() == 1 and x.shape != (rows,)):
+            raise ValueError(f"{name} must be a number or {rows} of them, got {tuple(x.shape)}")
+        if bool(torch.isnan(x).any()):
+            raise ValueError(f"{name} must not be NaN")
+        if name != "temperature" and bool((x < 0).any()):
+            raise ValueError(f"{name} must not be negative")
+        cols.append(x if rows is None else x.expand(rows))
+    return torch.stack(cols, dim=-1).to("cuda" if device is None else device)
+
+
+def sample_logits(logits, u, params, *, out=None, logp=False):
+    """A token for each row of the logits (n,) or (rows, n), float32 on the GPU,
+    as int64 () or (rows,) (`out`: where; default: a new tensor); -1 where every
+    logit is -inf or NaN.  Everything else on the same device:
+
+    u       float64 () or (rows,): a random number in [0, 1) for each row
+    params  float64 (4,) for every row, or (rows, 4): temperature, top_k, top_p,
+            min_p (sampling_params)
+
+    The tokens in descending order of their logits (of equal ones the lowest
+    first) weigh exp((x - max) / temperature).  top_k keeps the first k, top_p the
+    shortest beginning that holds that share of those, min_p those of at least that
+    weight; the token is the first whose running sum exceeds u times the sum of
+    all kept.  logp=True: (tokens, the logarithms of their shares of that sum,
+    float32)."""
+    import torch
+    f64 = torch.float64
+    if not isinstance(logits, torch.Tensor) or logits.dtype != torch.float32 or \
+            logits.dim() not in (1, 2):
+        raise ValueError("logits must be a float32 tensor (n,) or (rows, n)")
+    if not logits.is_cuda:
+        raise ValueError("logits must be on a GPU")
+    if logits.shape[-1] == 0:
+        raise ValueError("no logits to choose from")
+    dev, lead = logits.device, logits.shape[:-1]
+    rows = lead[0] if lead else 1
+    u = _tensor(u, "u", f64, lead, dev)
+    per_row = isinstance(params, torch.Tensor) and params.dim() == 2
+    params = _tensor(params, "params", f64, (rows, 4) if per_row else (4,), dev)
+    if out is None:
+        out = torch.empty(lead, dtype=torch.int64, device=dev)
+    elif not (isinstance(out, torch.Tensor) and out.dtype == torch.int64 and out.shape == lead
+              and out.device == dev and out.is_contiguous()):
+        raise ValueError("out must be a contiguous int64 tensor, one number a row")
+    x = logits.contiguous()
+    lp = torch.empty(lead, dtype=torch.float32, device=dev) if logp else None
+    _call(_lib.ensure_device().aq_sample, dev,
+          (x.data_ptr(), rows, x.shape[-1], u.data_ptr(), params.data_ptr(), 4 if per_row else 0,
+           out.data_ptr(), lp.data_ptr() if logp else None))
+    return (out, lp) if logp else out
+
+
+__all__ = ["adjust_logits", "pack_mask", "sample_logits", "sampling_params"]

@@ -434,6 +434,30 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
                      const float *bias, const int64_t *bias_off, int64_t n_bias,
                      const uint32_t *mask, int64_t mask_ld, float *out, void *stream);
 
+/* One token for each of `rows` rows of n logits (row-major), drawn with the given
+ * random numbers.  A row's tokens are ordered by logit, of equal ones the lowest
+ * token first (a NaN counts as -infinity, and a logit of -infinity is not in the
+ * order), and weigh w = exp((x - max) / temperature).  Of that order a row keeps
+ * the shortest of three beginnings, always its first token:
+ *   top_k tokens (below 1, or at least n: all; a fraction is dropped);
+ *   those up to the first where the sum of w reaches top_p times the sum of the
+ *     top_k (top_p of 1 or more: all);
+ *   those of w >= min_p (0 or less: all);
+ * and the token is the first whose running sum exceeds u times the sum of all kept.
+ * temperature 0 or less: the first token of the order.  Weights are formed in double
+ * and added as whole multiples of 2^-e of the largest, e = 62 - (bits of n), so the
+ * token is a function of the row alone.  (A token that weighs less than 2^-(e + 1)
+ * of the largest is never drawn.)
+ * u [rows] (below 0 or NaN: 0; 1 and more: the largest number below 1); params: row
+ * r's temperature, top_k, top_p, min_p at params + r * params_ld (params_ld 0: the
+ * same for every row; NaN: as if left out, for the temperature 0).  out [rows]: the
+ * token, -1 where every logit is -infinity; logp [rows] or NULL: the logarithm of
+ * its w over the sum of all kept (0 at temperature 0 or less, -infinity for -1).
+ * Device pointers; enqueue only.  n up to 2^31 - 1.  Replaces Sampler.sample past
+ * its repeat penalty (alpacca/sample.py:44-76). */
+int aq_sample(const float *logits, int64_t rows, int64_t n, const double *u,
+              const double *params, int64_t params_ld, int64_t *out, float *logp, void *stream);
+
 /* ==== 8-bit KV cache =====================================================
  *
  * The cache of one layer with keys and values in int8, a quarter of the fp32
@@ -516,6 +540,73 @@ int aq_attention_rope_kv8(const float *q, const float *k, const float *v, int n_
 /* k, v [n_kv][n][head_dim] fp32: the values of positions start .. start+n-1
  * (s c, rounded to fp32).  Enqueues only. */
 int aq_kv8_read(const aq_kv8 *cache, int64_t start, int64_t n, float *k, float *v, void *stream);
+
+/* ==== paged 16-bit KV cache ===============================================
+ *
+ * The keys and values of one layer for many sequences in fp16 or bf16 (no
+ * counterpart in the reference, whose cache holds one sequence in fp32,
+ * model.py:368-371).  Pages of page_size positions of all kv heads; a sequence's
+ * pages are a row of a table of page numbers, in the order of its positions.
+ * Sequences may share a prefix: positions 0 .. start - 1 of all of them then lie
+ * in the pages of one list, and a row's first page begins with position start.
+ *
+ * The tokens of a call: token i of N is at position pos[i] (int64) of the sequence
+ * in row seq[i] (int64; seq NULL: row i) of table [seqs][width] (int32).  Position
+ * p >= start is slot p - start of the row.  A token has no place where its position
+ * is below 0 or below start, its row or slot is outside the table, or its page's
+ * number is not one of the pool's: nothing is stored for it.  Such tokens and pages
+ * are no errors (a padded batch has them).  Two tokens of one call in one place
+ * leave it undefined which one's values it holds, value by value.
+ *
+ * The caller allocates k and v (aq_paged_sizes; device memory, 16-byte aligned, no
+ * initial content needed).  Calls on one cache are the caller's to order.  q, k, v
+ * and outputs are 16-byte aligned too (AQ_ERR_VALUE).  head_dim 64, 128 or 256,
+ * page_size a multiple of 32. */
+typedef struct aq_paged {
+  void *k, *v;      /* [n_pages][n_kv][page_size / 32][32 * head_dim] (aq_paged.hip) */
+  int64_t n_pages;
+  int32_t page_size, n_kv, head_dim, dtype; /* AQ_F16 or AQ_BF16              */
+} aq_paged;
+
+/* Bytes of each of a cache's two arrays (its pointers are not read).  Host only. */
+int aq_paged_sizes(const aq_paged *cache, size_t *bytes);
+
+/* Rotation of N tokens' queries and keys at their positions, as aq_rope_kv rotates
+ * them, bit for bit (cos_tab, sin_tab [n_pos][n_rot / 2]; n_rot 0: none), q [N]
+ * [n_head * head_dim] into q_out (which may be q; q NULL: no queries), and the keys
+ * and values [N][n_kv * head_dim], rounded to the cache's type (to nearest, ties to
+ * even; past fp16's range: infinity), into their places.  A token whose position is
+ * below 0 or (with n_rot) not below n_pos is left out altogether, its row of q_out
+ * as it was; one that has no place otherwise has its query rotated.  Enqueues only. */
+int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, int64_t N,
+                  int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
+                  int64_t n_pos, const int32_t *table, int64_t seqs, int64_t width,
+                  const int64_t *seq, const int64_t *pos, int64_t start, const aq_paged *cache,
+                  void *stream);
+
+/* Attention of N query rows (q [N][n_head * head_dim], rotated): row i attends to
+ * positions 0 .. pos[i] of its sequence, those below start in the pages
+ * prefix [n_prefix] (start <= n_prefix * page_size), the others in its row of the
+ * table.  Positions without a place are left out; a row that has none, or whose
+ * position is below 0, gives 0.  out [N][n_head * head_dim].  Groups n_head / n_kv of
+ * 1 to 16; N * n_head up to 2^24.  Float32 accuracy over the values stored.
+ * scratch: at least the bytes that aq_attention_paged_scratch says for the same
+ * call, 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
+int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
+                       const int32_t *table, int64_t seqs, int64_t width, const int64_t *seq,
+                       const int64_t *pos, const int32_t *prefix, int64_t n_prefix,
+                       int64_t start, void *scratch, size_t scratch_bytes, float *out,
+                       void *stream);
+
+/* Scratch bytes of that call.  Host only; AQ_ERR_VALUE for an unsupported shape. */
+int aq_attention_paged_scratch(const aq_paged *cache, int64_t N, int n_head, int64_t width,
+                               int64_t start, size_t *bytes);
+
+/* k, v [N][n_kv * head_dim] in the cache's type: the values that N tokens' places
+ * hold; 0 where a token has none.  Enqueues only. */
+int aq_paged_read(const aq_paged *cache, int64_t N, const int32_t *table, int64_t seqs,
+                  int64_t width, const int64_t *seq, const int64_t *pos, int64_t start, void *k,
+                  void *v, void *stream);
 
 /* ==== calibration ========================================================
  *
