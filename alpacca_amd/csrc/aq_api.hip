@@ -1497,7 +1497,7 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
 int aq_attention_paged_scratch(const aq_paged *cache, int64_t N, int n_head, int64_t width,
                                int64_t start, size_t *bytes) {
   if (int rc = paged_attention_shape(cache, N, n_head, width, start)) return rc;
-  if (bytes) *bytes = 0;
+  if (bytes) *bytes = aq::attention_paged_scratch(*cache, N, n_head, width, start);
   return AQ_OK;
 }
 
@@ -1515,9 +1515,14 @@ int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_h
   if (N && (!q || !out || (start && !prefix))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
   if (int rc = kv8_aligned(q, out, scratch, nullptr)) return rc;
   if (N == 0) return AQ_OK;
+  const size_t need = aq::attention_paged_scratch(*cache, N, n_head, width, start);
+  if (need && (!scratch || scratch_bytes < need))
+    return fail(AQ_ERR_VALUE, "the attention needs %zu bytes of scratch, not %zu", need,
+                scratch ? scratch_bytes : (size_t)0);
   hipError_t e = aq::launch_attention_paged(q, N, n_head, {table, seqs, width, seq, pos, start},
                                             {prefix, 1, n_prefix, nullptr, nullptr, start}, *cache,
-                                            out, static_cast<hipStream_t>(stream));
+                                            static_cast<float *>(scratch), out,
+                                            static_cast<hipStream_t>(stream));
   return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache attention launch");
 }
 

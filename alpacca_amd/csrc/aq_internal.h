@@ -258,8 +258,10 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
 hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c, void *k, void *v,
                              hipStream_t s);
 // pre: one row, the prefix's pages; its start is the prefix's length
+size_t attention_paged_scratch(const aq_paged &c, int64_t N, int n_head, int64_t width,
+                               int64_t start);
 hipError_t launch_attention_paged(const float *q, int64_t N, int n_head, const PagedTable &tab,
-                                  const PagedTable &pre, const aq_paged &c, float *out,
-                                  hipStream_t s);
+                                  const PagedTable &pre, const aq_paged &c, float *states,
+                                  float *out, hipStream_t s);
 
 }  // namespace aq
