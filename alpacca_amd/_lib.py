@@ -79,7 +79,8 @@ SIGNATURES = {
     "aq_attention_rope_kv8": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp,
                                      _vp, _vp]),
     "aq_kv8_read": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp]),
-    "aq_sample": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "aq_sample": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _sz, _vp, _vp, _vp]),
+    "aq_sample_scratch": (_i32, [_i64, _i64, _c.POINTER(_sz)]),
     "aq_paged_sizes": (_i32, [_vp, _c.POINTER(_sz)]),
     "aq_rope_paged": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp,
                              _i64, _i64, _vp, _vp, _i64, _vp, _vp]),

@@ -1390,19 +1390,36 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
 
 // ---- sampling ------------------------------------------------------------------------
 
-extern "C" {
-
-int aq_sample(const float *logits, int64_t rows, int64_t n, const double *u,
-              const double *params, int64_t params_ld, int64_t *out, float *logp, void *stream) {
-  if (rows < 0 || n < 0 || params_ld < 0) return fail(AQ_ERR_VALUE, "negative shape");
+namespace {
+int sample_shape(int64_t rows, int64_t n) {
+  if (rows < 0 || n < 0) return fail(AQ_ERR_VALUE, "negative shape");
   if (rows > 65535) return fail(AQ_ERR_VALUE, "at most 65535 rows per call");
   if (n > INT32_MAX) return fail(AQ_ERR_VALUE, "too many logits");
-  if (params_ld && params_ld < 4)
+  if (rows && n == 0) return fail(AQ_ERR_VALUE, "no logits to choose from");
+  return AQ_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int aq_sample_scratch(int64_t rows, int64_t n, size_t *bytes) {
+  if (int rc = sample_shape(rows, n)) return rc;
+  if (bytes) *bytes = rows ? aq::sample_scratch(rows, n) : 0;
+  return AQ_OK;
+}
+
+int aq_sample(const float *logits, int64_t rows, int64_t n, const double *u,
+              const double *params, int64_t params_ld, void *scratch, size_t scratch_bytes,
+              int64_t *out, float *logp, void *stream) {
+  if (int rc = sample_shape(rows, n)) return rc;
+  if (params_ld < 0 || (params_ld && params_ld < 4))
     return fail(AQ_ERR_VALUE, "a row's params are 4 numbers, not %lld", (long long)params_ld);
   if (rows == 0) return AQ_OK;
-  if (n == 0) return fail(AQ_ERR_VALUE, "no logits to choose from");
   if (!logits || !u || !params || !out) return fail(AQ_ERR_VALUE, "NULL pointer argument");
-  hipError_t e = aq::launch_sample(logits, rows, n, u, params, params_ld, out, logp,
+  const size_t need = aq::sample_scratch(rows, n);
+  if (!scratch || scratch_bytes < need || (uintptr_t)scratch % 8)
+    return fail(AQ_ERR_VALUE, "sampling needs %zu bytes of scratch, 8-byte aligned", need);
+  hipError_t e = aq::launch_sample(logits, rows, n, u, params, params_ld, scratch, out, logp,
                                    static_cast<hipStream_t>(stream));
   return e == hipSuccess ? AQ_OK : hip_fail(e, "sampling launch");
 }

@@ -240,8 +240,9 @@ hipError_t launch_logits_adjust(const float *logits, int64_t rows, int64_t n,
 
 // One token for each row of logits (aq_sample.hip).
 hipError_t launch_sample(const float *logits, int64_t rows, int64_t n, const double *u,
-                         const double *params, int64_t params_ld, int64_t *out, float *logp,
-                         hipStream_t s);
+                         const double *params, int64_t params_ld, void *scratch, int64_t *out,
+                         float *logp, hipStream_t s);
+size_t sample_scratch(int64_t rows, int64_t n);
 
 // Paged 16-bit KV cache (aq_paged.hip).  The places of a call's tokens: pos and
 // seq of each, and the table of pages whose slot 0 is position start.

@@ -11,6 +11,9 @@ and aq_sample, has the exact rules).
 """
 from __future__ import annotations
 
+import ctypes
+from functools import lru_cache
+
 from . import _lib
 
 
@@ -138,6 +141,13 @@ def sampling_params(rows=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, d
     return torch.stack(cols, dim=-1).to("cuda" if device is None else device)
 
 
+@lru_cache(maxsize=64)
+def _scratch_bytes(rows: int, n: int) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.load().aq_sample_scratch(rows, n, ctypes.byref(size)))
+    return size.value
+
+
 def sample_logits(logits, u, params, *, out=None, logp=False):
     """A token for each row of the logits (n,) or (rows, n), float32 on the GPU,
     as int64 () or (rows,) (`out`: where; default: a new tensor); -1 where every
@@ -174,9 +184,13 @@ def sample_logits(logits, u, params, *, out=None, logp=False):
         raise ValueError("out must be a contiguous int64 tensor, one number a row")
     x = logits.contiguous()
     lp = torch.empty(lead, dtype=torch.float32, device=dev) if logp else None
-    _call(_lib.ensure_device().aq_sample, dev,
-          (x.data_ptr(), rows, x.shape[-1], u.data_ptr(), params.data_ptr(), 4 if per_row else 0,
-           out.data_ptr(), lp.data_ptr() if logp else None))
+    n, lib = x.shape[-1], _lib.ensure_device()
+    size = _scratch_bytes(rows, n)
+    # of this call alone: calls on other streams, and graphs, have their own
+    scratch = torch.empty(size // 4, dtype=torch.float32, device=dev)
+    _call(lib.aq_sample, dev,
+          (x.data_ptr(), rows, n, u.data_ptr(), params.data_ptr(), 4 if per_row else 0,
+           scratch.data_ptr(), size, out.data_ptr(), lp.data_ptr() if logp else None))
     return (out, lp) if logp else out
 
 

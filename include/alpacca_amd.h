@@ -453,10 +453,15 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  * same for every row; NaN: as if left out, for the temperature 0).  out [rows]: the
  * token, -1 where every logit is -infinity; logp [rows] or NULL: the logarithm of
  * its w over the sum of all kept (0 at temperature 0 or less, -infinity for -1).
- * Device pointers; enqueue only.  n up to 2^31 - 1.  Replaces Sampler.sample past
- * its repeat penalty (alpacca/sample.py:44-76). */
+ * scratch: at least aq_sample_scratch's bytes, 8-byte aligned; nothing in it outlives
+ * the call.  Device pointers; enqueue only.  n up to 2^31 - 1.  Replaces
+ * Sampler.sample past its repeat penalty (alpacca/sample.py:44-76). */
 int aq_sample(const float *logits, int64_t rows, int64_t n, const double *u,
-              const double *params, int64_t params_ld, int64_t *out, float *logp, void *stream);
+              const double *params, int64_t params_ld, void *scratch, size_t scratch_bytes,
+              int64_t *out, float *logp, void *stream);
+
+/* Scratch bytes of that call.  Host only. */
+int aq_sample_scratch(int64_t rows, int64_t n, size_t *bytes);
 
 /* ==== 8-bit KV cache =====================================================
  *

@@ -260,13 +260,19 @@ def test_refusals():
     lib, p = _lib.load(), ctypes.c_void_p(64)
     bad = _lib.AQ_ERR_VALUE
 
-    def call(rows=1, n=4, ld=0, a=p, b=p, c=p, d=p):
-        return lib.aq_sample(a, rows, n, b, c, ld, d, None, None)
+    def call(rows=1, n=4, ld=0, a=p, b=p, c=p, d=p, e=p, size=1 << 30):
+        return lib.aq_sample(a, rows, n, b, c, ld, e, size, d, None, None)
     assert call(rows=-1) == bad and call(n=-1) == bad and call(ld=-1) == bad
     assert call(rows=65536) == bad and call(n=2 ** 31) == bad and call(n=0) == bad
     assert call(ld=3) == bad
-    for name in "abcd":
+    for name in "abcde":
         assert call(**{name: None}) == bad
+    size = ctypes.c_size_t()
+    assert lib.aq_sample_scratch(3, 5000, ctypes.byref(size)) == _lib.AQ_OK
+    assert call(rows=3, n=5000, size=size.value - 1) == bad
+    assert call(e=ctypes.c_void_p(68)) == bad
+    assert lib.aq_sample_scratch(3, 0, ctypes.byref(size)) == bad
+    assert lib.aq_sample_scratch(-1, 5, ctypes.byref(size)) == bad
     assert call(rows=0, a=None, b=None, c=None, d=None) == _lib.AQ_OK
 
 
