@@ -14,9 +14,11 @@
 // range, a negative position) is absent: not stored, not attended to.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "aq_internal.h"
+#include "aq_matmul_dma.h"
 
 namespace aq {
 namespace {
@@ -146,11 +148,18 @@ struct Ops<_Float16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
                                                   __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t take(float &a, float &b) {
-    const h2 h = __builtin_convertvector(f2v{a, b}, h2);
-    a -= (float)h[0];
-    b -= (float)h[1];
-    return __builtin_bit_cast(uint32_t, h);
+  // a and b in two pieces.  The first is cut off (one instruction for the pair), so
+  // that what it leaves has their signs and is exact; the second is rounded.
+  static __device__ __forceinline__ void split(float a, float b, uint32_t (&piece)[2]) {
+    const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+    // (a factor that the compiler does not know keeps this one mixed-precision
+    // multiply-add a value instead of a conversion and a difference)
+    float minus = -1.f;
+    asm("" : "+v"(minus));
+    const h2 l = __builtin_convertvector(
+        f2v{fmaf((float)h[0], minus, a), fmaf((float)h[1], minus, b)}, h2);
+    piece[0] = __builtin_bit_cast(uint32_t, h);
+    piece[1] = __builtin_bit_cast(uint32_t, l);
   }
 };
 template <>
@@ -160,11 +169,14 @@ struct Ops<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a),
                                                    __builtin_bit_cast(b8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t take(float &a, float &b) {
-    const b2 h = __builtin_convertvector(f2v{a, b}, b2);
-    a -= (float)h[0];
-    b -= (float)h[1];
-    return __builtin_bit_cast(uint32_t, h);
+  static __device__ __forceinline__ void split(float a, float b, uint32_t (&piece)[3]) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const b2 h = __builtin_convertvector(f2v{a, b}, b2);
+      a -= (float)h[0];
+      b -= (float)h[1];
+      piece[n] = __builtin_bit_cast(uint32_t, h);
+    }
   }
 };
 
@@ -190,12 +202,13 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
 
 // A query row of the lane's (its dimensions 32 ks + 8 (l / 16) + e) in pieces of
-// q log2(e) / sqrt(HD) 2^-back.  A row with an infinity or a NaN is NaN.
+// q log2(e) / sqrt(HD) / back, back a power of two.  A row with an infinity or a NaN
+// is NaN.
 template <int HD, typename T>
 struct QRow {
   static constexpr int NP = Ops<T>::NP;
   u4v piece[NP][HD / 32];
-  int back;
+  float back;
   __device__ __forceinline__ void load(const float *q, bool live) {
     const int cg = (threadIdx.x >> 4) & 3;
     const float f = 1.44269504088896341f / __builtin_sqrtf((float)HD);
@@ -218,8 +231,9 @@ struct QRow {
     }
     am = row_max(am);
     const bool bad = am == INFINITY;
-    const int up = am > 0.f && !bad ? 15 - __builtin_amdgcn_frexp_expf(am) : 0;
-    back = -up;
+    // (a row below 2^-110 keeps fewer bits of scores that are as good as 0)
+    const int up = am > 0.f && !bad ? min(15 - __builtin_amdgcn_frexp_expf(am), 125) : 0;
+    back = ldexpf(1.f, -up);
 #pragma unroll
     for (int ks = 0; ks < HD / 32; ++ks)
 #pragma unroll
@@ -227,8 +241,10 @@ struct QRow {
         float a = ldexpf(v[ks][2 * i], up), b = ldexpf(v[ks][2 * i + 1], up);
         a = bad ? NAN : a;
         b = bad ? NAN : b;
+        uint32_t parts[NP];
+        Ops<T>::split(a, b, parts);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) piece[p][ks][i] = Ops<T>::take(a, b);
+        for (int p = 0; p < NP; ++p) piece[p][ks][i] = parts[p];
       }
   }
 };
@@ -246,22 +262,23 @@ struct RowState {
   }
 };
 
-// raw scores of a block (a tile of positions each) to weights in pieces; the state
-// moves on to the new maximum.  Positions from `rem` on do not exist.
-template <int HD, typename T>
-__device__ __forceinline__ void weigh(f4v (&sc)[2], int back, int rem, RowState<HD> &st,
-                                      u4v (&w)[Ops<T>::NP]) {
+// raw scores of NB blocks (two tiles of positions each) to weights in pieces; the state
+// moves on to the new maximum.  TAIL: positions from rem[b] on of block b do not exist.
+// (back is a power of two: scores times it are exact, in the maximum and in the
+// multiply-add that gives a weight's exponent.)
+template <int HD, typename T, int NB, bool TAIL>
+__device__ __forceinline__ void weigh(f4v (&sc)[NB][2], float back, const int (&rem)[NB],
+                                      RowState<HD> &st, u4v (&w)[NB][Ops<T>::NP]) {
   const int cg = (threadIdx.x >> 4) & 3;
   float top = -INFINITY;
 #pragma unroll
-  for (int pt = 0; pt < 2; ++pt)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float z = ldexpf(sc[pt][r], back);
-      if (16 * pt + 4 * cg + r >= rem) z = -INFINITY;
-      sc[pt][r] = z;
-      top = fmaxf(top, z);
+    for (int e = 0; e < 8; ++e) {
+      if (TAIL && 16 * (e >> 2) + 4 * cg + (e & 3) >= rem[b]) sc[b][e >> 2][e & 3] = -INFINITY;
+      top = fmaxf(top, sc[b][e >> 2][e & 3]);
     }
+  top *= back;
   if (__any(top > st.m)) {
     const float m = fmaxf(st.m, ceilf(row_max(top)));
     const float f = st.m == -INFINITY ? 0.f : exp2_(st.m - m);
@@ -270,17 +287,23 @@ __device__ __forceinline__ void weigh(f4v (&sc)[2], int back, int rem, RowState<
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) st.o[i] *= f;
   }
-  const float ref = finite_ref(st.m) - kTop;
-  float p[8];
+  const float ref = kTop - finite_ref(st.m);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    p[e] = exp2_(sc[e >> 2][e & 3] - ref);
-    st.l += p[e];
+  for (int b = 0; b < NB; ++b) {
+    float p[8], l[4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = exp2_(fmaf(sc[b][e >> 2][e & 3], back, ref));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l[e] = p[e] + p[4 + e];
+    st.l += (l[0] + l[1]) + (l[2] + l[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t parts[Ops<T>::NP];
+      Ops<T>::split(p[2 * i], p[2 * i + 1], parts);
+#pragma unroll
+      for (int n = 0; n < Ops<T>::NP; ++n) w[b][n][i] = parts[n];
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int n = 0; n < Ops<T>::NP; ++n) w[n][i] = Ops<T>::take(p[2 * i], p[2 * i + 1]);
 }
 
 // values at positions from `rem` on become 0 (whatever lies there, a weight of 0
@@ -311,13 +334,56 @@ __device__ __forceinline__ int64_t of_lane(int64_t v, int lane) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// RT tiles of rows against blocks b0 + wave, b0 + wave + 4, .. below b1 of a list
-// of pages that holds len positions.  A wave's next keys are on their way while
-// it weighs the present ones.
-template <int HD, typename T, int RT>
-__device__ __forceinline__ void attend_blocks(const aq_paged &c, const int32_t *pages, int h,
-                                              int64_t b0, int64_t b1, int64_t len,
-                                              const QRow<HD, T> (&q)[RT], RowState<HD> (&st)[RT]) {
+// A tile of rows against NB blocks: keys(b, j) is operand j = pt * HD / 32 + ks of
+// block b, values(b, j) that of its dimensions 16 j ..  Products of different sums
+// follow one another: one that adds to the last one's result would wait for it.
+// scored() runs when the scores' products are on their way.
+template <int HD, typename T, int NB, bool TAIL, class K, class V, class Next>
+__device__ __forceinline__ void attend_block(const QRow<HD, T> &q, RowState<HD> &st,
+                                             const int (&rem)[NB], K &&keys, V &&values,
+                                             Next &&scored) {
+  constexpr int KS = HD / 32, NP = Ops<T>::NP;
+  f4v sc[NB][2];
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) sc[i >> 1][i & 1] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    u4v k[2 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) k[i] = keys(i >> 1, (i & 1) * KS + ks);
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i)
+        sc[i >> 1][i & 1] = Ops<T>::mfma(k[i], q.piece[p][ks], sc[i >> 1][i & 1]);
+  }
+  scored();
+  u4v w[NB][NP];
+  weigh<HD, T, NB, TAIL>(sc, q.back, rem, st, w);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < HD / 16; j += 4) {
+      u4v v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = values(b, j + i);
+        if (TAIL) v[i] = only_first(v[i], rem[b]);
+      }
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[j + i] = Ops<T>::mfma(v[i], w[b][p], st.o[j + i]);
+    }
+}
+
+// One tile of rows against blocks b0 + wave, b0 + wave + 4, .. below b1 of a list of
+// pages that holds len positions, straight from memory.  A wave's next keys are on
+// their way while it weighs the present ones.
+template <int HD, typename T>
+__device__ __forceinline__ void attend_strided(const aq_paged &c, const int32_t *pages, int h,
+                                               int64_t b0, int64_t b1, int64_t len,
+                                               const QRow<HD, T> &q, RowState<HD> &st) {
   constexpr int KS = HD / 32, DT = HD / 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u4v *kp = static_cast<const u4v *>(c.k) + lane, *vp = static_cast<const u4v *>(c.v) + lane;
@@ -333,41 +399,91 @@ __device__ __forceinline__ void attend_blocks(const aq_paged &c, const int32_t *
     while (left) {
       left &= left - 1;
       const int64_t after = len - (base + 4 * i) * kBlk;
-      const int rem = after < kBlk ? (int)after : kBlk;
+      const int rem[1] = {after < kBlk ? (int)after : kBlk};
 #pragma unroll
       for (int j = 0; j < DT; ++j) v[j] = vp[at + 64 * j];
-      f4v sc[RT][2];
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt) {
-          sc[t][pt] = f4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int p = Ops<T>::NP - 1; p >= 0; --p)
-              sc[t][pt] = Ops<T>::mfma(k[pt * KS + ks], q[t].piece[p][ks], sc[t][pt]);
-        }
-      if (left) {
+      auto keys = [&](int, int j) { return k[j]; };
+      auto values = [&](int, int j) { return v[j]; };
+      auto next = [&] {
+        if (!left) return;
         i = __builtin_ctzll(left);
         at = of_lane(mine, i) * (kBlk * HD / 8);
 #pragma unroll
         for (int j = 0; j < 2 * KS; ++j) k[j] = kp[at + 64 * j];
+      };
+      if (rem[0] < kBlk) attend_block<HD, T, 1, true>(q, st, rem, keys, values, next);
+      else attend_block<HD, T, 1, false>(q, st, rem, keys, values, next);
+    }
+  }
+}
+
+// The same for TW tiles of rows, a wave each, against blocks b0 .. b1 - 1,
+// which go through LDS in stages of 4 / TW ways of NB blocks: the four waves bring one
+// while another is computed.
+template <int HD, int TW>
+struct Stage {
+  static constexpr int NB = TW == 4 ? 2 : 1, WAYS = 4 / TW, BLOCKS = WAYS * NB;
+  static constexpr int BLOCK = HD * 128;  // bytes of K and V
+  static constexpr int BYTES = BLOCKS * BLOCK;
+};
+template <int HD, typename T, int TW, class Load>
+__device__ __forceinline__ void attend_staged(const aq_paged &c, const int32_t *pages, int h,
+                                              int64_t b0, int64_t b1, int64_t len, uint8_t *lds,
+                                              QRow<HD, T> &q, RowState<HD> &st,
+                                              Load &&load_rows) {
+  using St = Stage<HD, TW>;
+  constexpr int NB = St::NB;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds0 = lds_offset(lds);
+  for (int64_t base = b0; base < b1; base += 64) {
+    const int64_t mine = lane_block(c, pages, h, base + lane, b1) * (kBlk * HD * 2);  // bytes
+    uint64_t to_bring = __ballot(mine >= 0), to_do = to_bring;
+    auto bring = [&](int buf) {
+#pragma unroll
+      for (int p = 0; p < St::BLOCKS; ++p) {
+        if (!to_bring) break;
+        const int64_t at = of_lane(mine, __builtin_ctzll(to_bring));
+        to_bring &= to_bring - 1;
+        const char *k = static_cast<const char *>(c.k) + at, *v = static_cast<const char *>(c.v) + at;
+        const uint32_t to = lds0 + buf * St::BYTES + p * St::BLOCK;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+          const int x = 1024 * (4 * j + wave);
+          dma16(to + x, 16 * lane, k + x);
+          dma16(to + HD * 64 + x, 16 * lane, v + x);
+        }
       }
-      if (rem < kBlk) {
+    };
+    __syncthreads();  // (the buffers are free)
+    bring(0);
+    if (base == b0) load_rows();  // beside the first stage's way
+    for (int buf = 0; to_do; buf ^= 1) {
+      dma_barrier<0>();  // this stage is there, and the other buffer has been used
+      auto next = [&] { bring(buf ^ 1); };
+      // the wave's blocks of the stage
+      int rem[NB];
+      bool full = true;
 #pragma unroll
-        for (int j = 0; j < DT; ++j) v[j] = only_first(v[j], rem);
+      for (int p = 0; p < St::BLOCKS; ++p) {
+        if (p / NB == wave / TW) {
+          const int64_t behind = to_do ? len - (base + __builtin_ctzll(to_do)) * kBlk : 0;
+          rem[p % NB] = behind < kBlk ? (int)behind : kBlk;
+          full &= behind >= kBlk;
+        }
+        to_do &= to_do - 1;
       }
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        u4v w[Ops<T>::NP];
-        weigh<HD, T>(sc[t], q[t].back, rem, st[t], w);
-#pragma unroll
-        for (int j = 0; j < DT; ++j)
-#pragma unroll
-          for (int p = Ops<T>::NP - 1; p >= 0; --p)
-            st[t].o[j] = Ops<T>::mfma(v[j], w[p], st[t].o[j]);
+      if (rem[0] <= 0) {
+        next();
+        continue;
       }
+      const uint8_t *at = lds + buf * St::BYTES + (wave / TW) * (NB * St::BLOCK) + 16 * lane;
+      auto keys = [&](int b, int j) { return lds_read<u4v>(at + b * St::BLOCK + 1024 * j); };
+      auto values = [&](int b, int j) {
+        return lds_read<u4v>(at + b * St::BLOCK + HD * 64 + 1024 * j);
+      };
+      if (full) attend_block<HD, T, NB, false>(q, st, rem, keys, values, next);
+      else attend_block<HD, T, NB, true>(q, st, rem, keys, values, next);
     }
   }
 }
@@ -378,9 +494,10 @@ constexpr int kState = HD + 4;
 
 // How a call's work is split (host and kernels).
 struct PagedPlan {
-  int rt;          // tiles of 16 rows that a wave takes of the prefix
-  int groups;      // groups of 16 rt rows of a kv head
+  int tw;          // tiles of 16 rows of the prefix that a workgroup takes
+  int groups;      // groups of 16 tw rows of a kv head
   int sp, ss;      // splits of the prefix and of a row's own positions
+  unsigned pre, own;  // workgroups of each, in this order
   int states() const { return sp + ss; }
 };
 
@@ -390,45 +507,58 @@ __device__ __forceinline__ void put_dead(float *state) {
   state[HD + 1] = 0.f;
 }
 
-// Workgroups 0 .. n_pre - 1: split, group of rows and kv head of the prefix; then
-// split, kv head and row of the rows' own positions (a row that ends inside the
-// prefix has that part of it as its own).  The four waves take every fourth block
-// each and their states are merged through LDS.
-template <int HD, typename T, int RT>
+// Item `item` of the prefix: a split of a kv head, and a group of rows.  The groups
+// that read the same positions follow one another eight items apart, which is on
+// the same one of the eight dies, whose L2 then holds them.
+__device__ __forceinline__ void pick_unit(const PagedPlan &p, unsigned units, unsigned item,
+                                          unsigned &unit, unsigned &group) {
+  const unsigned groups = p.groups, full = units / 8 * 8;
+  if (item < full * groups) {
+    unit = item / (8 * groups) * 8 + item % 8;
+    group = item / 8 % groups;
+  } else {
+    item -= full * groups;
+    unit = full + item % (units - full);
+    group = item / (units - full);
+  }
+}
+
+// Items of the prefix: a split, a group of rows and a kv head; own ones: a split, a kv
+// head and a row (a row that ends inside the prefix has that part of it as its own).
+// Waves that share rows have their states merged through LDS.
+template <int HD, typename T, int TW>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     k_paged_attn(const float *__restrict__ q, int64_t N, int n_head, PagedTable tab,
                  PagedTable pre, aq_paged c, PagedPlan plan, float *__restrict__ states,
                  float *__restrict__ out) {
-  constexpr int LD = HD + 4;
-  __shared__ __attribute__((aligned(16))) float num[4][16][LD];
-  __shared__ float mm[4][16], ll[4][16];
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  auto num = reinterpret_cast<float(*)[16][HD + 4]>(lds);  // numerators, maximum, sum of 4 waves
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, cg = lane >> 4;
   const int G = n_head / c.n_kv, S = plan.sp + plan.ss;
-  const int n_pre = plan.sp * plan.groups * c.n_kv;
-  const bool is_pre = (int)blockIdx.x < n_pre;
+  const bool is_pre = blockIdx.x < plan.pre;
+  unsigned item = blockIdx.x - (is_pre ? 0u : plan.pre);
   int h, split;
   int64_t len, b0, b1;
   const int32_t *pages;
-  const int64_t rows = N * G;  // of a kv head
-  int64_t row0 = 0;            // of the group
-  int64_t n = 0;
+  const int rows = (int)N * G;  // of a kv head (N * n_head is below 2^24)
+  int row0 = 0;                 // of the group
+  int n = 0;
   if (is_pre) {
-    int x = blockIdx.x;
-    split = x % plan.sp;
-    x /= plan.sp;
-    h = x % c.n_kv;
-    row0 = (int64_t)(x / c.n_kv) * (16 * RT);
+    unsigned unit, group;
+    pick_unit(plan, (unsigned)(plan.sp * c.n_kv), item, unit, group);
+    split = (int)(unit % plan.sp);
+    h = (int)(unit / plan.sp);
+    row0 = (int)group * (16 * TW);
     pages = pre.pages;
     len = pre.start;
     const int64_t blocks = (len + kBlk - 1) / kBlk, each = (blocks + plan.sp - 1) / plan.sp;
     b0 = split * each;
     b1 = b0 + each < blocks ? b0 + each : blocks;
   } else {
-    int64_t x = (int64_t)blockIdx.x - n_pre;
-    split = (int)(x % plan.ss);
-    x /= plan.ss;
-    h = (int)(x % c.n_kv);
-    n = x / c.n_kv;
+    split = (int)(item % plan.ss);
+    item /= plan.ss;
+    h = (int)(item % c.n_kv);
+    n = (int)(item / c.n_kv);
     row0 = n * G;
     const int64_t pos = tab.pos[n], seq = tab.seq ? tab.seq[n] : n;
     len = 0;
@@ -448,80 +578,100 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     b1 = b0 + each < blocks ? b0 + each : blocks;
     split += plan.sp;
   }
-  auto write = [&](auto &st, int64_t first, int64_t end) {  // rows first .. of this tile
+  // the states of `tiles` tiles of rows, the first one's first row `first`, wave w's
+  // of tile w % tiles, to memory
+  auto write = [&](const RowState<HD> &st, int tiles, int first, int end) {
     const float l = row_sum(st.l);
+    __syncthreads();
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d)
       *reinterpret_cast<f4v *>(&num[wave][j][16 * d + 4 * cg]) = st.o[d];
-    if (cg == 0) mm[wave][j] = st.m, ll[wave][j] = l;
+    if (cg == 0) num[wave][j][HD] = st.m, num[wave][j][HD + 1] = l;
     __syncthreads();
     // 16 threads a row
     const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
-    const int64_t row = first + r;
-    if (row < end) {
-      const float m = fmaxf(fmaxf(mm[0][r], mm[1][r]), fmaxf(mm[2][r], mm[3][r]));
-      float f[4], sum = 0.f;
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int row = first + 16 * tile + r;
+      if (row >= end) break;
+      float m = -INFINITY, sum = 0.f;
+      for (int w = tile; w < 4; w += tiles) m = fmaxf(m, num[w][r][HD]);
+      f4v o[HD / 64];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        f[w] = mm[w][r] == -INFINITY ? 0.f : exp2_(mm[w][r] - m);
-        sum += ll[w][r] == 0.f ? 0.f : ll[w][r] * (m == -INFINITY ? 1.f : f[w]);
+      for (int d = 0; d < HD / 64; ++d) o[d] = f4v{0.f, 0.f, 0.f, 0.f};
+      for (int w = tile; w < 4; w += tiles) {
+        const float mw = num[w][r][HD], lw = num[w][r][HD + 1];
+        const float f = mw == -INFINITY ? 0.f : exp2_(mw - m);
+        sum += lw == 0.f ? 0.f : lw * (m == -INFINITY ? 1.f : f);
+#pragma unroll
+        for (int d = 0; d < HD / 64; ++d)
+          o[d] += f * *reinterpret_cast<const f4v *>(&num[w][r][64 * d + 4 * part]);
       }
-      const int64_t i = row / G, head = (int64_t)h * G + row % G;
-      const int64_t flat = i * n_head + head;
+      const int i = row / G;
+      const int64_t flat = (int64_t)i * n_head + h * G + (row - i * G);
       const bool skip = is_pre && tab.pos[i] < pre.start;
       float *dst = S == 1 ? out + flat * HD : states + (flat * S + split) * kState<HD>;
       const float inv = S == 1 ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
 #pragma unroll
-      for (int d = 4 * part; d < HD; d += 64) {
-        f4v o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) o += f[w] * *reinterpret_cast<const f4v *>(&num[w][r][d]);
-        *reinterpret_cast<f4v *>(dst + d) = o * inv;
-      }
+      for (int d = 0; d < HD / 64; ++d)
+        *reinterpret_cast<f4v *>(dst + 64 * d + 4 * part) = o[d] * inv;
       if (S != 1 && part == 0) {
         dst[HD] = skip ? -INFINITY : m;
         dst[HD + 1] = skip ? 0.f : sum;
       }
     }
-    __syncthreads();
   };
   if (is_pre) {
-    QRow<HD, T> qr[RT];
-    RowState<HD> st[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int64_t row = row0 + 16 * t + j;
+    QRow<HD, T> qr;
+    RowState<HD> st;
+    st.clear();
+    auto load_rows = [&] {
+      const int row = row0 + 16 * (wave % TW) + j;
       const bool live = row < rows;
-      const int64_t i = live ? row / G : 0, head = (int64_t)h * G + (live ? row % G : 0);
-      qr[t].load(q + (i * n_head + head) * HD, live);
-      st[t].clear();
+      const int i = live ? row / G : 0, head = h * G + (live ? row - i * G : 0);
+      qr.load(q + ((int64_t)i * n_head + head) * HD, live);
+    };
+    if constexpr (TW == 1) {
+      load_rows();
+      attend_strided<HD, T>(c, pages, h, b0, b1, len, qr, st);
+    } else {
+      attend_staged<HD, T, TW>(c, pages, h, b0, b1, len, lds, qr, st, load_rows);
     }
-    attend_blocks<HD, T, RT>(c, pages, h, b0, b1, len, qr, st);
-#pragma unroll
-    for (int t = 0; t < RT; ++t) write(st[t], row0 + 16 * t, rows);
+    write(st, TW, row0, rows);
   } else {
     if (b0 >= b1 && S != 1) {  // nothing of the row here
       if ((int)threadIdx.x < G)
-        put_dead<HD>(states + ((n * n_head + h * G + threadIdx.x) * S + split) * kState<HD>);
+        put_dead<HD>(states + (((int64_t)n * n_head + h * G + threadIdx.x) * S + split) * kState<HD>);
       return;
     }
-    QRow<HD, T> qr[1];
-    RowState<HD> st[1];
-    qr[0].load(q + (n * n_head + h * G + (j < G ? j : 0)) * HD, j < G);
-    st[0].clear();
-    attend_blocks<HD, T, 1>(c, pages, h, b0, b1, len, qr, st);
-    write(st[0], row0, row0 + G);
+    QRow<HD, T> qr;
+    RowState<HD> st;
+    qr.load(q + ((int64_t)n * n_head + h * G + (j < G ? j : 0)) * HD, j < G);
+    st.clear();
+    attend_strided<HD, T>(c, pages, h, b0, b1, len, qr, st);
+    write(st, 1, row0, row0 + G);
   }
 }
 
-// One wave an output row: the states of its splits, at most 64.
-template <int HD>
+// One row's states of its S <= 64 splits to its output: NT threads, four dimensions
+// each, HD / 4 of them a state, all loads under way at once.  One wave up to 8 states,
+// four from there on: 48 states of 256 rows of 128 in 4 us (13.3 in one wave, state
+// after state).
+template <int HD, int NT>
 __global__ void __launch_bounds__(256)
     k_paged_merge(const float *__restrict__ states, int64_t rows, int S, float *__restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int TPS = HD / 4, GROUPS = NT / TPS, PER = 64 / (NT == 64 ? 8 : 1) / GROUPS;
+  __shared__ __attribute__((aligned(16))) float num[NT == 256 ? 4 : 1][HD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = NT == 64 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (row >= rows) return;
   states += row * S * kState<HD>;
+  const int t = threadIdx.x & (NT - 1), g = t / TPS, d = 4 * (t % TPS);
+  f4v x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = g + GROUPS * i;
+    x[i] = *reinterpret_cast<const f4v *>(states + (s < S ? s : 0) * kState<HD> + d);
+  }
   float m = -INFINITY, l = 0.f;
   if (lane < S) {
     m = states[lane * kState<HD> + HD];
@@ -535,36 +685,60 @@ __global__ void __launch_bounds__(256)
   float sum = some ? l * f : 0.f;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-  constexpr int PER = HD / 64;
-  float o[PER] = {};
-  uint64_t left = __ballot(some);
-  while (left) {
-    const int s = __builtin_ctzll(left);
-    left &= left - 1;
-    const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+  const uint64_t live = __ballot(some);
+  f4v o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = fmaf(states[s * kState<HD> + PER * lane + i], fs, o[i]);
+  for (int i = 0; i < PER; ++i) {
+    const int s = g + GROUPS * i;
+    const float fs = __shfl(f, s & 63);
+    const bool use = s < S && (live >> (s & 63) & 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = use ? fmaf(x[i][e], fs, o[e]) : o[e];
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  // over the wave's groups
 #pragma unroll
-  for (int i = 0; i < PER; ++i) out[row * HD + PER * lane + i] = o[i] * inv;
+  for (int off = 32; off >= TPS && off > 0; off >>= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+  if constexpr (NT == 256) {
+    if (lane < TPS) *reinterpret_cast<f4v *>(&num[wave][d]) = o;
+    __syncthreads();
+    if (wave > 0 || lane >= TPS) return;
+    o = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const f4v *>(&num[w][d]);
+  }
+  if (lane < TPS)
+    *reinterpret_cast<f4v *>(out + row * HD + d) = o * (sum == 0.f ? 0.f : 1.f / sum);
 }
 
+// Splits.  A row's own positions: until 512 workgroups (two a CU), at least four blocks
+// each.  The prefix: tiles of 16 rows in one workgroup of four waves that share the
+// positions up to 16 rows and of two up to 32, bound by memory (8 rows of 4 heads over
+// 100000 positions 89 us in 48 splits of 8 heads, 92 in 32); past that four tiles that
+// share them through LDS, a workgroup a CU: the rows' own positions, bound by memory,
+// run on the same CUs (64 rows of 32 / 8 heads over 8000 and 1024 of their own 68 us;
+// with two workgroups of the prefix a CU, twice the states, 82; the two kinds in
+// turn 75, where rows that own little then wait for a late start: 28 against 25).
 PagedPlan paged_plan(const aq_paged &c, int64_t N, int n_head, int64_t width, int64_t start) {
-  const int64_t rows = N * (n_head / c.n_kv), want = 512;
-  PagedPlan p = {1, 0, 0, 1};
-  auto splits = [&](int64_t items, int64_t blocks) {  // at least a block a wave
-    int64_t s = (want + items - 1) / items;
-    const int64_t most = (blocks + 3) / 4;
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  const int64_t rows = N * (n_head / c.n_kv);
+  PagedPlan p = {};
+  p.tw = 1;
+  // `items` workgroups over `blocks` blocks each, split until there are `want`, but at
+  // least `least` blocks a split
+  auto splits = [&](int64_t want, int64_t items, int64_t blocks, int64_t least, int64_t most) {
+    const int64_t s = std::min((want + items - 1) / items, (blocks + least - 1) / least);
+    return (int)std::max<int64_t>(1, std::min(s, most));
   };
   if (start > 0) {
-    p.rt = rows > 16 && c.head_dim < 256 ? 2 : 1;
-    p.groups = (int)((rows + 16 * p.rt - 1) / (16 * p.rt));
-    p.sp = splits((int64_t)p.groups * c.n_kv, (start + kBlk - 1) / kBlk);
+    p.tw = rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    p.groups = (int)((rows + 16 * p.tw - 1) / (16 * p.tw));
+    p.sp = splits(p.tw == 2 ? 512 : 256, (int64_t)p.groups * c.n_kv, (start + kBlk - 1) / kBlk,
+                  p.tw == 4 ? 8 : 4, 48);
   }
-  p.ss = splits(N * c.n_kv, width * c.page_size / kBlk);
+  p.ss = splits(512, N * c.n_kv, width * c.page_size / kBlk, 4, p.sp ? 16 : 64);
+  p.pre = (unsigned)(p.sp * p.groups * c.n_kv);
+  p.own = (unsigned)(p.ss * N * c.n_kv);
   return p;
 }
 
@@ -612,24 +786,31 @@ hipError_t launch_attention_paged(const float *q, int64_t N, int n_head, const P
                                   const PagedTable &pre, const aq_paged &c, float *states,
                                   float *out, hipStream_t s) {
   const PagedPlan p = paged_plan(c, N, n_head, tab.width, tab.start);
-  const int64_t wgs = (int64_t)p.sp * p.groups * c.n_kv + (int64_t)p.ss * N * c.n_kv;
+  hipError_t e = hipSuccess;
   by_shape(c, [&](auto hd, auto t) {
     constexpr int HD = decltype(hd)::value;
-    auto go = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), 0, s, q, N, n_head, tab, pre, c, p,
+    auto go = [&](auto tw) {
+      constexpr int TW = decltype(tw)::value;
+      auto kern = k_paged_attn<HD, decltype(t), TW>;
+      constexpr int merge = 4 * 16 * (HD + 4) * (int)sizeof(float);
+      constexpr int lds = TW == 1 ? merge : std::max(merge, 2 * Stage<HD, TW>::BYTES);
+      e = set_dynamic_lds(reinterpret_cast<const void *>(kern), lds);
+      if (e != hipSuccess) return;
+      hipLaunchKernelGGL(kern, dim3(p.pre + p.own), dim3(256), lds, s, q, N, n_head, tab, pre, c, p,
                          states, out);
     };
-    if constexpr (HD < 256) {
-      if (p.rt == 2) go(k_paged_attn<HD, decltype(t), 2>);
-      else go(k_paged_attn<HD, decltype(t), 1>);
-    } else {
-      go(k_paged_attn<HD, decltype(t), 1>);
-    }
-    if (p.states() > 1)
-      hipLaunchKernelGGL((k_paged_merge<HD>), dim3((unsigned)((N * n_head + 3) / 4)), dim3(256), 0,
-                         s, states, N * n_head, p.states(), out);
+    if (p.tw == 1) go(std::integral_constant<int, 1>());
+    else if (p.tw == 2) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
+    if (e != hipSuccess) return;
+    if (p.states() > 8)
+      hipLaunchKernelGGL((k_paged_merge<HD, 256>), dim3((unsigned)(N * n_head)), dim3(256), 0, s,
+                         states, N * n_head, p.states(), out);
+    else if (p.states() > 1)
+      hipLaunchKernelGGL((k_paged_merge<HD, 64>), dim3((unsigned)((N * n_head + 3) / 4)),
+                         dim3(256), 0, s, states, N * n_head, p.states(), out);
   });
-  return hipGetLastError();
+  return e == hipSuccess ? hipGetLastError() : e;
 }
 
 }  // namespace aq
