@@ -1463,6 +1463,9 @@ int paged_tokens(const aq_paged *c, int64_t N, const int32_t *table, int64_t seq
   if (seqs < 0 || width < 0 || start < 0 || seqs > INT32_MAX || width > INT32_MAX)
     return fail(AQ_ERR_VALUE, "bad table shape (%lld rows of %lld pages, start %lld)",
                 (long long)seqs, (long long)width, (long long)start);
+  if (width > INT32_MAX / c->page_size)
+    return fail(AQ_ERR_VALUE, "rows of %lld pages of %d hold more than 2^31 - 1 positions",
+                (long long)width, c->page_size);
   if (N && (!pos || (seqs && width && !table))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
   return AQ_OK;
 }
@@ -1475,7 +1478,7 @@ int paged_attention_shape(const aq_paged *c, int64_t N, int n_head, int64_t widt
   if (N < 0 || N > ((int64_t)1 << 24) / n_head)
     return fail(AQ_ERR_VALUE, "%lld query rows of %d heads are too many for one call",
                 (long long)N, n_head);
-  if (width < 0 || start < 0 || width > INT32_MAX || start > ((int64_t)1 << 40))
+  if (width < 0 || start < 0 || width > INT32_MAX / c->page_size || start > INT32_MAX)
     return fail(AQ_ERR_VALUE, "bad table width %lld or start %lld", (long long)width,
                 (long long)start);
   return AQ_OK;
@@ -1508,6 +1511,8 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
   hipError_t e = aq::launch_rope_paged(q, k, v, q_out, N, n_head, n_rot, neox ? 1 : 0, cos_tab,
                                        sin_tab, n_pos, {table, seqs, width, seq, pos, start},
                                        *cache, static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidValue)
+    return fail(AQ_ERR_VALUE, "%lld tokens are too many for one call", (long long)N);
   return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache append launch");
 }
 
@@ -1553,6 +1558,8 @@ int aq_paged_read(const aq_paged *cache, int64_t N, const int32_t *table, int64_
   if (N == 0) return AQ_OK;
   hipError_t e = aq::launch_paged_read(N, {table, seqs, width, seq, pos, start}, *cache, k, v,
                                        static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidValue)
+    return fail(AQ_ERR_VALUE, "%lld tokens are too many for one call", (long long)N);
   return e == hipSuccess ? AQ_OK : hip_fail(e, "paged cache read launch");
 }
 

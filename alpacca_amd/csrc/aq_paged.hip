@@ -38,48 +38,212 @@ __device__ __forceinline__ T rounded(float x) {
   return (T)x;  // to nearest, ties to even
 }
 
+// A value that no store of the kernel reaches, at a place that is the same for the
+// whole wave: a scalar load.
+template <typename T>
+__device__ __forceinline__ T load_const(const T *p) {
+  return *(const __attribute__((address_space(4))) T *)p;
+}
+
 // the block that holds slot `slot` of row `seq`: its number in the pool's blocks of
-// kv head 0, or -1
+// kv head 0, or -1 (slots are below 2^31: the host sees to it)
 __device__ __forceinline__ int64_t block_of(const aq_paged &c, const PagedTable &t, int64_t seq,
                                             int64_t slot) {
-  const int64_t per = c.page_size / kBlk;
+  const int per = c.page_size / kBlk;
   if (seq < 0 || seq >= t.seqs || slot < 0 || slot >= t.width * c.page_size) return -1;
-  const int64_t id = t.pages[seq * t.width + slot / c.page_size];
+  const uint32_t block = (uint32_t)slot / kBlk, page = block / (uint32_t)per;
+  const int64_t id = load_const(t.pages + seq * t.width + page);
   if (id < 0 || id >= c.n_pages) return -1;
-  return id * c.n_kv * per + slot % c.page_size / kBlk;
+  return id * c.n_kv * per + (block - page * (uint32_t)per);
+}
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T>
+struct Vec;
+template <>
+struct Vec<_Float16> {
+  typedef _Float16 four __attribute__((ext_vector_type(4)));
+  typedef _Float16 eight __attribute__((ext_vector_type(8)));
+};
+template <>
+struct Vec<__bf16> {
+  typedef __bf16 four __attribute__((ext_vector_type(4)));
+  typedef __bf16 eight __attribute__((ext_vector_type(8)));
+};
+
+// A call's tokens and where they go.
+struct Place {
+  int64_t pos, block;  // block -1: no place
+  int s;               // the position in the block
+};
+__device__ __forceinline__ Place place_of(const aq_paged &c, const PagedTable &tab, int64_t n) {
+  Place p;
+  p.pos = load_const(tab.pos + n);
+  const int64_t seq = tab.seq ? load_const(tab.seq + n) : n, slot = p.pos - tab.start;
+  p.block = p.pos < 0 ? -1 : block_of(c, tab, seq, slot);
+  p.s = (int)(slot & (kBlk - 1));
+  return p;
+}
+// Values go four tokens at a time, where these lie side by side in a page (a prompt's do:
+// group g holds tokens 4 g - lead .., so that the first token's neighbours start at a
+// multiple of four), 8 bytes a dimension; other tokens one by one.
+__device__ __forceinline__ int lead_of(const PagedTable &tab) {
+  return (int)((load_const(tab.pos) - tab.start) & 3);
+}
+struct Group {
+  int64_t n[4];
+  Place p[4];
+  bool in[4], together;
+};
+__device__ __forceinline__ Group group_of(const aq_paged &c, const PagedTable &tab, int64_t N,
+                                          int64_t g, int64_t n_pos) {
+  Group r;
+  const int64_t first = 4 * g - lead_of(tab);
+  r.together = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.in[i] = first + i >= 0 && first + i < N;
+    r.n[i] = r.in[i] ? first + i : 0;
+    r.p[i] = place_of(c, tab, r.n[i]);
+    r.in[i] &= r.p[i].block >= 0 && r.p[i].pos < n_pos;
+    r.together &= r.in[i] && r.p[i].block == r.p[0].block && r.p[i].s == r.p[0].s + i;
+  }
+  r.together &= (r.p[0].s & 3) == 0;
+  return r;
 }
 
 // ---- rotation and append -------------------------------------------------------
+// A thread a unit, each value read once and written once: of a query or key 8 dimensions
+// (neox: the rotated ones are four and their four partners), 16 bytes of a page; of the
+// values four dimensions of four tokens.  Workgroups 0 .. n_qk - 1 take the queries and
+// keys, per_token of them a token, the others the values.
+//
+// One token of 32 / 8 heads of 64 3 us (its chain: position, page, store), 2048 of 32 / 8
+// of 128 bound by memory.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256)
     k_paged_append(const float *q, const float *__restrict__ k, const float *__restrict__ v,
-                   float *q_out, int n_head, int n_rot, int neox, const float *__restrict__ cos_t,
-                   const float *__restrict__ sin_t, int64_t n_pos, PagedTable tab, aq_paged c) {
+                   float *q_out, int64_t N, int n_head, int n_rot, int neox,
+                   const float *__restrict__ cos_t, const float *__restrict__ sin_t,
+                   int64_t n_pos, PagedTable tab, aq_paged c, unsigned per_token,
+                   unsigned per_group, unsigned n_qk) {
+#pragma clang fp contract(off)
+  const int64_t per = c.page_size / kBlk;
+  if (blockIdx.x >= n_qk) {
+    const unsigned b = blockIdx.x - n_qk;
+    const int u = (int)(b % per_group) * 256 + threadIdx.x;
+    if (u >= c.n_kv * (HD / 4)) return;
+    const int h = u / (HD / 4), d = 4 * (u % (HD / 4));
+    const Group g = group_of(c, tab, N, b / per_group, n_pos);
+    f4v x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = *reinterpret_cast<const f4v *>(v + (g.n[i] * c.n_kv + h) * HD + d);
+    T *vp = static_cast<T *>(c.v);
+    if (g.together) {
+      T *to = vp + (g.p[0].block + h * per) * (kBlk * HD) + v_place(g.p[0].s, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<typename Vec<T>::four *>(to + 8 * e) = typename Vec<T>::four{
+            rounded<T>(x[0][e]), rounded<T>(x[1][e]), rounded<T>(x[2][e]), rounded<T>(x[3][e])};
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!g.in[i]) continue;
+      T *to = vp + (g.p[i].block + h * per) * (kBlk * HD) + v_place(g.p[i].s, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[8 * e] = rounded<T>(x[i][e]);
+    }
+    return;
+  }
+  const int64_t n = blockIdx.x / per_token;
+  const int u = (int)(blockIdx.x % per_token) * 256 + threadIdx.x;
+  const int heads = (q ? n_head : 0) + c.n_kv;
+  if (u >= heads * (HD / 8)) return;
+  int h = u / (HD / 8);
+  const int i = u % (HD / 8), half = n_rot / 2;
+  const bool is_k = h < c.n_kv;
+  if (!is_k) h -= c.n_kv;
+  const float *src = is_k ? k + (n * c.n_kv + h) * HD : q + (n * n_head + h) * HD;
+  // the unit's two quads: side by side, or partners
+  const bool pairs = neox && 8 * i < n_rot;
+  const int a = pairs ? 4 * i : 8 * i, b = pairs ? a + half : a + 4;
+  f4v x = *reinterpret_cast<const f4v *>(src + a), y = *reinterpret_cast<const f4v *>(src + b);
+  const Place p = place_of(c, tab, n);
+  if (p.pos < 0 || p.pos >= n_pos) return;  // (the whole workgroup)
+  const float *cr = cos_t + p.pos * half, *sr = sin_t + p.pos * half;
+  if (pairs) {
+    const f4u cs = *reinterpret_cast<const f4u *>(cr + a), sn = *reinterpret_cast<const f4u *>(sr + a);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float r0 = x[e] * cs[e] - y[e] * sn[e];
+      const float r1 = x[e] * sn[e] + y[e] * cs[e];
+      x[e] = r0;
+      y[e] = r1;
+    }
+  } else if (!neox && 8 * i < n_rot) {
+    f4u cs, sn;  // of pairs 4 i .. 4 i + 3, those that exist
+    if (8 * i + 8 <= n_rot) {
+      cs = *reinterpret_cast<const f4u *>(cr + 4 * i);
+      sn = *reinterpret_cast<const f4u *>(sr + 4 * i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 4 * i + e < half ? 4 * i + e : half - 1;
+        cs[e] = cr[j], sn[e] = sr[j];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (4 * i + e >= half) continue;
+      const float x0 = e < 2 ? x[2 * e] : y[2 * e - 4], x1 = e < 2 ? x[2 * e + 1] : y[2 * e - 3];
+      const float r0 = x0 * cs[e] - x1 * sn[e];
+      const float r1 = x0 * sn[e] + x1 * cs[e];
+      if (e < 2) x[2 * e] = r0, x[2 * e + 1] = r1;
+      else y[2 * e - 4] = r0, y[2 * e - 3] = r1;
+    }
+  }
+  if (!is_k) {
+    float *dst = q_out + (n * n_head + h) * HD;
+    *reinterpret_cast<f4v *>(dst + a) = x;
+    *reinterpret_cast<f4v *>(dst + b) = y;
+    return;
+  }
+  if (p.block < 0) return;
+  T *to = static_cast<T *>(c.k) + (p.block + h * per) * (kBlk * HD);
+  const typename Vec<T>::four xs = {rounded<T>(x[0]), rounded<T>(x[1]), rounded<T>(x[2]),
+                                    rounded<T>(x[3])};
+  const typename Vec<T>::four ys = {rounded<T>(y[0]), rounded<T>(y[1]), rounded<T>(y[2]),
+                                    rounded<T>(y[3])};
+  *reinterpret_cast<typename Vec<T>::four *>(to + k_place<HD>(p.s, a)) = xs;
+  *reinterpret_cast<typename Vec<T>::four *>(to + k_place<HD>(p.s, b)) = ys;
+}
+
+// Neox rotation of dimensions that are no multiple of 8: a thread a pair of one head, for
+// the queries and keys (the values go as above).
+template <int HD, typename T>
+__global__ void __launch_bounds__(256)
+    k_paged_append_pairs(const float *q, const float *__restrict__ k, float *q_out, int n_head,
+                         int n_rot, const float *__restrict__ cos_t,
+                         const float *__restrict__ sin_t, int64_t n_pos, PagedTable tab,
+                         aq_paged c) {
 #pragma clang fp contract(off)
   const int64_t n = blockIdx.x;
-  const int64_t pos = tab.pos[n], seq = tab.seq ? tab.seq[n] : n;
-  if (pos < 0 || (n_rot && pos >= n_pos)) return;
-  const int64_t slot = pos - tab.start, blk = block_of(c, tab, seq, slot);
-  const int s = (int)(slot & (kBlk - 1)), half = n_rot / 2, pairs = HD / 2;
-  const int heads = (q ? n_head : 0) + c.n_kv;
-  for (int j = threadIdx.x; j < heads * pairs; j += 256) {
-    int h = j / pairs;
-    const int i = j % pairs;
+  const Place p = place_of(c, tab, n);
+  if (p.pos < 0 || p.pos >= n_pos) return;
+  const int half = n_rot / 2, heads = (q ? n_head : 0) + c.n_kv;
+  for (int j = threadIdx.x; j < heads * (HD / 2); j += 256) {
+    int h = j / (HD / 2);
+    const int i = j % (HD / 2);
     const bool is_k = h < c.n_kv;
     if (!is_k) h -= c.n_kv;
-    if (is_k && blk < 0) continue;
-    int a, b;
-    if (i < half) {
-      a = neox ? i : 2 * i;
-      b = neox ? i + half : 2 * i + 1;
-    } else {
-      a = n_rot + 2 * (i - half);
-      b = a + 1;
-    }
+    const int a = i < half ? i : n_rot + 2 * (i - half), b = i < half ? i + half : a + 1;
     const float *src = is_k ? k + (n * c.n_kv + h) * HD : q + (n * n_head + h) * HD;
     float x0 = src[a], x1 = src[b];
     if (i < half) {
-      const float cs = cos_t[pos * half + i], sn = sin_t[pos * half + i];
+      const float cs = cos_t[p.pos * half + i], sn = sin_t[p.pos * half + i];
       const float r0 = x0 * cs - x1 * sn;
       const float r1 = x0 * sn + x1 * cs;
       x0 = r0;
@@ -89,32 +253,66 @@ __global__ void __launch_bounds__(256)
       float *dst = q_out + (n * n_head + h) * HD;
       dst[a] = x0;
       dst[b] = x1;
-      continue;
+    } else if (p.block >= 0) {
+      T *to = static_cast<T *>(c.k) + (p.block + (int64_t)h * (c.page_size / kBlk)) * (kBlk * HD);
+      to[k_place<HD>(p.s, a)] = rounded<T>(x0);
+      to[k_place<HD>(p.s, b)] = rounded<T>(x1);
     }
-    const int64_t at = (blk + (int64_t)h * (c.page_size / kBlk)) * (kBlk * HD);
-    T *kp = static_cast<T *>(c.k) + at, *vp = static_cast<T *>(c.v) + at;
-    const float *vs = v + (n * c.n_kv + h) * HD;
-    kp[k_place<HD>(s, a)] = rounded<T>(x0);
-    kp[k_place<HD>(s, b)] = rounded<T>(x1);
-    vp[v_place(s, a)] = rounded<T>(vs[a]);
-    vp[v_place(s, b)] = rounded<T>(vs[b]);
   }
 }
 
 // ---- read-back -------------------------------------------------------------------
+// A thread a unit: 8 dimensions of a key, or four of four tokens' values.
 template <int HD>
 __global__ void __launch_bounds__(256)
-    k_paged_read(PagedTable tab, aq_paged c, uint16_t *__restrict__ ko, uint16_t *__restrict__ vo) {
-  const int64_t n = blockIdx.x;
-  const int64_t pos = tab.pos[n], seq = tab.seq ? tab.seq[n] : n;
-  const int64_t slot = pos - tab.start, blk = pos < 0 ? -1 : block_of(c, tab, seq, slot);
-  const int s = (int)(slot & (kBlk - 1));
-  for (int j = threadIdx.x; j < c.n_kv * HD; j += 256) {
-    const int h = j / HD, d = j % HD;
-    const int64_t at = (blk + (int64_t)h * (c.page_size / kBlk)) * (kBlk * HD);
-    ko[n * c.n_kv * HD + j] = blk < 0 ? 0 : static_cast<uint16_t *>(c.k)[at + k_place<HD>(s, d)];
-    vo[n * c.n_kv * HD + j] = blk < 0 ? 0 : static_cast<uint16_t *>(c.v)[at + v_place(s, d)];
+    k_paged_read(int64_t N, PagedTable tab, aq_paged c, uint16_t *__restrict__ ko,
+                 uint16_t *__restrict__ vo, unsigned per_token, unsigned per_group,
+                 unsigned n_k) {
+  typedef uint16_t four __attribute__((ext_vector_type(4)));
+  const int64_t per = c.page_size / kBlk;
+  if (blockIdx.x < n_k) {
+    const int64_t n = blockIdx.x / per_token;
+    const int u = (int)(blockIdx.x % per_token) * 256 + threadIdx.x;
+    if (u >= c.n_kv * (HD / 8)) return;
+    const int h = u / (HD / 8), d = 8 * (u % (HD / 8));
+    const Place p = place_of(c, tab, n);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (p.block >= 0)
+      x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(c.k) +
+                                           (p.block + h * per) * (kBlk * HD) +
+                                           k_place<HD>(p.s, d));
+    *reinterpret_cast<uint4 *>(ko + (n * c.n_kv + h) * HD + d) = x;
+    return;
   }
+  const unsigned b = blockIdx.x - n_k;
+  const int u = (int)(b % per_group) * 256 + threadIdx.x;
+  if (u >= c.n_kv * (HD / 4)) return;
+  const int h = u / (HD / 4), d = 4 * (u % (HD / 4));
+  const int64_t first = 4 * (int64_t)(b / per_group) - lead_of(tab);
+  const Group g = group_of(c, tab, N, b / per_group, INT64_MAX);
+  const uint16_t *vp = static_cast<const uint16_t *>(c.v);
+  four x[4];
+  if (g.together) {
+    const uint16_t *from = vp + (g.p[0].block + h * per) * (kBlk * HD) + v_place(g.p[0].s, d);
+    four y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const four *>(from + 8 * e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = four{y[0][i], y[1][i], y[2][i], y[3][i]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = four{0, 0, 0, 0};
+      if (!g.in[i]) continue;
+      const uint16_t *from = vp + (g.p[i].block + h * per) * (kBlk * HD) + v_place(g.p[i].s, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] = from[8 * e];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (first + i >= 0 && first + i < N)
+      *reinterpret_cast<four *>(vo + ((first + i) * c.n_kv + h) * HD + d) = x[i];
 }
 
 // ---- attention -----------------------------------------------------------------
@@ -129,7 +327,6 @@ __global__ void __launch_bounds__(256)
 // Weights are P = 2^(z - m + 14), m the running maximum rounded up to a whole
 // number, so that rescaling is exact and rare, and the pieces hold 22 bits of what
 // counts.  The sum of the weights is kept per lane, in fp32.
-typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef unsigned int u4v __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -322,11 +519,11 @@ __device__ __forceinline__ u4v only_first(u4v v, int rem) {
 // of a list of pages, one a lane; -1: absent.
 __device__ __forceinline__ int64_t lane_block(const aq_paged &c, const int32_t *pages, int h,
                                               int64_t b, int64_t end) {
-  const int per = c.page_size / kBlk;
+  const uint32_t per = c.page_size / kBlk, page = (uint32_t)b / per;
   if (b >= end) return -1;
-  const int64_t id = pages[b / per];
+  const int64_t id = pages[page];
   if (id < 0 || id >= c.n_pages) return -1;
-  return (id * c.n_kv + h) * per + b % per;
+  return (id * c.n_kv + h) * per + ((uint32_t)b - page * per);
 }
 __device__ __forceinline__ int64_t of_lane(int64_t v, int lane) {
   const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
@@ -759,19 +956,36 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
                              int64_t N, int n_head, int n_rot, int neox, const float *cos_t,
                              const float *sin_t, int64_t n_pos, const PagedTable &tab,
                              const aq_paged &c, hipStream_t s) {
+  if (n_rot == 0) neox = 0, n_pos = INT64_MAX;  // (no table, and no end to it)
+  const bool by_pairs = neox && n_rot % 8 != 0;
+  const int64_t heads = (q ? n_head : 0) + c.n_kv;
+  const int64_t per_token = (heads * c.head_dim / 8 + 255) / 256;
+  const int64_t per_group = ((int64_t)c.n_kv * c.head_dim / 4 + 255) / 256;
+  const int64_t n_qk = by_pairs ? 0 : N * per_token, n_v = (N + 6) / 4 * per_group;
+  if (n_qk + n_v > INT32_MAX || N > INT32_MAX) return hipErrorInvalidValue;
   by_shape(c, [&](auto hd, auto t) {
-    hipLaunchKernelGGL((k_paged_append<decltype(hd)::value, decltype(t)>), dim3((unsigned)N),
-                       dim3(256), 0, s, q, k, v, q_out, n_head, n_rot, neox, cos_t, sin_t, n_pos,
-                       tab, c);
+    constexpr int HD = decltype(hd)::value;
+    typedef decltype(t) T;
+    if (by_pairs)
+      hipLaunchKernelGGL((k_paged_append_pairs<HD, T>), dim3((unsigned)N), dim3(256), 0, s, q, k,
+                         q_out, n_head, n_rot, cos_t, sin_t, n_pos, tab, c);
+    hipLaunchKernelGGL((k_paged_append<HD, T>), dim3((unsigned)(n_qk + n_v)), dim3(256), 0, s, q,
+                       k, v, q_out, N, n_head, n_rot, neox, cos_t, sin_t, n_pos, tab, c,
+                       (unsigned)per_token, (unsigned)per_group, (unsigned)n_qk);
   });
   return hipGetLastError();
 }
 
 hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c, void *k, void *v,
                              hipStream_t s) {
+  const int64_t per_token = ((int64_t)c.n_kv * c.head_dim / 8 + 255) / 256;
+  const int64_t per_group = ((int64_t)c.n_kv * c.head_dim / 4 + 255) / 256;
+  const int64_t n_k = N * per_token, n_v = (N + 6) / 4 * per_group;
+  if (n_k + n_v > INT32_MAX) return hipErrorInvalidValue;
   by_shape(c, [&](auto hd, auto) {
-    hipLaunchKernelGGL((k_paged_read<decltype(hd)::value>), dim3((unsigned)N), dim3(256), 0, s,
-                       tab, c, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v));
+    hipLaunchKernelGGL((k_paged_read<decltype(hd)::value>), dim3((unsigned)(n_k + n_v)), dim3(256),
+                       0, s, N, tab, c, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v),
+                       (unsigned)per_token, (unsigned)per_group, (unsigned)n_k);
   });
   return hipGetLastError();
 }

@@ -566,7 +566,7 @@ int aq_kv8_read(const aq_kv8 *cache, int64_t start, int64_t n, float *k, float *
  * The caller allocates k and v (aq_paged_sizes; device memory, 16-byte aligned, no
  * initial content needed).  Calls on one cache are the caller's to order.  q, k, v
  * and outputs are 16-byte aligned too (AQ_ERR_VALUE).  head_dim 64, 128 or 256,
- * page_size a multiple of 32. */
+ * page_size a multiple of 32; width * page_size and start below 2^31 (AQ_ERR_VALUE). */
 typedef struct aq_paged {
   void *k, *v;      /* [n_pages][n_kv][page_size / 32][32 * head_dim] (aq_paged.hip) */
   int64_t n_pages;
