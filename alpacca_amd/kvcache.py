@@ -53,6 +53,15 @@ def check_heads(n_head: int, n_kv: int, head_dim: int) -> None:
                          f"got {n_head} for {n_kv}")
 
 
+def check_paged_heads(n_head: int, n_kv: int, head_dim: int) -> None:
+    """ValueError for heads that the paged cache's attention does not take."""
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"the paged KV cache takes head_dim {HEAD_DIMS}, got {head_dim}")
+    if n_kv < 1 or n_head < 1 or n_head % n_kv or n_head // n_kv > MAX_GROUP:
+        raise ValueError(f"the paged KV cache takes 1 to {MAX_GROUP} query heads per kv head, "
+                         f"got {n_head} for {n_kv}")
+
+
 class _Heads:
     """What the caches' calls have in common: their arguments, rows of heads of
     head_dim on the cache's device."""
@@ -448,4 +457,5 @@ class PagedKVCache(_Heads):
         return k, v
 
 
-__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "PagedKVCache", "QuantKVCache", "check_heads"]
+__all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "PagedKVCache", "QuantKVCache", "check_heads",
+           "check_paged_heads"]

@@ -13,7 +13,10 @@ Mirrors the reference's ``Model`` where it touches the hot path:
 * ``generate_greedy(prompt, n)`` - ``n`` greedy tokens after the prompt
   (argmax of the logits, tensor.py:187-194, fed back as the next token),
   with the reference sampler's repetition penalty, or presence and frequency
-  penalties, per-token biases and a mask of allowed tokens (logits.py).
+  penalties, per-token biases and a mask of allowed tokens (logits.py);
+* ``generate_samples(prompt, n, n_seq)`` - several sampled continuations of one
+  prompt (alpacca/sample.py:44-76 for each token), drawn together: the prompt's
+  keys and values are held once, in pages that all of them read.
 
 ``Model(..., kv_dtype="q8")`` keeps the KV cache in 8 bits (kvcache.py): a
 quarter of the fp32 cache's bytes, which the reference keeps.
@@ -38,8 +41,8 @@ import numpy as np
 
 from . import _lib
 from .kvcache import BLOCK as KV_BLOCK
-from .kvcache import QuantKVCache, check_heads
-from .logits import adjust_logits, pack_mask
+from .kvcache import PagedKVCache, QuantKVCache, check_heads, check_paged_heads
+from .logits import adjust_logits, pack_mask, sample_logits, sampling_params
 from .qmatrix import (DENSE_DTYPES, MIXABLE_DTYPES, DenseMatrix, QuantMatrix,
                       interleave_rows, matvec_fused_device, matvec_multi_device,
                       pair_rows_supported)
@@ -454,13 +457,48 @@ class Model:
             self._bb = b
         return b
 
-    def _enqueue_prefill(self, tokens: list[int]) -> None:
+    def _enqueue_batch_layers(self, b: dict, T: int, attend, prec: str) -> None:
+        """The layers of the batched step for T rows whose embeddings are in X:
+        RMSNorm of all rows, matmul_t for every projection, attend(layer), which
+        takes Q, K, V (not rotated) to A, SwiGLU, residual adds."""
+        hp, lib, s = self.hp, _lib.load(), self.stream.cuda_stream
+        sv, chk = ctypes.c_void_p(s), _lib.check
+        p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        X, H, O, Q, K, V, A, G, U, S = (b[k] for k in "XHOQKVAGUS")
+        GU = b["GU"]
+        eps, n_layers = ctypes.c_float(hp.rms_eps), len(self.layers)
+        # the first RMSNorm on its own; each later one shares a launch
+        # with the residual add before it (aq_add_rmsnorm, the same bits)
+        chk(lib.aq_rmsnorm(p(X), p(self.layers[0]["attn_norm"]), T, hp.n_embd, eps, p(H), sv))
+        for li, ly in enumerate(self.layers):
+            for role, out in (("attn_q", Q), ("attn_k", K), ("attn_v", V)):
+                ly[role].matmul_t_device(H.data_ptr(), T, out.data_ptr(), s, prec)
+                if ly[role + ".bias"] is not None:  # q + bq over the batch
+                    chk(lib.aq_add_rows(p(out), p(ly[role + ".bias"]), T, out.shape[1], sv))
+            attend(li)
+            ly["attn_output"].matmul_t_device(A.data_ptr(), T, O.data_ptr(), s, prec)
+            chk(lib.aq_add_rmsnorm(p(X), p(O), p(ly["ffn_norm"]), T, hp.n_embd, eps, p(H), sv))
+            if ly["ffn_gate_up"] is not None:  # (gate, up) pairs from one product
+                ly["ffn_gate_up"].matmul_t_swiglu_device(H.data_ptr(), T, GU.data_ptr(),
+                                                         S.data_ptr(), s, prec)
+            else:
+                ly["ffn_gate"].matmul_t_device(H.data_ptr(), T, G.data_ptr(), s, prec)
+                ly["ffn_up"].matmul_t_device(H.data_ptr(), T, U.data_ptr(), s, prec)
+                chk(lib.aq_swiglu(p(G), p(U), T * hp.n_ff, p(S), sv))
+            ly["ffn_down"].matmul_t_device(S.data_ptr(), T, O.data_ptr(), s, prec)
+            if li + 1 < n_layers:
+                chk(lib.aq_add_rmsnorm(p(X), p(O), p(self.layers[li + 1]["attn_norm"]), T,
+                                       hp.n_embd, eps, p(H), sv))
+            else:
+                chk(lib.aq_add(p(X), p(O), T * hp.n_embd, sv))
+
+    def _enqueue_prefill(self, tokens: list[int], store=None) -> None:
         """The batched step over chunks of prefill_chunk tokens at positions
-        n_past..: RMSNorm of all rows, matmul_t for every projection (float32
-        accuracy unless prefill_precision says otherwise), RoPE + KV store of the
-        chunk, causal attention of its queries, SwiGLU, residual adds; then
-        the head on the last token only, whose logits the stream leaves in
-        self.logits."""
+        n_past..: the layers (float32 accuracy unless prefill_precision says
+        otherwise) with RoPE + KV store of the chunk and causal attention of its
+        queries; then the head on the last token only, whose logits the stream
+        leaves in self.logits.  store(layer, pos0, T): called with a chunk's keys
+        and values in K and V, before their rotation."""
         hp, torch = self.hp, self.torch
         if self.n_past + len(tokens) > self.n_ctx:
             raise RuntimeError(f"context window full ({self.n_ctx} tokens)")
@@ -469,58 +507,34 @@ class Model:
         lib, s = _lib.load(), self.stream.cuda_stream
         sv, chk = ctypes.c_void_p(s), _lib.check
         p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
-        prec = self.prefill_precision
         neox = 1 if hp.rope_style == "neox" else 0
         chunk = self.prefill_chunk
         b = self._batch_buffers(min(chunk, len(tokens)))
-        X, H, O, Q, K, V, A, G, U, S = (b[k] for k in "XHOQKVAGUS")
-        GU = b["GU"]
-        eps, n_layers = ctypes.c_float(hp.rms_eps), len(self.layers)
+        X, Q, K, V, A = (b[k] for k in "XQKVA")
+
+        def attend(li):
+            if store is not None:
+                store(li, pos0, T)
+            if self.kv8:
+                cache = self.kv8[li].handle
+                chk(lib.aq_rope_kv8(p(Q), p(K), p(V), p(Q), T, hp.n_head, hp.n_rot, neox,
+                                    p(self.rope_cos), p(self.rope_sin), None, pos0, cache, sv))
+                chk(lib.aq_attention_kv8(p(Q), cache, T, hp.n_head, None, pos0, p(A), sv))
+                return
+            kc, vc = self.kv[li, 0], self.kv[li, 1]
+            chk(lib.aq_rope_kv(p(Q), p(K), p(V), T, hp.n_head, hp.n_kv, hp.head_dim, hp.n_rot,
+                               neox, p(self.rope_cos), p(self.rope_sin), None, pos0, self.n_ctx,
+                               p(kc), p(vc), sv))
+            chk(lib.aq_attention_batch(p(Q), p(kc), p(vc), T, hp.n_head, hp.n_kv, hp.head_dim,
+                                       self.n_ctx, None, pos0, p(A), sv))
+
         with torch.cuda.stream(self.stream):
             for c0 in range(0, len(tokens), chunk):
                 toks = tokens[c0:c0 + chunk]
                 T, pos0 = len(toks), self.n_past
                 b["ids"][:T].copy_(torch.tensor(toks, dtype=torch.int64))
                 self.tok_embd.rows_at_device(b["ids"].data_ptr(), T, X.data_ptr(), s)
-                # the first RMSNorm on its own; each later one shares a launch
-                # with the residual add before it (aq_add_rmsnorm, the same bits)
-                chk(lib.aq_rmsnorm(p(X), p(self.layers[0]["attn_norm"]), T, hp.n_embd, eps,
-                                   p(H), sv))
-                for li, ly in enumerate(self.layers):
-                    for role, out in (("attn_q", Q), ("attn_k", K), ("attn_v", V)):
-                        ly[role].matmul_t_device(H.data_ptr(), T, out.data_ptr(), s, prec)
-                        if ly[role + ".bias"] is not None:  # q + bq over the batch
-                            chk(lib.aq_add_rows(p(out), p(ly[role + ".bias"]), T,
-                                                out.shape[1], sv))
-                    if self.kv8:
-                        cache = self.kv8[li].handle
-                        chk(lib.aq_rope_kv8(p(Q), p(K), p(V), p(Q), T, hp.n_head, hp.n_rot, neox,
-                                            p(self.rope_cos), p(self.rope_sin), None, pos0, cache,
-                                            sv))
-                        chk(lib.aq_attention_kv8(p(Q), cache, T, hp.n_head, None, pos0, p(A), sv))
-                    else:
-                        kc, vc = self.kv[li, 0], self.kv[li, 1]
-                        chk(lib.aq_rope_kv(p(Q), p(K), p(V), T, hp.n_head, hp.n_kv, hp.head_dim,
-                                           hp.n_rot, neox, p(self.rope_cos), p(self.rope_sin),
-                                           None, pos0, self.n_ctx, p(kc), p(vc), sv))
-                        chk(lib.aq_attention_batch(p(Q), p(kc), p(vc), T, hp.n_head, hp.n_kv,
-                                                   hp.head_dim, self.n_ctx, None, pos0, p(A), sv))
-                    ly["attn_output"].matmul_t_device(A.data_ptr(), T, O.data_ptr(), s, prec)
-                    chk(lib.aq_add_rmsnorm(p(X), p(O), p(ly["ffn_norm"]), T, hp.n_embd, eps,
-                                           p(H), sv))
-                    if ly["ffn_gate_up"] is not None:  # (gate, up) pairs from one product
-                        ly["ffn_gate_up"].matmul_t_swiglu_device(H.data_ptr(), T, GU.data_ptr(),
-                                                                 S.data_ptr(), s, prec)
-                    else:
-                        ly["ffn_gate"].matmul_t_device(H.data_ptr(), T, G.data_ptr(), s, prec)
-                        ly["ffn_up"].matmul_t_device(H.data_ptr(), T, U.data_ptr(), s, prec)
-                        chk(lib.aq_swiglu(p(G), p(U), T * hp.n_ff, p(S), sv))
-                    ly["ffn_down"].matmul_t_device(S.data_ptr(), T, O.data_ptr(), s, prec)
-                    if li + 1 < n_layers:
-                        chk(lib.aq_add_rmsnorm(p(X), p(O), p(self.layers[li + 1]["attn_norm"]),
-                                               T, hp.n_embd, eps, p(H), sv))
-                    else:
-                        chk(lib.aq_add(p(X), p(O), T * hp.n_embd, sv))
+                self._enqueue_batch_layers(b, T, attend, self.prefill_precision)
                 self.n_past += T
                 self._kv_end = self.n_past
             self.x.copy_(X[T - 1])
@@ -720,6 +734,134 @@ class Model:
         self.n_past = self._kv_end = n_p + n_gen - 1
         self.cached_ids = list(prompt) + out[:-1]
         return out
+
+    def generate_samples(self, prompt: list[int], n_gen: int, n_seq: int = 1,
+                         temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
+                         kv_dtype: str = "f16", page_size: int = 64, graph: bool = True,
+                         logit_bias: dict | None = None, allowed=None,
+                         timing: dict | None = None) -> list[list[int]]:
+        """n_seq sampled continuations of n_gen tokens each: token i of sequence
+        r is drawn with the random number U[i, r], U = torch.rand(n_gen, n_seq,
+        dtype=torch.float64) of a CPU generator seeded with `seed`, and
+        temperature, top_k, top_p and min_p (a number for all sequences, or one for
+        each) as logits.sample_logits has them, after logit_bias and `allowed`
+        (as in generate_greedy).
+
+        Starts from an empty cache and runs the prompt as generate_greedy does;
+        its keys and values also go into pages of kv_dtype ("f16" or "bf16") that
+        all sequences read, beside pages of their own for what they add.  The steps
+        run all sequences at once, as replays of one captured step (graph=True).
+        Leaves the model's own cache with the prompt.  `timing` receives gen_ms (of
+        the n_gen - 1 steps after the first token), steps and prefill_ms.
+        RuntimeError (and an empty cache) where a row of logits had none above
+        -inf."""
+        torch, hp = self.torch, self.hp
+        if not prompt or n_gen < 1 or n_seq < 1:
+            raise ValueError("need a non-empty prompt, n_gen >= 1 and n_seq >= 1")
+        if kv_dtype not in ("f16", "bf16"):
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r} (f16, bf16)")
+        check_paged_heads(hp.n_head, hp.n_kv, hp.head_dim)
+        n_p = len(prompt)
+        if n_p + n_gen - 1 > self.n_ctx:
+            raise RuntimeError(f"context window full ({self.n_ctx} tokens)")
+        if min(prompt) < 0 or max(prompt) >= hp.n_vocab:
+            raise IndexError("row index out of range")
+        params = sampling_params(n_seq, temperature, top_k, top_p, min_p, device=self.dev)
+        adjust, _ = self._adjustment(0.0, 0.0, logit_bias, allowed)
+        lib, s, chk = _lib.load(), self.stream.cuda_stream, _lib.check
+        sv = ctypes.c_void_p(s)
+        p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        neox = 1 if hp.rope_style == "neox" else 0
+        dtype = torch.float16 if kv_dtype == "f16" else torch.bfloat16
+        U = torch.rand(n_gen, n_seq, generator=torch.Generator().manual_seed(seed),
+                       dtype=torch.float64)
+        self.reset()
+        self.stream.wait_stream(torch.cuda.current_stream(self.dev))
+        with torch.cuda.stream(self.stream):
+            # made, used and freed on self.stream
+            U = U.to(self.dev)
+            n_pre, width = -(-n_p // page_size), -(-(n_gen - 1) // page_size)
+            pages = torch.arange(n_pre + n_seq * width, dtype=torch.int32, device=self.dev)
+            prefix, table = pages[:n_pre], pages[n_pre:].view(n_seq, width)
+            caches = [PagedKVCache(hp.n_kv, pages.numel(), hp.head_dim, page_size, dtype, self.dev)
+                      for _ in self.layers]
+            at = torch.arange(n_p, device=self.dev)  # the prompt's positions, all of row 0
+            row = torch.zeros_like(at)
+            pos = torch.full((n_seq,), n_p, dtype=torch.int64, device=self.dev)
+            tok = torch.zeros(n_seq, dtype=torch.int64, device=self.dev)
+            hist = torch.zeros((n_gen, n_seq), dtype=torch.int64, device=self.dev)
+            u = U[0].clone()
+            logits = torch.empty((n_seq, hp.n_vocab), dtype=torch.float32, device=self.dev)
+        b = self._batch_buffers(n_seq)
+        size = ctypes.c_size_t()
+        chk(lib.aq_attention_paged_scratch(caches[0].handle, n_seq, hp.n_head, width, n_p,
+                                           ctypes.byref(size)))
+        with torch.cuda.stream(self.stream):
+            scratch = torch.empty(size.value, dtype=torch.uint8, device=self.dev)
+
+        def store(li, pos0, T):
+            bb = self._bb
+            chk(lib.aq_rope_paged(None, p(bb["K"]), p(bb["V"]), None, T, hp.n_head, hp.n_rot, neox,
+                                  p(self.rope_cos), p(self.rope_sin), self.n_ctx, p(prefix), 1,
+                                  n_pre, p(row), at[pos0:].data_ptr(), 0, caches[li].handle, sv))
+
+        def attend(li):
+            chk(lib.aq_rope_paged(p(b["Q"]), p(b["K"]), p(b["V"]), p(b["Q"]), n_seq, hp.n_head,
+                                  hp.n_rot, neox, p(self.rope_cos), p(self.rope_sin), self.n_ctx,
+                                  p(table), n_seq, width, None, p(pos), n_p, caches[li].handle,
+                                  sv))
+            chk(lib.aq_attention_paged(p(b["Q"]), caches[li].handle, n_seq, hp.n_head, p(table),
+                                       n_seq, width, None, p(pos), p(prefix), n_pre, n_p,
+                                       p(scratch), size.value, p(b["A"]), sv))
+
+        def choose():
+            if adjust is not None:
+                adjust_logits(logits, out=logits, **adjust)
+            sample_logits(logits, u, params, out=tok)
+
+        def step():
+            self.tok_embd.rows_at_device(tok.data_ptr(), n_seq, b["X"].data_ptr(), s)
+            self._enqueue_batch_layers(b, n_seq, attend, "auto")
+            chk(lib.aq_rmsnorm(p(b["X"]), p(self.out_norm), n_seq, hp.n_embd,
+                               ctypes.c_float(hp.rms_eps), p(b["H"]), sv))
+            self.output.matmul_t_device(b["H"].data_ptr(), n_seq, logits.data_ptr(), s, "auto")
+            choose()
+
+        run = step
+        if graph and n_gen > 1:  # captured first: what its eager run stores and chooses
+            g = self._capture(step)  # is overwritten below
+            run = g.replay
+        import time
+        t_pf = time.perf_counter()
+        try:
+            self._enqueue_prefill(list(prompt), store)
+            if timing is not None:
+                self.stream.synchronize()
+                t_pf = time.perf_counter() - t_pf
+            with torch.cuda.stream(self.stream):
+                logits.copy_(self.logits.expand_as(logits))
+                choose()
+                hist[0].copy_(tok)
+                begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+                begin.record(self.stream)
+                for i in range(1, n_gen):
+                    u.copy_(U[i])
+                    run()
+                    hist[i].copy_(tok)
+                    pos.add_(1)
+                end.record(self.stream)
+        finally:  # the buffers and the graph are in use until here
+            self.stream.synchronize()
+        if timing is not None:
+            timing["gen_ms"] = begin.elapsed_time(end)
+            timing["steps"] = n_gen - 1
+            timing["prefill_ms"] = t_pf * 1e3  # host wall clock, synchronized
+        out = hist.cpu()
+        if bool((out < 0).any()):
+            self.reset()
+            raise RuntimeError("a row of logits had none above -inf at generated token "
+                               f"{int((out < 0).any(1).nonzero()[0])}")
+        return out.T.tolist()
 
     def _adjustment(self, presence: float, frequency: float, bias, allowed) -> tuple:
         """adjust_logits' arguments for one row but the window and penalties
