@@ -535,10 +535,10 @@ __device__ __forceinline__ int64_t of_lane(int64_t v, int lane) {
 // block b, values(b, j) that of its dimensions 16 j ..  Products of different sums
 // follow one another: one that adds to the last one's result would wait for it.
 // scored() runs when the scores' products are on their way.
-template <int HD, typename T, int NB, bool TAIL, class K, class V, class Next>
-__device__ __forceinline__ void attend_block(const QRow<HD, T> &q, RowState<HD> &st,
-                                             const int (&rem)[NB], K &&keys, V &&values,
-                                             Next &&scored) {
+template <int HD, typename T, int NB, bool TAIL, class K, class Next>
+__device__ __forceinline__ void score_block(const QRow<HD, T> &q, RowState<HD> &st,
+                                            const int (&rem)[NB], K &&keys, Next &&scored,
+                                            u4v (&w)[NB][Ops<T>::NP]) {
   constexpr int KS = HD / 32, NP = Ops<T>::NP;
   f4v sc[NB][2];
 #pragma unroll
@@ -555,8 +555,15 @@ __device__ __forceinline__ void attend_block(const QRow<HD, T> &q, RowState<HD> 
         sc[i >> 1][i & 1] = Ops<T>::mfma(k[i], q.piece[p][ks], sc[i >> 1][i & 1]);
   }
   scored();
-  u4v w[NB][NP];
   weigh<HD, T, NB, TAIL>(sc, q.back, rem, st, w);
+}
+template <int HD, typename T, int NB, bool TAIL, class K, class V, class Next>
+__device__ __forceinline__ void attend_block(const QRow<HD, T> &q, RowState<HD> &st,
+                                             const int (&rem)[NB], K &&keys, V &&values,
+                                             Next &&scored) {
+  constexpr int NP = Ops<T>::NP;
+  u4v w[NB][NP];
+  score_block<HD, T, NB, TAIL>(q, st, rem, keys, scored, w);
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -574,14 +581,29 @@ __device__ __forceinline__ void attend_block(const QRow<HD, T> &q, RowState<HD> 
     }
 }
 
+// The tokens whose rows share a tile: row j is token j / G's, which sees `len` positions.
+struct Tokens {
+  int count, G;
+  int least;  // of their lengths
+  int mine;   // the lane's row's
+  const int64_t *pos;
+  int64_t start, room;
+  __device__ __forceinline__ int len(int t) const {
+    const int64_t n = load_const(pos + t) - start + 1;
+    return (int)(n < room ? n : room);
+  }
+};
+
 // One tile of rows against blocks b0 + wave, b0 + wave + 4, .. below b1 of a list of
-// pages that holds len positions, straight from memory.  A wave's next keys are on
-// their way while it weighs the present ones.
+// pages, straight from memory; len: the largest of the tokens' lengths.  A wave's next
+// keys are on their way while it weighs the present ones.  In blocks where a token's
+// positions end, each token's sums take its own values alone: what lies behind them may
+// be an infinity or a NaN, which a weight of 0 would not undo.
 template <int HD, typename T>
 __device__ __forceinline__ void attend_strided(const aq_paged &c, const int32_t *pages, int h,
-                                               int64_t b0, int64_t b1, int64_t len,
+                                               int64_t b0, int64_t b1, const Tokens &tok,
                                                const QRow<HD, T> &q, RowState<HD> &st) {
-  constexpr int KS = HD / 32, DT = HD / 16;
+  constexpr int KS = HD / 32, DT = HD / 16, NP = Ops<T>::NP;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u4v *kp = static_cast<const u4v *>(c.k) + lane, *vp = static_cast<const u4v *>(c.v) + lane;
   for (int64_t base = b0 + wave; base < b1; base += 4 * 64) {
@@ -595,8 +617,7 @@ __device__ __forceinline__ void attend_strided(const aq_paged &c, const int32_t 
     for (int j = 0; j < 2 * KS; ++j) k[j] = kp[at + 64 * j];
     while (left) {
       left &= left - 1;
-      const int64_t after = len - (base + 4 * i) * kBlk;
-      const int rem[1] = {after < kBlk ? (int)after : kBlk};
+      const int first = (int)(base + 4 * i) * kBlk;  // the block's first position
 #pragma unroll
       for (int j = 0; j < DT; ++j) v[j] = vp[at + 64 * j];
       auto keys = [&](int, int j) { return k[j]; };
@@ -608,8 +629,28 @@ __device__ __forceinline__ void attend_strided(const aq_paged &c, const int32_t 
 #pragma unroll
         for (int j = 0; j < 2 * KS; ++j) k[j] = kp[at + 64 * j];
       };
-      if (rem[0] < kBlk) attend_block<HD, T, 1, true>(q, st, rem, keys, values, next);
-      else attend_block<HD, T, 1, false>(q, st, rem, keys, values, next);
+      if (first + kBlk <= tok.least) {
+        const int rem[1] = {kBlk};
+        attend_block<HD, T, 1, false>(q, st, rem, keys, values, next);
+        continue;
+      }
+      const int rem[1] = {tok.mine - first};
+      u4v w[1][NP];
+      score_block<HD, T, 1, true>(q, st, rem, keys, next, w);
+#pragma unroll 1
+      for (int t = 0; t < tok.count; ++t) {
+        const int len = tok.count == 1 ? tok.least : tok.len(t);
+        if (len <= first) continue;
+        const bool its = (lane & 15) / tok.G == t || tok.count == 1;
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+          const u4v x = only_first(v[j], len - first);
+          f4v o = st.o[j];
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) o = Ops<T>::mfma(x, w[0][p], o);
+          st.o[j] = its ? o : st.o[j];
+        }
+      }
     }
   }
 }
@@ -721,7 +762,8 @@ __device__ __forceinline__ void pick_unit(const PagedPlan &p, unsigned units, un
 }
 
 // Items of the prefix: a split, a group of rows and a kv head; own ones: a split, a kv
-// head and a row (a row that ends inside the prefix has that part of it as its own).
+// head and a row, or the rows of neighbours of one sequence (a row that ends inside the
+// prefix has that part of it as its own).
 // Waves that share rows have their states merged through LDS.
 template <int HD, typename T, int TW>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
@@ -737,6 +779,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
   int h, split;
   int64_t len, b0, b1;
   const int32_t *pages;
+  Tokens tok = {1, G, 0, 0, nullptr, 0, 0};
   const int rows = (int)N * G;  // of a kv head (N * n_head is below 2^24)
   int row0 = 0;                 // of the group
   int n = 0;
@@ -757,16 +800,46 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     h = (int)(item % c.n_kv);
     n = (int)(item / c.n_kv);
     row0 = n * G;
-    const int64_t pos = tab.pos[n], seq = tab.seq ? tab.seq[n] : n;
+    const int64_t pos = load_const(tab.pos + n), seq = tab.seq ? load_const(tab.seq + n) : n;
+    const int64_t room = tab.width * c.page_size;
+    // (the 64 tokens about it, below, loaded at once with its own)
+    const bool share = tab.seq && G <= 8;
+    const int around = n & ~63;
+    int64_t lp = -1, ls = -1;
+    if (share && around + lane < (int)N) lp = tab.pos[around + lane], ls = tab.seq[around + lane];
     len = 0;
     pages = nullptr;
     if (pos >= 0 && pos < pre.start) {
       pages = pre.pages;
       len = pos + 1;
+      tok = {1, G, (int)len, (int)len, nullptr, 0, 0};
     } else if (pos >= 0 && seq >= 0 && seq < tab.seqs) {
       pages = tab.pages + seq * tab.width;
-      const int64_t room = tab.width * c.page_size;
       len = pos - tab.start < room ? pos - tab.start + 1 : room;
+      tok = {1, G, (int)len, (int)len, tab.pos + n, tab.start, room};
+      if (share) {
+        // Neighbours of one sequence share a tile: runs inside 64 tokens, 16 / G at a
+        // time, the first of them for all.
+        const int i = n - around, per = 16 / G;
+        const bool joins = lp >= tab.start && lp >= 0 && ls == seq;
+        const uint64_t others = ~__ballot(joins);
+        const uint64_t below = others & ((1ull << i) - 1);
+        const int from = below ? 64 - __builtin_clzll(below) : 0;  // the run's first
+        const uint64_t above = i < 63 ? others >> (i + 1) : 0;
+        const int to = above ? i + 1 + __builtin_ctzll(above) : 64;
+        if ((i - from) % per) return;
+        tok.count = min(per, to - i);
+        // the shortest and the longest of them, and the lane's row's
+        const int64_t its = lp - tab.start + 1 < room ? lp - tab.start + 1 : room;
+        int lo = INT32_MAX, hi = 0;
+        for (int t = 0; t < tok.count; ++t) {
+          const int l = __builtin_amdgcn_readlane((int)its, i + t);
+          lo = min(lo, l), hi = max(hi, l);
+          if (j / G == t) tok.mine = l;
+        }
+        tok.least = lo;
+        len = hi;
+      }
     }
     const int64_t blocks = (len + kBlk - 1) / kBlk;
     int64_t each = (blocks + plan.ss - 1) / plan.ss;
@@ -829,23 +902,28 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
     };
     if constexpr (TW == 1) {
       load_rows();
-      attend_strided<HD, T>(c, pages, h, b0, b1, len, qr, st);
+      const Tokens one = {1, G, (int)len, (int)len, nullptr, 0, 0};
+      attend_strided<HD, T>(c, pages, h, b0, b1, one, qr, st);
     } else {
       attend_staged<HD, T, TW>(c, pages, h, b0, b1, len, lds, qr, st, load_rows);
     }
     write(st, TW, row0, rows);
   } else {
-    if (b0 >= b1 && S != 1) {  // nothing of the row here
-      if ((int)threadIdx.x < G)
-        put_dead<HD>(states + (((int64_t)n * n_head + h * G + threadIdx.x) * S + split) * kState<HD>);
+    const int live = tok.count * G;
+    if (b0 >= b1 && S != 1) {  // nothing of the rows here
+      const int r = threadIdx.x;
+      if (r < live)
+        put_dead<HD>(states + (((int64_t)(n + r / G) * n_head + h * G + r % G) * S + split) *
+                                  kState<HD>);
       return;
     }
     QRow<HD, T> qr;
     RowState<HD> st;
-    qr.load(q + ((int64_t)n * n_head + h * G + (j < G ? j : 0)) * HD, j < G);
+    const int r = j < live ? j : 0;
+    qr.load(q + ((int64_t)(n + r / G) * n_head + h * G + r % G) * HD, j < live);
     st.clear();
-    attend_strided<HD, T>(c, pages, h, b0, b1, len, qr, st);
-    write(st, 1, row0, row0 + G);
+    attend_strided<HD, T>(c, pages, h, b0, b1, tok, qr, st);
+    write(st, 1, row0, row0 + live);
   }
 }
 
@@ -909,33 +987,40 @@ __global__ void __launch_bounds__(256)
     *reinterpret_cast<f4v *>(out + row * HD + d) = o * (sum == 0.f ? 0.f : 1.f / sum);
 }
 
-// Splits.  A row's own positions: until 512 workgroups (two a CU), at least four blocks
-// each.  The prefix: tiles of 16 rows in one workgroup of four waves that share the
+// Splits.  The prefix: tiles of 16 rows in one workgroup of four waves that share the
 // positions up to 16 rows and of two up to 32, bound by memory (8 rows of 4 heads over
 // 100000 positions 89 us in 48 splits of 8 heads, 92 in 32); past that four tiles that
 // share them through LDS, a workgroup a CU: the rows' own positions, bound by memory,
 // run on the same CUs (64 rows of 32 / 8 heads over 8000 and 1024 of their own 68 us;
 // with two workgroups of the prefix a CU, twice the states, 82; the two kinds in
 // turn 75, where rows that own little then wait for a late start: 28 against 25).
+// A row's own positions: what takes the fewest rounds of the workgroups that the GPU
+// holds beside the prefix's, where a workgroup's start and end count as much as four
+// blocks (24 sequences' two rows of 28 / 4 heads over 4001 positions in 8 splits 43 us, in
+// 5 51; before neighbours shared a tile 59 in 3, 44 in 6).
 PagedPlan paged_plan(const aq_paged &c, int64_t N, int n_head, int64_t width, int64_t start) {
-  const int64_t rows = N * (n_head / c.n_kv);
+  const int64_t rows = N * (n_head / c.n_kv), places = c.head_dim == 256 ? 256 : 512;
   PagedPlan p = {};
   p.tw = 1;
-  // `items` workgroups over `blocks` blocks each, split until there are `want`, but at
-  // least `least` blocks a split
-  auto splits = [&](int64_t want, int64_t items, int64_t blocks, int64_t least, int64_t most) {
-    const int64_t s = std::min((want + items - 1) / items, (blocks + least - 1) / least);
-    return (int)std::max<int64_t>(1, std::min(s, most));
-  };
   if (start > 0) {
     p.tw = rows > 32 ? 4 : rows > 16 ? 2 : 1;
     p.groups = (int)((rows + 16 * p.tw - 1) / (16 * p.tw));
-    p.sp = splits(p.tw == 2 ? 512 : 256, (int64_t)p.groups * c.n_kv, (start + kBlk - 1) / kBlk,
-                  p.tw == 4 ? 8 : 4, 48);
+    const int64_t items = (int64_t)p.groups * c.n_kv, want = p.tw == 2 ? 512 : 256;
+    const int64_t blocks = (start + kBlk - 1) / kBlk, least = p.tw == 4 ? 8 : 4;
+    const int64_t s = std::min((want + items - 1) / items, (blocks + least - 1) / least);
+    p.sp = (int)std::max<int64_t>(1, std::min<int64_t>(s, 48));
+    p.pre = (unsigned)(p.sp * items);
   }
-  p.ss = splits(512, N * c.n_kv, width * c.page_size / kBlk, 4, p.sp ? 16 : 64);
-  p.pre = (unsigned)(p.sp * p.groups * c.n_kv);
-  p.own = (unsigned)(p.ss * N * c.n_kv);
+  const int64_t items = N * c.n_kv, blocks = width * c.page_size / kBlk;
+  const int64_t left = std::max<int64_t>(places - p.pre, places / 2);
+  const int64_t most = std::min<int64_t>((blocks + 3) / 4, p.sp ? 16 : 64);
+  p.ss = 1;
+  int64_t best = INT64_MAX;
+  for (int64_t s = 1; s <= std::max<int64_t>(most, 1); ++s) {
+    const int64_t cost = (items * s + left - 1) / left * ((blocks + s - 1) / s + 4);
+    if (cost <= best) best = cost, p.ss = (int)s;
+  }
+  p.own = (unsigned)(p.ss * items);
   return p;
 }
 

@@ -308,6 +308,54 @@ def test_attend_several_tokens(n_head, n_kv, hd, T):
 
 
 @gpu
+@pytest.mark.parametrize("n_head,n_kv,hd", [(8, 2, 64), (14, 2, 128), (3, 3, 128), (8, 1, 256),
+                                            (10, 1, 64)])
+@pytest.mark.parametrize("start", [0, 70])
+def test_attend_runs_of_tokens(n_head, n_kv, hd, start):
+    """Tokens of one sequence beside one another in every manner: runs longer than
+    a tile and across 64 tokens, positions in any order and the same twice, padding
+    and rows that end inside the prefix between them, rows out of the table."""
+    seqs, own = 4, 150
+    c, table, prefix, K, V, KP, VP = setting(n_head, n_kv, hd, 32, "f16", seqs, own, start, seed=hd)
+    g = torch.Generator().manual_seed(n_head + start)
+    N = 150
+    seq = torch.randint(0, seqs, (N,), generator=g).sort().values
+    seq[60:70] = seq[64]  # a run across the border
+    seq[:70:7] = 3
+    seq[100], seq[101], seq[102] = 9, 9, -1
+    pos = start + torch.randint(0, own, (N,), generator=g)
+    pos[30:40] = torch.arange(start + 20, start + 30)
+    pos[41:44] = start + 77
+    pos[50] = -1
+    pos[52] = max(start - 3, 0)
+    q = rand(N, n_head * hd, seed=18)
+    check_attend(c, q, table, pos.cuda(), seq.cuda(), K, V, prefix, start, KP, VP)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n_head,n_kv,hd,T", [(8, 2, 64, 4), (14, 2, 128, 2), (4, 4, 128, 16)])
+def test_tokens_do_not_see_what_comes_after_them(n_head, n_kv, hd, T, dtype):
+    """Infinities and NaNs at a position reach the tokens of its sequence that attend
+    to it, and not those beside them that end before it, in the same block or an
+    earlier one."""
+    own, seqs = 100, 2
+    c, table, _, K, V, _, _ = setting(n_head, n_kv, hd, 32, dtype, seqs, own, 0)
+    pos = torch.tensor([(90 - 5 * t) % 97 for t in range(T)]).repeat(seqs).cuda()
+    seq = torch.arange(seqs).repeat_interleave(T).cuda()
+    q = rand(seqs * T, n_head * hd, seed=19)
+    want = check_attend(c, q, table, pos, seq, K, V)
+    for value in (float("nan"), INF, -INF):
+        at = torch.tensor([88], device="cuda")
+        x = torch.full((1, n_kv * hd), value, device="cuda")
+        c.append(x, x, table[1:], at, seq=torch.zeros_like(at))
+        got = c.attend(q, table, pos, seq=seq)
+        hit = (seq == 1) & (pos >= 88)
+        assert bool(hit.any()) and torch.equal(got[~hit], want[~hit])
+        assert bool((~got[hit].isfinite()).any(1).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attend_long(dtype):
     """Long own pages of few rows, and a long prefix of one row."""
