@@ -62,6 +62,12 @@ def check_paged_heads(n_head: int, n_kv: int, head_dim: int) -> None:
                          f"got {n_head} for {n_kv}")
 
 
+def check_page_size(page_size: int) -> None:
+    """ValueError for a number of positions that a page does not take."""
+    if page_size < 32 or page_size % 32 or page_size > 65536:
+        raise ValueError(f"pages hold a multiple of 32 positions up to 65536, got {page_size}")
+
+
 class _Heads:
     """What the caches' calls have in common: their arguments, rows of heads of
     head_dim on the cache's device."""
@@ -458,4 +464,4 @@ class PagedKVCache(_Heads):
 
 
 __all__ = ["BLOCK", "HEAD_DIMS", "MAX_GROUP", "PagedKVCache", "QuantKVCache", "check_heads",
-           "check_paged_heads"]
+           "check_page_size", "check_paged_heads"]

@@ -41,7 +41,8 @@ import numpy as np
 
 from . import _lib
 from .kvcache import BLOCK as KV_BLOCK
-from .kvcache import PagedKVCache, QuantKVCache, check_heads, check_paged_heads
+from .kvcache import (PagedKVCache, QuantKVCache, check_heads, check_page_size,
+                      check_paged_heads)
 from .logits import adjust_logits, pack_mask, sample_logits, sampling_params
 from .qmatrix import (DENSE_DTYPES, MIXABLE_DTYPES, DenseMatrix, QuantMatrix,
                       interleave_rows, matvec_fused_device, matvec_multi_device,
@@ -760,6 +761,7 @@ class Model:
             raise ValueError("need a non-empty prompt, n_gen >= 1 and n_seq >= 1")
         if kv_dtype not in ("f16", "bf16"):
             raise ValueError(f"unknown kv_dtype {kv_dtype!r} (f16, bf16)")
+        check_page_size(page_size)
         check_paged_heads(hp.n_head, hp.n_kv, hp.head_dim)
         n_p = len(prompt)
         if n_p + n_gen - 1 > self.n_ctx:

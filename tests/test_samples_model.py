@@ -187,3 +187,25 @@ def test_heads():
         for n_head, n_kv in ((MAX_GROUP * 3 + 3, 3), (7, 2), (2, 4), (0, 1)):
             with pytest.raises(ValueError):
                 check_paged_heads(n_head, n_kv, hd)
+
+
+def test_page_sizes():
+    from alpacca_amd.kvcache import check_page_size
+    for size in (32, 64, 96, 65536):
+        check_page_size(size)
+    for size in (0, -64, 20, 31, 33, 65568, 1 << 40):
+        with pytest.raises(ValueError, match="multiple of 32"):
+            check_page_size(size)
+
+
+@gpu
+@pytest.mark.parametrize("size", [0, -64, 33, 1 << 20])
+def test_bad_page_size_leaves_the_cache(size):
+    """Refused before the model's own cache is emptied."""
+    from alpacca_amd.model import Model
+    m = Model(*tiny())
+    m.generate_greedy([1, 2, 3], 2)
+    n_past = m.n_past
+    with pytest.raises(ValueError, match="multiple of 32"):
+        m.generate_samples([1, 2], 3, page_size=size)
+    assert m.n_past == n_past > 0
