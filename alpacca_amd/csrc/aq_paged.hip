@@ -589,8 +589,8 @@ struct Tokens {
   const int64_t *pos;
   int64_t start, room;
   __device__ __forceinline__ int len(int t) const {
-    const int64_t n = load_const(pos + t) - start + 1;
-    return (int)(n < room ? n : room);
+    const int64_t n = load_const(pos + t) - start;
+    return (int)(n < room ? n + 1 : room);
   }
 };
 
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2)
         if ((i - from) % per) return;
         tok.count = min(per, to - i);
         // the shortest and the longest of them, and the lane's row's
-        const int64_t its = lp - tab.start + 1 < room ? lp - tab.start + 1 : room;
+        const int64_t its = lp - tab.start < room ? lp - tab.start + 1 : room;
         int lo = INT32_MAX, hi = 0;
         for (int t = 0; t < tok.count; ++t) {
           const int l = __builtin_amdgcn_readlane((int)its, i + t);

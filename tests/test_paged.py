@@ -333,6 +333,18 @@ def test_attend_runs_of_tokens(n_head, n_kv, hd, start):
 
 
 @gpu
+@pytest.mark.parametrize("start", [0, 64])
+def test_positions_past_the_table(start):
+    """A row attends to all that its row of the table holds, alone or in a run."""
+    seqs, own, end = 3, 96, (1 << 63) - 1
+    c, table, prefix, K, V, KP, VP = setting(8, 2, 64, 32, "f16", seqs, own, start, seed=7)
+    pos = torch.tensor([start + 4, end, start + 95, start + 96, end - 1, end, start], device="cuda")
+    q = rand(7, 8 * 64, seed=20)
+    for seq in ([0, 0, 0, 1, 1, 1, 2], [0, 1, 2, 0, 1, 2, 0], [2] * 7):
+        check_attend(c, q, table, pos, torch.tensor(seq, device="cuda"), K, V, prefix, start, KP, VP)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("n_head,n_kv,hd,T", [(8, 2, 64, 4), (14, 2, 128, 2), (4, 4, 128, 16)])
 def test_tokens_do_not_see_what_comes_after_them(n_head, n_kv, hd, T, dtype):
