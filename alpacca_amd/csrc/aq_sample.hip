@@ -539,7 +539,9 @@ struct BinOrder {
       lo = hi - lo > width ? hi - width : lo;
     }
     if (in_bin > kRest) t_hi = r.last;
-    while (in_bin > kRest) {  // of equal logits the lowest tokens first
+    // of equal logits the lowest tokens first (one token always ends it, also where
+    // another stream writes the logits meanwhile)
+    while (in_bin > kRest && t_lo < t_hi) {
       int shift = 0;
       while (((t_hi - t_lo) >> shift) >= kBins) ++shift;
       fill_bins(s.fine, from, r, has,
