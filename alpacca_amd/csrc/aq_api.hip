@@ -1503,7 +1503,8 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
   if (int rc = paged_tokens(cache, N, table, seqs, width, pos, start)) return rc;
   if (n_rot < 0 || n_rot > cache->head_dim || n_rot % 2)
     return fail(AQ_ERR_VALUE, "n_rot %d must be even and <= head_dim %d", n_rot, cache->head_dim);
-  if (n_rot && (!cos_tab || !sin_tab || n_pos < 0)) return fail(AQ_ERR_VALUE, "NULL rotation table");
+  if (n_rot && (!cos_tab || !sin_tab || n_pos < 0))
+    return fail(AQ_ERR_VALUE, "NULL rotation table");
   if (q && (n_head <= 0 || n_head > 65535)) return fail(AQ_ERR_VALUE, "bad n_head %d", n_head);
   if (N && (!k || !v || (q && !q_out))) return fail(AQ_ERR_VALUE, "NULL pointer argument");
   if (int rc = kv8_aligned(q, k, v, q_out)) return rc;

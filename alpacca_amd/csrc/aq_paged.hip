@@ -119,8 +119,8 @@ __device__ __forceinline__ Group group_of(const aq_paged &c, const PagedTable &t
 // values four dimensions of four tokens.  Workgroups 0 .. n_qk - 1 take the queries and
 // keys, per_token of them a token, the others the values.
 //
-// One token of 32 / 8 heads of 64 3 us (its chain: position, page, store), 2048 of 32 / 8
-// of 128 bound by memory.
+// One token of 32 / 8 heads of 64 3.2 us (a launch's start and its chain: position, page,
+// store), 64 of 32 / 8 of 128 5.9, 2048 of them 21.7, bound by memory (92 MB: 4.2 TB/s).
 template <int HD, typename T>
 __global__ void __launch_bounds__(256)
     k_paged_append(const float *q, const float *__restrict__ k, const float *__restrict__ v,
@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(256)
   if (p.pos < 0 || p.pos >= n_pos) return;  // (the whole workgroup)
   const float *cr = cos_t + p.pos * half, *sr = sin_t + p.pos * half;
   if (pairs) {
-    const f4u cs = *reinterpret_cast<const f4u *>(cr + a), sn = *reinterpret_cast<const f4u *>(sr + a);
+    const f4u cs = *reinterpret_cast<const f4u *>(cr + a);
+    const f4u sn = *reinterpret_cast<const f4u *>(sr + a);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float r0 = x[e] * cs[e] - y[e] * sn[e];
@@ -262,7 +263,9 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- read-back -------------------------------------------------------------------
-// A thread a unit: 8 dimensions of a key, or four of four tokens' values.
+// A thread a unit: 8 dimensions of a key, or four of four tokens' values.  1 token of 8
+// heads of 64 3.2 us, 64 of 8 of 128 5.4, 2048 7.4 to 9.6 (16.8 MB: a launch's start and
+// end, then memory).
 template <int HD>
 __global__ void __launch_bounds__(256)
     k_paged_read(int64_t N, PagedTable tab, aq_paged c, uint16_t *__restrict__ ko,
@@ -596,7 +599,9 @@ struct Tokens {
 
 // One tile of rows against blocks b0 + wave, b0 + wave + 4, .. below b1 of a list of
 // pages, straight from memory; len: the largest of the tokens' lengths.  A wave's next
-// keys are on their way while it weighs the present ones.  In blocks where a token's
+// keys are on their way while it weighs the present ones; with eight waves a CU that is
+// enough to be bound by memory: 64 rows' own positions of 8 heads of 128 at 4.7 to 5.1
+// TB/s, the rate of a large copy.  In blocks where a token's
 // positions end, each token's sums take its own values alone: what lies behind them may
 // be an infinity or a NaN, which a weight of 0 would not undo.
 template <int HD, typename T>
@@ -657,7 +662,11 @@ __device__ __forceinline__ void attend_strided(const aq_paged &c, const int32_t 
 
 // The same for TW tiles of rows, a wave each, against blocks b0 .. b1 - 1,
 // which go through LDS in stages of 4 / TW ways of NB blocks: the four waves bring one
-// while another is computed.
+// while another is computed.  64 rows of 32 / 8 heads of 128 over 8000 positions 38 us in
+// fp16, 43 in bf16 (33 MB: 7 us, and as long on the matrix units): bound by a wave's own
+// chain of barrier, scores, weights and sums, which one wave a SIMD beside the rows' own
+// positions does not overlap.  Straight from memory 50 and 70; one block a stage 42; two
+// tiles of rows a wave, or three waves a SIMD, spill registers (105, 41 to 58).
 template <int HD, int TW>
 struct Stage {
   static constexpr int NB = TW == 4 ? 2 : 1, WAYS = 4 / TW, BLOCKS = WAYS * NB;
@@ -683,7 +692,8 @@ __device__ __forceinline__ void attend_staged(const aq_paged &c, const int32_t *
         if (!to_bring) break;
         const int64_t at = of_lane(mine, __builtin_ctzll(to_bring));
         to_bring &= to_bring - 1;
-        const char *k = static_cast<const char *>(c.k) + at, *v = static_cast<const char *>(c.v) + at;
+        const char *k = static_cast<const char *>(c.k) + at;
+        const char *v = static_cast<const char *>(c.v) + at;
         const uint32_t to = lds0 + buf * St::BYTES + p * St::BLOCK;
 #pragma unroll
         for (int j = 0; j < HD / 64; ++j) {

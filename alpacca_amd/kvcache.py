@@ -381,8 +381,8 @@ class PagedKVCache(_Heads):
         by cos / sin (positions, n_rot / 2; None: as it is), and rotate q
         (N, n_head * head_dim) into q_out (default: a new tensor; may be q), which
         is returned.  A token whose position is below 0 or past the tables is left
-        out, its row of q_out as it was (a new tensor's: undefined).  Two tokens in one place leave it undefined
-        whose values it holds."""
+        out, its row of q_out as it was (a new tensor's: undefined).  Two tokens in
+        one place leave it undefined whose values it holds."""
         torch = self._torch
         k, v = self._rows(k, "k", self.n_kv), self._rows(v, "v", self.n_kv)
         N = k.shape[0]
