@@ -20,8 +20,9 @@
 // finds from these largest a logit tau above which everything asked lies (at least k
 // tokens are as large as the k-th largest of them; and a sum that they alone reach
 // is reached above the last of them), reads the blocks that reach tau again, and
-// answers from the few tokens it finds: one wave sorts up to 64, up to kCap go into
-// bins.  Rows so flat that more matter are read pass by pass, into bins too.
+// answers from the few tokens it finds: one wave sorts up to 64, the workgroup up to
+// kWG, up to kCap go into bins.  Rows so flat that more matter are read pass by pass,
+// into bins too.
 #include <math.h>
 
 #include <type_traits>
@@ -158,7 +159,6 @@ struct Shared {
 struct Quad {
   f4u v;
   int64_t first;
-  int skip;  // elements below `at`
 };
 __device__ __forceinline__ Quad load_quad(const float *x, int64_t at, int64_t n) {
   Quad q;
@@ -316,30 +316,95 @@ struct Answer {
   uint64_t sum;
 };
 
+template <int E>
 struct WaveOrder {
-  int m;  // tokens, in the first lanes
-  uint64_t v, sum;
-  double w;
-  __device__ __forceinline__ uint64_t run(int i) const { return of_lane(sum, i); }
-  __device__ __forceinline__ uint64_t all() const { return run(m - 1); }
+  int m;  // tokens: lane l has the places l, l + 64, ..
+  uint64_t v[E], sum[E];
+  double w[E];
+  __device__ __forceinline__ uint64_t at(const uint64_t (&x)[E], int i) const {
+    uint64_t y = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) y = i / 64 == e ? x[e] : y;
+    return of_lane(y, i % 64);
+  }
+  __device__ __forceinline__ uint64_t all() const { return at(sum, m - 1); }
   __device__ __forceinline__ Answer ask(const Row &, bool by_count, uint64_t goal) const {
-    const uint64_t has = __ballot(sum >= goal);  // (lanes past m hold the last sum)
-    const int i = by_count ? (int)goal - 1 : has ? __builtin_ctzll(has) : 64;
+    int i = 0;  // (places past m hold the last sum)
+#pragma unroll
+    for (int e = 0; e < E; ++e) i += __popcll(__ballot(sum[e] < goal));
+    if (by_count) i = (int)goal - 1;
     if (i >= m) return {0, 0};
-    return {of_lane(v, i), run(i)};
+    return {at(v, i), at(sum, i)};
   }
   __device__ __forceinline__ uint64_t heavier(const Row &, double least) const {
-    const int n = __popcll(__ballot((int)(threadIdx.x & 63) < m && w >= least));
-    return n ? run(n - 1) : 0;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      n += __popcll(__ballot(64 * e + (int)(threadIdx.x & 63) < m && w[e] >= least));
+    return n ? at(sum, n - 1) : 0;
   }
 };
 // list[0 .. m), at most 64 tokens, sorted: the calling wave's
-__device__ __forceinline__ WaveOrder wave_order(const uint64_t *list, int m, const Row &r) {
+__device__ __forceinline__ WaveOrder<1> wave_order(const uint64_t *list, int m, const Row &r) {
   const int lane = threadIdx.x & 63;
   uint64_t v = lane < m ? list[lane] : 0;
   sort_wave(v);
   const double w = r.weight(logit_of(v));
-  return {m, v, running_wave<uint64_t>(lane < m ? r.units(w) : 0), w};
+  return {m, {v}, {running_wave<uint64_t>(lane < m ? r.units(w) : 0)}, {w}};
+}
+// How many of RUNS sorted runs of 64 places are larger than v, by halving.
+template <int RUNS>
+__device__ __forceinline__ int larger_than(const uint64_t *runs, uint64_t v) {
+  int at[RUNS] = {}, all = 0;
+#pragma unroll
+  for (int step = 32; step > 0; step /= 2) {
+    uint64_t y[RUNS];
+#pragma unroll
+    for (int w = 0; w < RUNS; ++w) y[w] = runs[64 * w + at[w] + step - 1];
+#pragma unroll
+    for (int w = 0; w < RUNS; ++w) at[w] += y[w] > v ? step : 0;
+  }
+#pragma unroll
+  for (int w = 0; w < RUNS; ++w) all += at[w] + (runs[64 * w + at[w]] > v ? 1 : 0);
+  return all;
+}
+// s.list[0 .. m), at most kWG tokens, sorted by the whole workgroup: a wave sorts 64 of
+// them, and a token's place is how many of each wave's are larger.  The order lies in
+// s.coarse, from where the calling wave has it.
+struct Sorted {
+  uint64_t runs[kWG], place[kWG], sum[kWG];
+  double weight[kWG];
+};
+__device__ __forceinline__ WaveOrder<kWaves> sorted_order(int m, const Shared &s) {
+  const Sorted &o = reinterpret_cast<const Sorted &>(s.coarse);
+  WaveOrder<kWaves> w;
+  w.m = m;
+#pragma unroll
+  for (int e = 0; e < kWaves; ++e) {
+    const int i = 64 * e + (threadIdx.x & 63);
+    w.v[e] = o.place[i], w.sum[e] = o.sum[i], w.w[e] = o.weight[i];
+  }
+  return w;
+}
+__device__ __forceinline__ void sort_list(int m, const Row &r, Shared &s) {
+  const int t = threadIdx.x;
+  Sorted &o = reinterpret_cast<Sorted &>(s.coarse);
+  static_assert(sizeof(Sorted) <= sizeof(Bins) && kWaves == 8, "");
+  uint64_t v = t < m ? s.list[t] : 0;
+  sort_wave(v);
+  o.runs[t] = v;
+  o.place[t] = 0;
+  __syncthreads();
+  if (v)
+    o.place[m <= 128   ? larger_than<2>(o.runs, v)
+            : m <= 256 ? larger_than<4>(o.runs, v)
+                       : larger_than<8>(o.runs, v)] = v;
+  __syncthreads();
+  v = o.place[t];
+  const double weight = r.weight(logit_of(v));
+  o.sum[t] = running(t < m ? r.units(weight) : 0, s);
+  o.weight[t] = weight;
+  __syncthreads();
 }
 
 // The answer from the m first tokens of the order.  total: of the whole row (without
@@ -414,17 +479,23 @@ __device__ __forceinline__ int find_bin(const Bins &b, Shared &s, bool by_count,
                                         Before &before, uint32_t &in_bin, bool both = true) {
   constexpr int PER = kBins / kWG;
   const int t = threadIdx.x;
-  uint64_t mass = 0, count = 0;
+  uint64_t masses[PER], mass = 0, count = 0;
+  uint32_t counts[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) mass += b.mass[PER * t + i], count += b.count[PER * t + i];
+  for (int i = 0; i < PER; ++i) masses[i] = b.mass[PER * t + i], counts[i] = b.count[PER * t + i];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mass += masses[i], count += counts[i];
   if (t == 0) s.bin = kBins;
   uint64_t m = !by_count || both ? running(mass, s) - mass + before.sum : 0;
   uint64_t c = by_count ? running(count, s) - count + before.count : 0;
   if ((by_count ? c : m) < goal && (by_count ? c + count : m + mass) >= goal) {
-    int i = PER * t;
-    for (; (by_count ? c + b.count[i] : m + b.mass[i]) < goal; ++i)
-      m += b.mass[i], c += b.count[i];
-    s.bin = i, s.mass = m, s.count = c, s.in_bin = b.count[i];
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (!found && (by_count ? c + counts[i] : m + masses[i]) >= goal)
+        found = true, s.bin = PER * t + i, s.mass = m, s.count = c, s.in_bin = counts[i];
+      m += masses[i], c += counts[i];
+    }
   }
   __syncthreads();
   const int bin = (int)s.bin;
@@ -571,56 +642,103 @@ struct BinOrder {
 // ---- few tokens --------------------------------------------------------------------
 
 // All tokens >= tau into the list, from the `reach` blocks that have any (s.block); the
-// list's length may pass kCap, its content does not.  A thread's quads are kWG apart,
-// U under way.
-template <int U>
+// list's length may pass kCap, its content does not.  First the numbers of the quads
+// that have any (they lie in s.coarse), up to kQuads of a thread's under way; then, a
+// thread each, their tokens: looking at every element of every quad instead took 5 us for
+// 286 blocks, this 3.4.  Where a thread has two quads at most they are all looked at.
 __device__ __forceinline__ int gather(const float *x, int64_t n, float tau, int reach, Shared &s) {
+  constexpr int kQuads = 12;
   const int t = threadIdx.x, lane = t & 63;
-  const int shift = part_shift(n) - 3 - 2;  // quads of a block
+  // a place in s.n_list's count for each of a lane's `mine`
+  auto places = [&](uint32_t mine) {
+    const uint32_t sum = running_wave(mine);
+    uint32_t base = 0;
+    if (lane == 63) base = atomicAdd(&s.n_list, sum);
+    return sum - mine + __builtin_amdgcn_readlane(base, 63);
+  };
+  auto listed = [&] {
+    __syncthreads();
+    const int m = (int)s.n_list;
+    __syncthreads();
+    return m;
+  };
   if (t == 0) s.n_list = 0;
   __syncthreads();
   if (n < 4) {
     if (t < n && x[t] >= tau) s.list[atomicAdd(&s.n_list, 1u)] = place_of(x[t], t);
-  } else {
-    const uint32_t quads = (uint32_t)reach << shift;
-    for (uint32_t c = 0; c < quads; c += kWG * U) {
-      Quad q[U];
+    return listed();
+  }
+  uint32_t *hits = reinterpret_cast<uint32_t *>(s.coarse.mass);
+  static_assert(sizeof(s.coarse.mass) >= kCap * sizeof(uint32_t), "");
+  const int shift = part_shift(n) - 3 - 2;  // quads of a block
+  const uint32_t quads = (uint32_t)reach << shift, end = (uint32_t)((n + 3) / 4);
+  auto quad_of = [&](uint32_t j) {
+    return j < quads ? (uint32_t)s.block[j >> shift] << shift | (j & ((1u << shift) - 1)) : end;
+  };
+  const bool all = quads <= 2 * kWG;
+  for (uint32_t c = 0; c < quads && !all; c += kWG * kQuads) {
+    f4u v[kQuads];
+    uint32_t quad[kQuads];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const uint32_t j = c + kWG * i + t, k = j >> shift;
-        const uint32_t block = s.block[k < (uint32_t)reach ? k : 0];
-        const int64_t at =
-            k < (uint32_t)reach ? 4 * (int64_t)((block << shift) | (j & ((1u << shift) - 1))) : n;
-        q[i] = load_quad(x, at, n);
-        q[i].skip = (int)(at - q[i].first < 4 ? at - q[i].first : 4);
-      }
-      uint32_t mine = 0;
+    for (int i = 0; i < kQuads; ++i) {
+      if (c + kWG * i >= quads) continue;
+      quad[i] = quad_of(c + kWG * i + t);
+      const int64_t at = 4 * (int64_t)quad[i];
+      v[i] = *reinterpret_cast<const f4u *>(x + (at < n - 4 ? at : n - 4));
+    }
+    uint32_t has = 0;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
+    for (int i = 0; i < kQuads; ++i) {
+      if (c + kWG * i >= quads) continue;
+      const float top = fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]));
+      if (top >= tau && quad[i] < end) has |= 1u << i;
+    }
+    if (!__any(has)) continue;
+    uint32_t j = places(__popc(has));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine += ((q[i].v[e] >= tau) & (e >= q[i].skip)) ? 1u : 0u;
-      if (!__any(mine)) continue;
-      uint32_t j = running_wave(mine) - mine;
-      const uint32_t all = __builtin_amdgcn_readlane(j + mine, 63);
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(&s.n_list, all);
-      j += __builtin_amdgcn_readfirstlane(base);
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (!mine) break;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((q[i].v[e] >= tau) & (e >= q[i].skip)) {
-            if (j < kCap) s.list[j] = place_of(q[i].v[e], (uint32_t)(q[i].first + e));
-            ++j;
-          }
+    for (int i = 0; i < kQuads; ++i) {
+      if (c + kWG * i >= quads) continue;
+      if (has >> i & 1) {
+        if (j < kCap) hits[j] = quad[i];
+        ++j;
       }
     }
   }
-  __syncthreads();
-  const int m = (int)s.n_list;
-  __syncthreads();
-  return m;
+  const int m = all ? (int)quads : listed();
+  if (m > kCap) return m;
+  if (!all) {
+    if (t == 0) s.n_list = 0;
+    __syncthreads();
+  }
+  for (int c = 0; c < m; c += 2 * kWG) {
+    int64_t first[2], at[2];
+    f4u v[2];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = c + kWG * i + t;
+      first[i] = 4 * (int64_t)(j >= m ? end : all ? quad_of(j) : hits[j]);
+      at[i] = first[i] < n - 4 ? first[i] : n - 4;  // (the last quad is moved inside)
+      if (c + kWG * i < m) v[i] = *reinterpret_cast<const f4u *>(x + at[i]);
+    }
+    auto is = [&](int i, int e) { return (v[i][e] >= tau) & (at[i] + e >= first[i]); };
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c + kWG * i < m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine += is(i, e) ? 1u : 0u;
+    uint32_t j = places(mine);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (c + kWG * i < m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (is(i, e)) {
+            if (j < kCap) s.list[j] = place_of(v[i][e], (uint32_t)(at[i] + e));
+            ++j;
+          }
+  }
+  return listed();
 }
 
 // tops: the blocks' largest logits, low the smallest of them.  false: the row's answer
@@ -685,13 +803,14 @@ __device__ __forceinline__ bool choose_few(const float *x, int64_t n, const Row 
   __syncthreads();
   const int reach = (int)s.n_list;
   __syncthreads();
-  const int m = reach << (part_shift(n) - 5) <= 2 * kWG ? gather<2>(x, n, tau, reach, s)
-                                                        : gather<8>(x, n, tau, reach, s);
+  const int m = gather(x, n, tau, reach, s);
   if (m > kCap) return false;
   total = whole_sum;
-  if (m <= 64) {
+  if (m <= kWG) {
+    if (m > 64) sort_list(m, r, s);
     if (t < 64) {
-      const uint64_t p = decide(wave_order(s.list, m, r), r, m, whole, to_min_p, total);
+      const uint64_t p = m > 64 ? decide(sorted_order(m, s), r, m, whole, to_min_p, total)
+                                : decide(wave_order(s.list, m, r), r, m, whole, to_min_p, total);
       if (t == 0) s.place = p, s.total = total;
     }
     __syncthreads();
@@ -796,10 +915,11 @@ __global__ void __launch_bounds__(256)
 }
 
 // One workgroup a row.  A chain of short steps, so bound by their latency and not by
-// bytes (the launch's start, the parts' results, tau, the blocks that reach it, the
-// list's sort or bins): one row of 128256 9.5 us, 64 of them with a top-k of 40 and top-p 10,
-// with top-p 0.9 alone 19.  Rows so flat that tokens past kCap count (a temperature of 1.3 with
-// top-p and no top-k) read the row several times, 150 to 190.
+// bytes (the launch's start and the parts' results 2 us, tau 3, the blocks that reach it
+// 1.5 to 3.5, the list's order 2 to 4, the answer 2): one row of 128256 9.2 us, 64 of
+// them with a top-k of 40 and top-p 10, with top-p 0.9 alone, lists of up to 418 tokens,
+// 15.8 (19.2 with such lists in bins).  Rows so flat that tokens past kCap count (a
+// temperature of 1.3 with top-p and no top-k) read the row several times, 150 to 190.
 __global__ void __launch_bounds__(kWG)
     k_sample(const float *__restrict__ logits, int64_t n, const double *__restrict__ u,
              const double *__restrict__ params, int64_t params_ld, const double *__restrict__ sums,

@@ -5,7 +5,10 @@ Tolerances.  The kernel adds weights as whole multiples of 2^-e of the largest,
 e = 62 - bits(n): a sum of n of them is off by n 2^-(e + 1) at most, plus a double
 exponential's 2^-50 or so each.  Where u times the sum lies nearer to a border than
 SLACK of the sum, the oracle takes either side's token; that happens to a row in
-1e7 here.  A logarithm is rounded to fp32 once: 2^-24 of it, beside 1e-9 for the
+1e7 here.  So it does where top-p times the sum lies that near to one, for the same
+reason: of 200 equal logits 0.9 keeps 180 if the product is rounded to a double, 181 if
+it is not, as the double 0.9 is 0.9 + 2.2e-17, and so do other tokens whose weights are
+2e-13 together.  A logarithm is rounded to fp32 once: 2^-24 of it, beside 1e-9 for the
 sum."""
 from __future__ import annotations
 
@@ -49,19 +52,22 @@ def kept_of(x, temp, k, p, min_p):
 
 
 def want(x, u, temp, k, p, min_p):
-    """The tokens that may come out, and their log-probabilities."""
-    o, w = kept_of(x, temp, k, p, min_p)
-    if len(o) == 0:
-        return {-1: -np.inf}
-    run = np.cumsum(w)
+    """The tokens that may come out, and their log-probabilities (for each way to take
+    top-p's border)."""
     u = min(max(u if u == u else 0.0, 0.0), 1 - 2 ** -53)
     out = {}
-    for g in (u - SLACK, u, u + SLACK):
-        i = min(int(np.searchsorted(run, g * run[-1], side="right")), len(o) - 1)
-        while i > 0 and w[i] == 0:
-            i -= 1
-        with np.errstate(divide="ignore"):
-            out[int(o[i])] = float(np.log(w[i]) - np.log(run[-1])) if temp > 0 else 0.0
+    for share in sorted({p, p * (1 - SLACK), p * (1 + SLACK)} if p < 1 else {p}):
+        o, w = kept_of(x, temp, k, share, min_p)
+        if len(o) == 0:
+            return {-1: {-np.inf}}
+        run = np.cumsum(w)
+        for g in (u - SLACK, u, u + SLACK):
+            i = min(int(np.searchsorted(run, g * run[-1], side="right")), len(o) - 1)
+            while i > 0 and w[i] == 0:
+                i -= 1
+            with np.errstate(divide="ignore"):
+                lp = float(np.log(w[i]) - np.log(run[-1])) if temp > 0 else 0.0
+            out.setdefault(int(o[i]), set()).add(lp)
     return out
 
 
@@ -77,11 +83,10 @@ def check(x, u, par):
     for r in range(len(x)):
         ok = want(x[r], float(u[r]), *(par[r] if par.ndim == 2 else par))
         assert int(tok[r]) in ok, (r, int(tok[r]), ok, u[r], par)
-        ref = ok[int(tok[r])]
-        if math.isinf(ref):
-            assert lp[r] == ref
-        else:
-            assert abs(lp[r] - ref) <= abs(ref) * 2 ** -24 + 1e-9 + 1e-12 * abs(ref), (r, lp[r], ref)
+        refs = ok[int(tok[r])]
+        assert any(lp[r] == ref if math.isinf(ref) else
+                   abs(lp[r] - ref) <= abs(ref) * 2 ** -24 + 1e-9 + 1e-12 * abs(ref)
+                   for ref in refs), (r, lp[r], refs)
 
 
 def logits(rng, rows, n, spread=3.0):
@@ -114,6 +119,23 @@ def test_each_row_its_own():
     rng = np.random.default_rng(5)
     rows, n = 3 * len(SETTINGS), 20011
     check(logits(rng, rows, n), rng.random(rows), np.array(SETTINGS * 3))
+
+
+@gpu
+@pytest.mark.parametrize("n", [40003, 9001])
+@pytest.mark.parametrize("m", [1, 63, 64, 65, 128, 129, 200, 256, 257, 511, 512, 513, 1024, 1025,
+                               4095, 4096, 4097, 8000])
+def test_lengths_of_what_is_kept(m, n):
+    """As many tokens far above the others as each way of ordering takes, and one
+    more: scattered, together at the row's end, and in groups of equal ones."""
+    rng = np.random.default_rng(m)
+    x = rng.standard_normal((6, n)).astype(np.float32) - 40
+    head = (0.002 * np.arange(m)[::-1]).astype(np.float32)
+    for r in range(6):
+        where = rng.choice(n, m, replace=False) if r % 2 else np.arange(n - m, n)
+        x[r, rng.permutation(where) if r < 4 else where] = head if r < 2 else np.floor(2 * head)
+    for par in ((1.0, m, 1.0, 0.0), (1.0, m, 0.97, 0.0), (3.0, 0, 0.999, 0.0), (1.0, 0, 0.9, 1e-3)):
+        check(x, rng.random(6), par)
 
 
 @gpu
