@@ -139,6 +139,22 @@ def test_lengths_of_what_is_kept(m, n):
 
 
 @gpu
+@pytest.mark.parametrize("heavy", [2, 3, 17, 64, 500])
+def test_heavy_tokens_side_by_side(heavy):
+    """What is kept lies together, where the largest of 64 tokens each say little of
+    the sum; and a body that weighs little, as much, or most."""
+    rng = np.random.default_rng(heavy)
+    n, rows = 30011, 8
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    for r in range(rows):
+        first = int(rng.integers(0, n - heavy)) if r % 2 else 640 + 64 * r
+        x[r, first:first + heavy] = 8 + 0.7 * r - rng.uniform(0, 0.5, heavy)
+    for par in ((0.9, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 0, 0.999, 1e-4), (0.8, 0, 0.5, 0.0),
+                (1.0, heavy, 0.9, 0.0)):
+        check(x, rng.random(rows), par)
+
+
+@gpu
 @pytest.mark.parametrize("u", [0.0, 1e-300, 0.25, 0.5, 1 - 2 ** -53, 1.0, 7.0, -3.0, np.nan])
 def test_ends_of_u(u):
     rng = np.random.default_rng(11)
