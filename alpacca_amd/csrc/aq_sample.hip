@@ -19,7 +19,8 @@
 // logit of every 64 tokens and, without a top-k, sums.  k_sample, a workgroup a row,
 // finds from these largest a logit tau above which everything asked lies (at least k
 // tokens are as large as the k-th largest of them; and a sum that they alone reach
-// is reached above the last of them), reads the blocks that reach tau again, and
+// is reached above the last of them; where they are too few for either, what lies above
+// tau is counted or summed before it is used), reads the blocks that reach tau again, and
 // answers from the few tokens it finds: one wave sorts up to 64, the workgroup up to
 // kWG, up to kCap go into bins.  Rows so flat that more matter are read pass by pass,
 // into bins too.
@@ -409,7 +410,9 @@ __device__ __forceinline__ void sort_list(int m, const Row &r, Shared &s) {
 
 // The answer from the m first tokens of the order.  total: of the whole row (without
 // a top-k) on entry, of what is kept on return.  whole: there are no more tokens;
-// to_min_p: what min-p keeps is among them.  0: they end too early.
+// to_min_p: what min-p keeps is among them.  With a top-k of k they are at least k, or
+// the whole row, or hold what min-p keeps of a row without top-p.  0: they end too
+// early.
 template <class Order>
 __device__ __forceinline__ uint64_t decide(const Order &order, const Row &r, int64_t m, bool whole,
                                            bool to_min_p, uint64_t &total) {
@@ -420,7 +423,6 @@ __device__ __forceinline__ uint64_t decide(const Order &order, const Row &r, int
     uint64_t goal;
     if (step == 0) {
       if (r.k ? r.k >= m : whole) total = order.all();
-      if (r.k && m < r.k && !whole && !to_min_p) return 0;
       open = !r.k && !whole;
       if (!r.k || r.k >= m) continue;
       by_count = true;
@@ -803,20 +805,30 @@ __device__ __forceinline__ bool choose_few(const float *x, int64_t n, const Row 
     tau = floor_;
   }
   if (floor_ >= tau && !(r.k && r.p < 1.0)) tau = floor_;
+  constexpr float kLowest = -3.402823466e38f;
   const bool to_min_p = floor_ >= tau;
-  tau = fmaxf(tau, -3.402823466e38f);
-  const bool whole = tau == -3.402823466e38f;
-  // the blocks that reach tau, in no order
-  if (t == 0) s.n_list = 0;
-  __syncthreads();
+  tau = fmaxf(tau, kLowest);
+  bool whole;
+  int m;
+  for (;;) {
+    whole = tau == kLowest;
+    // the blocks that reach tau, in no order
+    if (t == 0) s.n_list = 0;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBlocks; ++i)
-    if (tops[i] >= tau) s.block[atomicAdd(&s.n_list, 1u)] = (uint16_t)(i * kWG + t);
-  __syncthreads();
-  const int reach = (int)s.n_list;
-  __syncthreads();
-  const int m = gather(x, n, tau, reach, s);
-  if (m > kCap) return false;
+    for (int i = 0; i < kBlocks; ++i)
+      if (tops[i] >= tau) s.block[atomicAdd(&s.n_list, 1u)] = (uint16_t)(i * kWG + t);
+    __syncthreads();
+    const int reach = (int)s.n_list;
+    __syncthreads();
+    m = gather(x, n, tau, reach, s);
+    if (m > kCap) return false;
+    // Fewer blocks than k have anything: tau is the smallest of their largest, and k
+    // tokens need not reach it.  top-p's share is of all k, whatever min-p keeps, so a
+    // list short of them is made of all tokens (once: it is whole then).
+    if (whole || !r.k || m >= r.k || (to_min_p && !(r.p < 1.0))) break;
+    tau = kLowest;
+  }
   total = whole_sum;
   if (m <= kWG) {
     if (m > 64) sort_list(m, r, s);
@@ -830,8 +842,8 @@ __device__ __forceinline__ bool choose_few(const float *x, int64_t n, const Row 
     total = s.total;
     __syncthreads();
   } else {
-    Row lr = r;  // bins over the list's range
-    lr.inv_bin = (float)kBins / (r.top - tau);
+    Row lr = r;  // bins over the list's range, where it has an end
+    if (!whole) lr.inv_bin = (float)kBins / (r.top - tau);
     const ListTokens tokens = {s.list, m};
     const BinOrder<ListTokens> order = {tokens, s};
     order.fill(lr);
