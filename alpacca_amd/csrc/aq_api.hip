@@ -1481,6 +1481,9 @@ int paged_attention_shape(const aq_paged *c, int64_t N, int n_head, int64_t widt
   if (width < 0 || start < 0 || width > INT32_MAX / c->page_size || start > INT32_MAX)
     return fail(AQ_ERR_VALUE, "bad table width %lld or start %lld", (long long)width,
                 (long long)start);
+  if (!aq::attention_paged_fits(*c, N, n_head, width, start))
+    return fail(AQ_ERR_VALUE, "%lld query rows of %d kv heads are too many for one call",
+                (long long)N, c->n_kv);
   return AQ_OK;
 }
 }  // namespace

@@ -259,6 +259,8 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
 hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c, void *k, void *v,
                              hipStream_t s);
 // pre: one row, the prefix's pages; its start is the prefix's length
+bool attention_paged_fits(const aq_paged &c, int64_t N, int n_head, int64_t width,
+                          int64_t start);  // in one launch
 size_t attention_paged_scratch(const aq_paged &c, int64_t N, int n_head, int64_t width,
                                int64_t start);
 hipError_t launch_attention_paged(const float *q, int64_t N, int n_head, const PagedTable &tab,

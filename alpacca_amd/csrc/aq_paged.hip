@@ -24,6 +24,8 @@ namespace aq {
 namespace {
 
 constexpr int kBlk = 32;
+// workgroups of one launch: a grid holds fewer than 2^32 threads, 256 a workgroup
+constexpr int64_t kMaxGrid = (1 << 24) - 1;
 
 template <int HD>
 __device__ __forceinline__ int k_place(int s, int d) {
@@ -1023,7 +1025,8 @@ PagedPlan paged_plan(const aq_paged &c, int64_t N, int n_head, int64_t width, in
   }
   const int64_t items = N * c.n_kv, blocks = width * c.page_size / kBlk;
   const int64_t left = std::max<int64_t>(places - p.pre, places / 2);
-  const int64_t most = std::min<int64_t>((blocks + 3) / 4, p.sp ? 16 : 64);
+  const int64_t fit = items ? (kMaxGrid - p.pre) / items : 1;  // splits that one launch takes
+  const int64_t most = std::min({(blocks + 3) / 4, (int64_t)(p.sp ? 16 : 64), fit});
   p.ss = 1;
   int64_t best = INT64_MAX;
   for (int64_t s = 1; s <= std::max<int64_t>(most, 1); ++s) {
@@ -1057,7 +1060,7 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
   const int64_t per_token = (heads * c.head_dim / 8 + 255) / 256;
   const int64_t per_group = ((int64_t)c.n_kv * c.head_dim / 4 + 255) / 256;
   const int64_t n_qk = by_pairs ? 0 : N * per_token, n_v = (N + 6) / 4 * per_group;
-  if (n_qk + n_v > INT32_MAX || N > INT32_MAX) return hipErrorInvalidValue;
+  if (n_qk + n_v > kMaxGrid || N > kMaxGrid) return hipErrorInvalidValue;
   by_shape(c, [&](auto hd, auto t) {
     constexpr int HD = decltype(hd)::value;
     typedef decltype(t) T;
@@ -1076,13 +1079,19 @@ hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c
   const int64_t per_token = ((int64_t)c.n_kv * c.head_dim / 8 + 255) / 256;
   const int64_t per_group = ((int64_t)c.n_kv * c.head_dim / 4 + 255) / 256;
   const int64_t n_k = N * per_token, n_v = (N + 6) / 4 * per_group;
-  if (n_k + n_v > INT32_MAX) return hipErrorInvalidValue;
+  if (n_k + n_v > kMaxGrid) return hipErrorInvalidValue;
   by_shape(c, [&](auto hd, auto) {
     hipLaunchKernelGGL((k_paged_read<decltype(hd)::value>), dim3((unsigned)(n_k + n_v)), dim3(256),
                        0, s, N, tab, c, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v),
                        (unsigned)per_token, (unsigned)per_group, (unsigned)n_k);
   });
   return hipGetLastError();
+}
+
+bool attention_paged_fits(const aq_paged &c, int64_t N, int n_head, int64_t width,
+                          int64_t start) {
+  const PagedPlan p = paged_plan(c, N, n_head, width, start);
+  return (int64_t)p.pre + p.own <= kMaxGrid && (p.states() <= 8 || N * n_head <= kMaxGrid);
 }
 
 size_t attention_paged_scratch(const aq_paged &c, int64_t N, int n_head, int64_t width,

@@ -582,7 +582,9 @@ int aq_paged_sizes(const aq_paged *cache, size_t *bytes);
  * and values [N][n_kv * head_dim], rounded to the cache's type (to nearest, ties to
  * even; past fp16's range: infinity), into their places.  A token whose position is
  * below 0 or (with n_rot) not below n_pos is left out altogether, its row of q_out
- * as it was; one that has no place otherwise has its query rotated.  Enqueues only. */
+ * as it was; one that has no place otherwise has its query rotated.  AQ_ERR_VALUE, and
+ * nothing stored, for more tokens than one launch takes (2^24 - 1 workgroups of 256
+ * threads, a thread 8 dimensions of a head).  Enqueues only. */
 int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, int64_t N,
                   int n_head, int n_rot, int neox, const float *cos_tab, const float *sin_tab,
                   int64_t n_pos, const int32_t *table, int64_t seqs, int64_t width,
@@ -594,7 +596,8 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
  * prefix [n_prefix] (start <= n_prefix * page_size), the others in its row of the
  * table.  Positions without a place are left out; a row that has none, or whose
  * position is below 0, gives 0.  out [N][n_head * head_dim].  Groups n_head / n_kv of
- * 1 to 16; N * n_head up to 2^24.  Float32 accuracy over the values stored.
+ * 1 to 16; N * n_head up to 2^24, and as many rows as one launch takes, 2^24 - 1
+ * workgroups (AQ_ERR_VALUE: N * n_kv close to 2^24).  Float32 accuracy over the values stored.
  * scratch: at least the bytes that aq_attention_paged_scratch says for the same
  * call, 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
 int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
@@ -608,7 +611,8 @@ int aq_attention_paged_scratch(const aq_paged *cache, int64_t N, int n_head, int
                                int64_t start, size_t *bytes);
 
 /* k, v [N][n_kv * head_dim] in the cache's type: the values that N tokens' places
- * hold; 0 where a token has none.  Enqueues only. */
+ * hold; 0 where a token has none.  As many tokens as aq_rope_paged takes without
+ * queries (AQ_ERR_VALUE).  Enqueues only. */
 int aq_paged_read(const aq_paged *cache, int64_t N, const int32_t *table, int64_t seqs,
                   int64_t width, const int64_t *seq, const int64_t *pos, int64_t start, void *k,
                   void *v, void *stream);
