@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(256)
 // 16x16x32 matrix instructions of the cache's type, with every fp32 operand in
 // pieces of that type (x = sum of pieces: two of fp16, 22 bits; three of bf16, 24):
 //   S^T (positions x rows) = K Q^T, Q's row times log2(e) / sqrt(head_dim) and a
-//     power of two that brings its largest value to [2^14, 2^15): lane l holds row
-//     l % 16's scores at positions 16 pt + 4 (l / 16) + r (pt = 0, 1; r = 0 .. 3);
+//     power of two (Ops<T>::shift): lane l holds row l % 16's scores at positions
+//     16 pt + 4 (l / 16) + r (pt = 0, 1; r = 0 .. 3);
 //   O^T (dimensions x rows) += V^T P^T: those eight weights are the lane's operand
 //     as it holds them.  Lane l gets row l % 16's dimensions 16 dt + 4 (l / 16) + r.
 // Weights are P = 2^(z - m + 14), m the running maximum rounded up to a whole
@@ -346,6 +346,12 @@ struct Ops;
 template <>
 struct Ops<_Float16> {
   static constexpr int NP = 2;
+  // The power of two that a query row is raised by, am its largest value: to
+  // [2^14, 2^15) after the factor f, where the second piece's last bit is a normal one's.
+  // (A row below 2^-110 keeps fewer bits of scores that are as good as 0.)
+  static __device__ __forceinline__ int shift(float am, float f) {
+    return min(15 - __builtin_amdgcn_frexp_expf(am * f), 125);
+  }
   static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
                                                   __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -367,6 +373,13 @@ struct Ops<_Float16> {
 template <>
 struct Ops<__bf16> {
   static constexpr int NP = 3;
+  // bf16 has float32's exponents, and so have the keys: rows go down by 2^12, and sums of
+  // their products pass float32's range only where the scores (which come back up in
+  // the weights' exponents) are past it themselves.  A row whose last piece would then not
+  // be normal is brought to 2^-24, from where no key takes a sum past 2^(128 + 8 - 24).
+  static __device__ __forceinline__ int shift(float am, float) {
+    return am < 0x1p-64f ? -24 - __builtin_amdgcn_frexp_expf(am) : -12;
+  }
   static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a),
                                                    __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -422,7 +435,7 @@ struct QRow {
       for (int i = 0; i < 2; ++i) {
         const f4v x = *reinterpret_cast<const f4v *>(q + 32 * ks + 8 * cg + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[ks][4 * i + e] = live ? x[e] * f : 0.f;
+        for (int e = 0; e < 4; ++e) v[ks][4 * i + e] = live ? x[e] : 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -433,14 +446,13 @@ struct QRow {
     }
     am = row_max(am);
     const bool bad = am == INFINITY;
-    // (a row below 2^-110 keeps fewer bits of scores that are as good as 0)
-    const int up = am > 0.f && !bad ? min(15 - __builtin_amdgcn_frexp_expf(am), 125) : 0;
+    const int up = am > 0.f && !bad ? Ops<T>::shift(am, f) : 0;
     back = ldexpf(1.f, -up);
 #pragma unroll
     for (int ks = 0; ks < HD / 32; ++ks)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float a = ldexpf(v[ks][2 * i], up), b = ldexpf(v[ks][2 * i + 1], up);
+        float a = ldexpf(v[ks][2 * i], up) * f, b = ldexpf(v[ks][2 * i + 1], up) * f;
         a = bad ? NAN : a;
         b = bad ? NAN : b;
         uint32_t parts[NP];

@@ -597,8 +597,9 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
  * table.  Positions without a place are left out; a row that has none, or whose
  * position is below 0, gives 0.  out [N][n_head * head_dim].  Groups n_head / n_kv of
  * 1 to 16; N * n_head up to 2^24, and as many rows as one launch takes, 2^24 - 1
- * workgroups (AQ_ERR_VALUE: N * n_kv close to 2^24).  Float32 accuracy over the values stored.
- * scratch: at least the bytes that aq_attention_paged_scratch says for the same
+ * workgroups (AQ_ERR_VALUE: N * n_kv close to 2^24).  Float32 accuracy over the values
+ * stored, for queries and keys of any size whose scores q.k / sqrt(head_dim) are up to
+ * 2.3e38 (past that, as with an infinity or a NaN, a row may be NaN).  scratch: at least the bytes that aq_attention_paged_scratch says for the same
  * call, 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
 int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
                        const int32_t *table, int64_t seqs, int64_t width, const int64_t *seq,
