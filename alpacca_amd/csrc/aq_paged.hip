@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256)
 //     16 pt + 4 (l / 16) + r (pt = 0, 1; r = 0 .. 3);
 //   O^T (dimensions x rows) += V^T P^T: those eight weights are the lane's operand
 //     as it holds them.  Lane l gets row l % 16's dimensions 16 dt + 4 (l / 16) + r.
-// Weights are P = 2^(z - m + 14), m the running maximum rounded up to a whole
+// Weights are P = 2^(z - m + Ops<T>::kTop), m the running maximum rounded up to a whole
 // number, so that rescaling is exact and rare, and the pieces hold 22 bits of what
 // counts.  The sum of the weights is kept per lane, in fp32.
 typedef float f2v __attribute__((ext_vector_type(2)));
@@ -339,13 +339,12 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
-constexpr float kTop = 14.f;  // weights reach 2^14 in the pieces
-
 template <typename T>
 struct Ops;
 template <>
 struct Ops<_Float16> {
   static constexpr int NP = 2;
+  static constexpr float kTop = 14.f;  // weights reach 2^14: their second piece is normal
   // The power of two that a query row is raised by, am its largest value: to
   // [2^14, 2^15) after the factor f, where the second piece's last bit is a normal one's.
   // (A row below 2^-110 keeps fewer bits of scores that are as good as 0.)
@@ -373,6 +372,7 @@ struct Ops<_Float16> {
 template <>
 struct Ops<__bf16> {
   static constexpr int NP = 3;
+  static constexpr float kTop = 0.f;  // values may be as large as float32: weights are not
   // bf16 has float32's exponents, and so have the keys: rows go down by 2^12, and sums of
   // their products pass float32's range only where the scores (which come back up in
   // the weights' exponents) are past it themselves.  A row whose last piece would then not
@@ -501,7 +501,7 @@ __device__ __forceinline__ void weigh(f4v (&sc)[NB][2], float back, const int (&
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) st.o[i] *= f;
   }
-  const float ref = kTop - finite_ref(st.m);
+  const float ref = Ops<T>::kTop - finite_ref(st.m);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     float p[8], l[4];
@@ -750,7 +750,7 @@ __device__ __forceinline__ void attend_staged(const aq_paged &c, const int32_t *
   }
 }
 
-// The partial state of a row: HD numerators relative to 2^(m - kTop), m, l.
+// The partial state of a row: HD numerators relative to 2^(m - Ops<T>::kTop), m, l.
 template <int HD>
 constexpr int kState = HD + 4;
 

@@ -598,8 +598,9 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
  * position is below 0, gives 0.  out [N][n_head * head_dim].  Groups n_head / n_kv of
  * 1 to 16; N * n_head up to 2^24, and as many rows as one launch takes, 2^24 - 1
  * workgroups (AQ_ERR_VALUE: N * n_kv close to 2^24).  Float32 accuracy over the values
- * stored, for queries and keys of any size whose scores q.k / sqrt(head_dim) are up to
- * 2.3e38 (past that, as with an infinity or a NaN, a row may be NaN).  scratch: at least the bytes that aq_attention_paged_scratch says for the same
+ * stored, whatever the size of queries, keys and values, where float32 holds the scores
+ * q.k / sqrt(head_dim) (up to 2.3e38) and the sums of e^(score - largest) v; past that, as
+ * with an infinity or a NaN among them, a row's outputs may be infinite or NaN.  scratch: at least the bytes that aq_attention_paged_scratch says for the same
  * call, 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
 int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
                        const int32_t *table, int64_t seqs, int64_t width, const int64_t *seq,

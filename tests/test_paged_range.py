@@ -1,5 +1,5 @@
-"""Attention over the paged cache with keys and queries of any size that bf16 and
-float32 hold.  Tolerance: that of tests/test_paged.py, whose check_attend this uses
+"""Attention over the paged cache with queries, keys and values of any size that bf16
+and float32 hold.  Tolerance: that of tests/test_paged.py, whose check_attend this uses
 (where scores are so large that their own rounding decides, it says no more than that
 the output is a number)."""
 from __future__ import annotations
@@ -61,3 +61,35 @@ def test_rows_of_different_sizes_together():
     # a row's bits do not depend on its neighbours'
     alone = c.attend(q[5:6].expand(N, -1).contiguous(), table, pos, start=64, prefix=prefix)
     assert torch.equal(alone[5], want[5])
+
+
+@gpu
+@pytest.mark.parametrize("vscale", [1e-30, 1e10, 1e32, 1e35, 1e36])
+@pytest.mark.parametrize("n_head,n_kv,hd,N,own,start", [
+    (8, 2, 64, 5, 50, 130), (16, 2, 128, 40, 40, 64), (4, 2, 256, 3, 33, 30), (8, 1, 64, 2, 300, 0)])
+def test_bf16_values_of_any_size(n_head, n_kv, hd, N, own, start, vscale):
+    """Values whose weighted sums float32 holds (at most 300 of 4e36 each here)."""
+    from tests.test_paged import fill
+    c, table, prefix, K, V, KP, VP = setting(n_head, n_kv, hd, 32, "bf16", N, own, start)
+    V, VP = ((x.double() * vscale).bfloat16() for x in (V, VP))
+    fill(c, table, K, V, start)
+    if start:
+        fill(c, prefix[None, :], KP[None], VP[None])
+    q = rand(N, n_head * hd, seed=15)
+    pos = (start + torch.arange(N) * 7 % own).cuda()
+    pos[0] = start + own - 1
+    out = check_attend(c, q, table, pos, None, K, V, prefix if start else None, start, KP, VP)
+    assert bool(out.isfinite().all())
+
+
+@gpu
+def test_one_value_next_to_the_largest():
+    """A row of one position gives its value, whatever it is."""
+    c, table, prefix, K, V, KP, VP = setting(8, 2, 64, 32, "bf16", 3, 1, 0)
+    top = torch.finfo(torch.bfloat16).max
+    v = torch.linspace(-top, top, 3 * 2 * 64, dtype=torch.float64).bfloat16().view(3, 128).cuda()
+    pos = torch.zeros(3, dtype=torch.int64, device="cuda")
+    c.append(rand(3, 128, seed=1), v.float(), table, pos)
+    out = c.attend(rand(3, 512, seed=2), table, pos).view(3, 2, 4, 64)
+    want = v.double().view(3, 2, 1, 64).expand(-1, -1, 4, -1)
+    assert bool(((out.double() - want).abs() <= 2.0 ** -20 * want.abs()).all())
