@@ -26,6 +26,8 @@ namespace {
 constexpr int kBlk = 32;
 // workgroups of one launch: a grid holds fewer than 2^32 threads, 256 a workgroup
 constexpr int64_t kMaxGrid = (1 << 24) - 1;
+// the end of positions that no table ends: all from 0 on are below it
+constexpr uint64_t kAnyPos = (uint64_t)1 << 63;
 
 template <int HD>
 __device__ __forceinline__ int k_place(int s, int d) {
@@ -99,7 +101,7 @@ struct Group {
   bool in[4], together;
 };
 __device__ __forceinline__ Group group_of(const aq_paged &c, const PagedTable &tab, int64_t N,
-                                          int64_t g, int64_t n_pos) {
+                                          int64_t g, uint64_t n_pos) {
   Group r;
   const int64_t first = 4 * g - lead_of(tab);
   r.together = true;
@@ -108,7 +110,7 @@ __device__ __forceinline__ Group group_of(const aq_paged &c, const PagedTable &t
     r.in[i] = first + i >= 0 && first + i < N;
     r.n[i] = r.in[i] ? first + i : 0;
     r.p[i] = place_of(c, tab, r.n[i]);
-    r.in[i] &= r.p[i].block >= 0 && r.p[i].pos < n_pos;
+    r.in[i] &= r.p[i].block >= 0 && (uint64_t)r.p[i].pos < n_pos;
     r.together &= r.in[i] && r.p[i].block == r.p[0].block && r.p[i].s == r.p[0].s + i;
   }
   r.together &= (r.p[0].s & 3) == 0;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(256)
     k_paged_append(const float *q, const float *__restrict__ k, const float *__restrict__ v,
                    float *q_out, int64_t N, int n_head, int n_rot, int neox,
                    const float *__restrict__ cos_t, const float *__restrict__ sin_t,
-                   int64_t n_pos, PagedTable tab, aq_paged c, unsigned per_token,
+                   uint64_t n_pos, PagedTable tab, aq_paged c, unsigned per_token,
                    unsigned per_group, unsigned n_qk) {
 #pragma clang fp contract(off)
   const int64_t per = c.page_size / kBlk;
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(256)
   const int a = pairs ? 4 * i : 8 * i, b = pairs ? a + half : a + 4;
   f4v x = *reinterpret_cast<const f4v *>(src + a), y = *reinterpret_cast<const f4v *>(src + b);
   const Place p = place_of(c, tab, n);
-  if (p.pos < 0 || p.pos >= n_pos) return;  // (the whole workgroup)
+  if ((uint64_t)p.pos >= n_pos) return;  // (the whole workgroup; a position below 0 too)
   const float *cr = cos_t + p.pos * half, *sr = sin_t + p.pos * half;
   if (pairs) {
     const f4u cs = *reinterpret_cast<const f4u *>(cr + a);
@@ -230,12 +232,12 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(256)
     k_paged_append_pairs(const float *q, const float *__restrict__ k, float *q_out, int n_head,
                          int n_rot, const float *__restrict__ cos_t,
-                         const float *__restrict__ sin_t, int64_t n_pos, PagedTable tab,
+                         const float *__restrict__ sin_t, uint64_t n_pos, PagedTable tab,
                          aq_paged c) {
 #pragma clang fp contract(off)
   const int64_t n = blockIdx.x;
   const Place p = place_of(c, tab, n);
-  if (p.pos < 0 || p.pos >= n_pos) return;
+  if ((uint64_t)p.pos >= n_pos) return;
   const int half = n_rot / 2, heads = (q ? n_head : 0) + c.n_kv;
   for (int j = threadIdx.x; j < heads * (HD / 2); j += 256) {
     int h = j / (HD / 2);
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(256)
   if (u >= c.n_kv * (HD / 4)) return;
   const int h = u / (HD / 4), d = 4 * (u % (HD / 4));
   const int64_t first = 4 * (int64_t)(b / per_group) - lead_of(tab);
-  const Group g = group_of(c, tab, N, b / per_group, INT64_MAX);
+  const Group g = group_of(c, tab, N, b / per_group, kAnyPos);
   const uint16_t *vp = static_cast<const uint16_t *>(c.v);
   four x[4];
   if (g.together) {
@@ -1066,7 +1068,8 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
                              int64_t N, int n_head, int n_rot, int neox, const float *cos_t,
                              const float *sin_t, int64_t n_pos, const PagedTable &tab,
                              const aq_paged &c, hipStream_t s) {
-  if (n_rot == 0) neox = 0, n_pos = INT64_MAX;  // (no table, and no end to it)
+  if (n_rot == 0) neox = 0;
+  const uint64_t end = n_rot ? (uint64_t)n_pos : kAnyPos;  // (no table, and no end to it)
   const bool by_pairs = neox && n_rot % 8 != 0;
   const int64_t heads = (q ? n_head : 0) + c.n_kv;
   const int64_t per_token = (heads * c.head_dim / 8 + 255) / 256;
@@ -1078,9 +1081,9 @@ hipError_t launch_rope_paged(const float *q, const float *k, const float *v, flo
     typedef decltype(t) T;
     if (by_pairs)
       hipLaunchKernelGGL((k_paged_append_pairs<HD, T>), dim3((unsigned)N), dim3(256), 0, s, q, k,
-                         q_out, n_head, n_rot, cos_t, sin_t, n_pos, tab, c);
+                         q_out, n_head, n_rot, cos_t, sin_t, end, tab, c);
     hipLaunchKernelGGL((k_paged_append<HD, T>), dim3((unsigned)(n_qk + n_v)), dim3(256), 0, s, q,
-                       k, v, q_out, N, n_head, n_rot, neox, cos_t, sin_t, n_pos, tab, c,
+                       k, v, q_out, N, n_head, n_rot, neox, cos_t, sin_t, end, tab, c,
                        (unsigned)per_token, (unsigned)per_group, (unsigned)n_qk);
   });
   return hipGetLastError();
