@@ -768,9 +768,18 @@ class Model:
             raise RuntimeError(f"context window full ({self.n_ctx} tokens)")
         if min(prompt) < 0 or max(prompt) >= hp.n_vocab:
             raise IndexError("row index out of range")
+        lib, s, chk = _lib.load(), self.stream.cuda_stream, _lib.check
+        # what the step's calls refuse they refuse here, before anything is changed
+        n_pre, width = -(-n_p // page_size), -(-(n_gen - 1) // page_size)
+        size = ctypes.c_size_t()
+        shape = _lib.Paged(None, None, n_pre + n_seq * width, page_size, hp.n_kv, hp.head_dim,
+                           _lib.DTYPE_IDS["F16"])
+        chk(lib.aq_sample_scratch(n_seq, hp.n_vocab, ctypes.byref(size)))
+        chk(lib.aq_paged_sizes(ctypes.addressof(shape), ctypes.byref(size)))
+        chk(lib.aq_attention_paged_scratch(ctypes.addressof(shape), n_seq, hp.n_head, width, n_p,
+                                           ctypes.byref(size)))
         params = sampling_params(n_seq, temperature, top_k, top_p, min_p, device=self.dev)
         adjust, _ = self._adjustment(0.0, 0.0, logit_bias, allowed)
-        lib, s, chk = _lib.load(), self.stream.cuda_stream, _lib.check
         sv = ctypes.c_void_p(s)
         p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
         neox = 1 if hp.rope_style == "neox" else 0
@@ -782,7 +791,6 @@ class Model:
         with torch.cuda.stream(self.stream):
             # made, used and freed on self.stream
             U = U.to(self.dev)
-            n_pre, width = -(-n_p // page_size), -(-(n_gen - 1) // page_size)
             pages = torch.arange(n_pre + n_seq * width, dtype=torch.int32, device=self.dev)
             prefix, table = pages[:n_pre], pages[n_pre:].view(n_seq, width)
             caches = [PagedKVCache(hp.n_kv, pages.numel(), hp.head_dim, page_size, dtype, self.dev)
@@ -794,12 +802,8 @@ class Model:
             hist = torch.zeros((n_gen, n_seq), dtype=torch.int64, device=self.dev)
             u = U[0].clone()
             logits = torch.empty((n_seq, hp.n_vocab), dtype=torch.float32, device=self.dev)
-        b = self._batch_buffers(n_seq)
-        size = ctypes.c_size_t()
-        chk(lib.aq_attention_paged_scratch(caches[0].handle, n_seq, hp.n_head, width, n_p,
-                                           ctypes.byref(size)))
-        with torch.cuda.stream(self.stream):
             scratch = torch.empty(size.value, dtype=torch.uint8, device=self.dev)
+        b = self._batch_buffers(n_seq)
 
         def store(li, pos0, T):
             bb = self._bb
