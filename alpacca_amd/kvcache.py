@@ -316,6 +316,10 @@ class PagedKVCache(_Heads):
         dtype = torch.float16 if dtype is None else dtype
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"the paged cache holds float16 or bfloat16, not {dtype}")
+        check_page_size(page_size)
+        for x, what in ((n_kv, "n_kv"), (n_pages, "n_pages"), (head_dim, "head_dim")):
+            if not 0 < x < 2 ** 31:  # (a C integer would keep its low bits)
+                raise ValueError(f"bad cache shape: {what} {x}")
         name = "F16" if dtype == torch.float16 else "BF16"
         self._c = _lib.Paged(None, None, n_pages, page_size, n_kv, head_dim,
                              _lib.DTYPE_IDS[name])
@@ -368,8 +372,8 @@ class PagedKVCache(_Heads):
             seq = self._index(seq, "seq", i64, 1)
             if seq.shape != pos.shape:
                 raise ValueError(f"seq has {seq.shape[0]} tokens, pos {pos.shape[0]}")
-        if start < 0:
-            raise ValueError(f"start {start} is below 0")
+        if not 0 <= start < 2 ** 63:
+            raise ValueError(f"start {start} is below 0 or past int64")
         return (table, pos, seq), (table.data_ptr(), table.shape[0], table.shape[1],
                                    None if seq is None else seq.data_ptr(), pos.data_ptr())
 
