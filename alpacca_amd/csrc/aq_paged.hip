@@ -1013,10 +1013,11 @@ __global__ void __launch_bounds__(256)
     *reinterpret_cast<f4v *>(out + row * HD + d) = o * (sum == 0.f ? 0.f : 1.f / sum);
 }
 
-// Splits.  The prefix: tiles of 16 rows in one workgroup of four waves that share the
-// positions up to 16 rows and of two up to 32, bound by memory (8 rows of 4 heads over
-// 100000 positions 89 us in 48 splits of 8 heads, 92 in 32); past that four tiles that
-// share them through LDS, a workgroup a CU: the rows' own positions, bound by memory,
+// Splits.  The prefix, in workgroups of four waves: up to 16 rows one tile, straight from
+// memory, which the waves part the positions of (8 rows of 4 heads over 100000 positions
+// 89 us in 48 splits of 8 heads, 92 in 32); up to 32 rows two tiles, two waves each, which
+// share stages of two blocks in LDS; past that four tiles, a wave each, that share all
+// positions through LDS, a workgroup a CU: the rows' own positions, bound by memory,
 // run on the same CUs (64 rows of 32 / 8 heads over 8000 and 1024 of their own 68 us;
 // with two workgroups of the prefix a CU, twice the states, 82; the two kinds in
 // turn 75, where rows that own little then wait for a late start: 28 against 25).

@@ -444,10 +444,12 @@ int aq_logits_adjust(const float *logits, int64_t rows, int64_t n, const int64_t
  *     top_k (top_p of 1 or more: all);
  *   those of w >= min_p (0 or less: all);
  * and the token is the first whose running sum exceeds u times the sum of all kept.
- * temperature 0 or less: the first token of the order.  Weights are formed in double
- * and added as whole multiples of 2^-e of the largest, e = 62 - (bits of n), so the
- * token is a function of the row alone.  (A token that weighs less than 2^-(e + 1)
- * of the largest is never drawn.)
+ * temperature 0 or less: the first token of the order.  Weights are formed in double,
+ * and running sums add them as whole multiples of 2^-e of the largest, e = 62 - (bits of
+ * n).  A whole row's sum without top_k is that or a sum of doubles, n 2^-(e + 1) of the
+ * largest away at most; which one goes by the row's logits and settings, so the token is a
+ * function of these and u.  (A token that weighs less than 2^-(e + 1) of the largest is
+ * never drawn.)
  * u [rows] (below 0 or NaN: 0; 1 and more: the largest number below 1); params: row
  * r's temperature, top_k, top_p, min_p at params + r * params_ld (params_ld 0: the
  * same for every row; NaN: as if left out, for the temperature 0).  out [rows]: the
@@ -566,7 +568,8 @@ int aq_kv8_read(const aq_kv8 *cache, int64_t start, int64_t n, float *k, float *
  * The caller allocates k and v (aq_paged_sizes; device memory, 16-byte aligned, no
  * initial content needed).  Calls on one cache are the caller's to order.  q, k, v
  * and outputs are 16-byte aligned too (AQ_ERR_VALUE).  head_dim 64, 128 or 256,
- * page_size a multiple of 32; width * page_size and start below 2^31 (AQ_ERR_VALUE). */
+ * page_size a multiple of 32; width * page_size below 2^31, and for the attention start
+ * too (AQ_ERR_VALUE). */
 typedef struct aq_paged {
   void *k, *v;      /* [n_pages][n_kv][page_size / 32][32 * head_dim] (aq_paged.hip) */
   int64_t n_pages;
