@@ -1106,6 +1106,9 @@ hipError_t launch_paged_read(int64_t N, const PagedTable &tab, const aq_paged &c
 
 bool attention_paged_fits(const aq_paged &c, int64_t N, int n_head, int64_t width,
                           int64_t start) {
+  // (splits are held below the bound, and the prefix's workgroups are fewer than
+  // N n_head / 16 + n_kv + 512: no plan is made for ordinary calls)
+  if (N * n_head <= 1 << 22) return true;
   const PagedPlan p = paged_plan(c, N, n_head, width, start);
   return (int64_t)p.pre + p.own <= kMaxGrid && (p.states() <= 8 || N * n_head <= kMaxGrid);
 }
