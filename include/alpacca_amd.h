@@ -603,8 +603,9 @@ int aq_rope_paged(const float *q, const float *k, const float *v, float *q_out, 
  * workgroups (AQ_ERR_VALUE: N * n_kv close to 2^24).  Float32 accuracy over the values
  * stored, whatever the size of queries, keys and values, where float32 holds the scores
  * q.k / sqrt(head_dim) (up to 2.3e38) and the sums of e^(score - largest) v; past that, as
- * with an infinity or a NaN among them, a row's outputs may be infinite or NaN.  scratch: at least the bytes that aq_attention_paged_scratch says for the same
- * call, 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
+ * with an infinity or a NaN among them, a row's outputs may be infinite or NaN.
+ * scratch: at least the bytes that aq_attention_paged_scratch says for the same call,
+ * 16-byte aligned; nothing in it outlives the call.  Enqueues only. */
 int aq_attention_paged(const float *q, const aq_paged *cache, int64_t N, int n_head,
                        const int32_t *table, int64_t seqs, int64_t width, const int64_t *seq,
                        const int64_t *pos, const int32_t *prefix, int64_t n_prefix,

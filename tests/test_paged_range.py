@@ -66,7 +66,8 @@ def test_rows_of_different_sizes_together():
 @gpu
 @pytest.mark.parametrize("vscale", [1e-30, 1e10, 1e32, 1e35, 1e36])
 @pytest.mark.parametrize("n_head,n_kv,hd,N,own,start", [
-    (8, 2, 64, 5, 50, 130), (16, 2, 128, 40, 40, 64), (4, 2, 256, 3, 33, 30), (8, 1, 64, 2, 300, 0)])
+    (8, 2, 64, 5, 50, 130), (16, 2, 128, 40, 40, 64), (4, 2, 256, 3, 33, 30),
+    (8, 1, 64, 2, 300, 0)])
 def test_bf16_values_of_any_size(n_head, n_kv, hd, N, own, start, vscale):
     """Values whose weighted sums float32 holds (at most 300 of 4e36 each here)."""
     from tests.test_paged import fill
